@@ -1,0 +1,332 @@
+"""Timed cases of the two operator families a training pass with many classes or large batches uses:
+
+  class_ce   1x1 head + softmax cross entropy over many classes with all its gradients, the logits never kept
+             (ops.class_ce; ops.class_ce_fwd for the loss of each pixel alone)
+  act8       activations kept in 8 bits between forward and backward (ops.act8_pack / act8_unpack), and the backward of
+             BatchNorm + LeakyReLU that reads them (ops.act8_bn_act_bwd)
+
+Each case runs in the operators' plain form (elementary torch operations in fp32), or with `own` set through the package."""
+import math
+
+import torch
+
+own = False
+
+BLOCK = 256          # elements of a plane that share one scale (the format of act8)
+SLOPE = 0.2          # LeakyReLU slope of the networks
+EPS = 1e-5
+
+F32, BF16 = "fp32", "bf16"
+_DT = {F32: torch.float32, BF16: torch.bfloat16}
+
+
+# ----------------------------------------------------------------------------------------------------------------- cases
+def _ce(name, shape, classes, h="fp32", w="fp32", op="class_ce", mean="all"):
+    return {"name": name, "op": op, "shape": "x".join(str(s) for s in shape), "classes": classes, "h": h, "w": w, "mean": mean}
+
+
+def _a8(name, op, shape, dtype="fp32", ref=False):
+    return {"name": name, "op": op, "shape": "x".join(str(s) for s in shape), "dtype": dtype, "ref": ref}
+
+
+def listed():
+    return [
+        # latency: the head of a small crop with a handful of classes, one image
+        _ce("ce_crop", (1, 16, 33, 31), 9),
+        # the narrow network's last block (16 channels) at the benchmark's batch and size, a whole-body label set
+        _ce("ce_pixels16", (16, 16, 256, 256), 104),
+        # the wide network's last block (64 channels) at its own size, an odd class count, mean over the labelled pixels
+        _ce("ce_pixels64", (4, 64, 320, 320), 151, mean="valid"),
+        # the same in bf16 storage (fp32 weights, as everywhere in the package)
+        _ce("ce_pixels64_bf16", (16, 64, 256, 256), 256, h=BF16),
+        # the code z_i (512 channels, 1/16 of the image) classified into a codebook's entries
+        _ce("ce_code512", (16, 512, 16, 16), 8192),
+        # rows of features against a large vocabulary, all bf16: the largest product
+        _ce("ce_rows_bf16", (6400, 512), 32768, h=BF16, w=BF16),
+        # the loss of every pixel alone and its log-sum (hard-pixel selection, validation)
+        _ce("nll_pixels64", (8, 64, 192, 192), 1000, op="class_nll"),
+        _ce("nll_rows_bf16", (1000, 512), 32001, h=BF16, w=BF16, op="class_nll"),
+        # a checkpoint written and read back: the widest activation of a pass, raw convolution output
+        _a8("act8_keep", "act8_keep", (16, 64, 256, 256)),
+        _a8("act8_keep_odd_bf16", "act8_keep", (3, 48, 77, 91), BF16),
+        # BatchNorm + LeakyReLU backward out of a checkpoint: the widest activation; a residual block's deepest one, whose mask is its output's sign
+        _a8("act8_bwd", "act8_bwd", (16, 64, 256, 256)),
+        _a8("act8_bwd_deep_ref", "act8_bwd", (4, 128, 12, 12), ref=True),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    kind = rng.choice(["class_ce", "class_ce", "class_ce", "class_nll", "act8_keep", "act8_bwd", "act8_bwd"])
+    if kind.startswith("class"):
+        while True:
+            h = rng.choice([F32, BF16])
+            w = rng.choice([F32, BF16]) if h == BF16 else F32
+            if rng.random() < 0.6:                       # pixels: narrow features, up to about a thousand classes
+                side = _log(rng, 7, 320)
+                shape = (_log(rng, 1, 16), rng.choice([16, 32, 64, _log(rng, 8, 128)]), side, side + rng.randint(0, 9))
+                classes = _log(rng, 5, 1200)
+            else:                                        # codes / rows: wide features, large vocabularies
+                c = rng.choice([256, 512, _log(rng, 100, 640)])
+                rows = _log(rng, 1, 8192)
+                shape = (rows, c) if rng.random() < 0.5 else (max(1, rows // 256), c, 16, 16 + rng.randint(0, 4))
+                classes = _log(rng, 500, 40000)
+            n = math.prod(shape) // shape[1]
+            if n * shape[1] * classes <= 6400 * 512 * 32768 and n * (shape[1] + classes) <= 16 * 256 * 256 * 330:
+                return {"op": kind, "shape": "x".join(str(s) for s in shape), "classes": classes, "h": h, "w": w, "mean": rng.choice(["all", "valid"])}
+    while True:
+        side = _log(rng, 5, 330)
+        shape = (_log(rng, 1, 16), _log(rng, 4, 256), side, side + rng.randint(0, 7))
+        if math.prod(shape) <= 16 * 64 * 256 * 256:
+            return {"op": kind, "shape": "x".join(str(s) for s in shape), "dtype": rng.choice([F32, F32, BF16]), "ref": kind == "act8_bwd" and rng.random() < 0.5}
+
+
+def _shape(case):
+    return tuple(int(s) for s in case["shape"].split("x"))
+
+
+# ----------------------------------------------------------------------------------------------------------------- inputs
+def _leaky(x):
+    return torch.where(x > 0, x, x * SLOPE)
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed * 1000003 + 17)
+    shape = _shape(case)
+
+    def randn(*s):
+        return torch.randn(*s, generator=gen, device="cuda")
+
+    if case["op"].startswith("class"):
+        n, c, sp, v = shape[0], shape[1], shape[2:], case["classes"]
+        w = randn(v, c) * (1.6 / math.sqrt(c))
+        b = randn(v) * 0.3
+        lab = torch.randint(0, v, (n, *sp), generator=gen, device="cuda")
+        # features of a partly trained network: noise through the activation, drawn towards the weights of the pixel's class
+        pull = w[lab.reshape(n, -1)].transpose(1, 2) if sp else w[lab]
+        h = _leaky(randn(*shape) + 0.8 * pull.reshape(shape))
+        void = torch.rand(n, *sp, generator=gen, device="cuda") < 0.05          # unlabelled pixels
+        lab = torch.where(void, torch.full_like(lab, 255 if v <= 255 else -100), lab)
+        return {"op": case["op"], "h": h.to(_DT[case["h"]]).contiguous(), "w": w.to(_DT[case["w"]]), "b": b, "lab": lab.contiguous(), "mean": case["mean"]}
+
+    n, c, hh, ww = shape
+    dt = _DT[case["dtype"]]
+    u = (randn(*shape) * (0.5 + torch.rand(1, c, 1, 1, generator=gen, device="cuda")) + randn(1, c, 1, 1)).to(dt)
+    gamma = 0.5 + torch.rand(c, generator=gen, device="cuda")
+    beta = randn(c) * 0.3
+    uf = u.float()
+    mean = uf.mean((0, 2, 3))
+    inv = 1.0 / torch.sqrt(((uf - mean.view(1, c, 1, 1)) ** 2).mean((0, 2, 3)) + EPS)
+    scale = gamma * inv
+    coef = torch.stack([scale, beta - mean * scale, mean, inv], 1).contiguous()
+    if case["op"] == "act8_keep":
+        return {"op": case["op"], "x": u, "coef": coef}
+    state = {"op": case["op"], "coef": coef, "ref": None, "dtype": dt}
+    state["g"] = (randn(*shape) * 0.01).to(dt)
+    state["q"], state["s"] = _pack(uf, coef)
+    if case["ref"]:
+        out = _leaky(uf * scale.view(1, c, 1, 1) + coef[:, 1].view(1, c, 1, 1) + randn(*shape))
+        state["ref"] = _pack(out, None)[0]
+    return state
+
+
+# ----------------------------------------------------------------------------------------------------------------- plain form
+def _centre(coef):
+    """The zero of the BatchNorm's output where it lies within four standard deviations of the mean, else the mean; and which of the two."""
+    scale, shift, mean, inv = coef.double().unbind(1)
+    t = -shift / scale
+    at_zero = ((t - mean).abs() * inv) <= 4.0
+    return torch.where(at_zero, t, mean), at_zero
+
+
+def _pack(x, coef):
+    # (64 bits: a value next to the border of two steps has to fall on the same side everywhere)
+    n, c = x.shape[:2]
+    d = x.double().reshape(n, c, -1)
+    if coef is not None:
+        d = d - _centre(coef)[0].view(1, c, 1)
+    hw = d.shape[2]
+    nb = (hw + BLOCK - 1) // BLOCK
+    d = torch.cat([d, d.new_zeros(n, c, nb * BLOCK - hw)], 2).view(n, c, nb, BLOCK)
+    s = d.abs().amax(3).float() / 127.0
+    q = torch.round(d / s.double().unsqueeze(3))
+    q = torch.where((q == 0) & (d != 0), torch.sign(d), q)
+    q = q.view(n, c, nb * BLOCK)[:, :, :hw].to(torch.int8).reshape(x.shape).contiguous()
+    return q, s
+
+
+def _kept(q, s, coef):
+    """The values a checkpoint stands for."""
+    n, c = q.shape[:2]
+    hw = q[0, 0].numel()
+    d = q.reshape(n, c, hw).double() * s.double().repeat_interleave(BLOCK, 2)[:, :, :hw]
+    if coef is not None:
+        d = d + _centre(coef)[0].view(1, c, 1)
+    return d.reshape(q.shape)
+
+
+def _plain_ce(h, w, b, lab, mean, need_grad):
+    n, c = h.shape[:2]
+    v = w.shape[0]
+    x = h.float().reshape(n, c, -1).transpose(1, 2).reshape(-1, c)
+    y = lab.reshape(-1)
+    wf = w.float()
+    z = torch.matmul(x, wf.t()) + b
+    m = z.amax(1, keepdim=True)
+    e = torch.exp(z - m)
+    total = e.sum(1, keepdim=True)
+    ok = (y >= 0) & (y < v)
+    pick = z.gather(1, torch.where(ok, y, torch.zeros_like(y)).unsqueeze(1))
+    nll = torch.where(ok, ((m - pick) + torch.log(total)).squeeze(1), torch.zeros_like(total.squeeze(1)))
+    if not need_grad:
+        return nll.view(lab.shape), (m + torch.log(total)).view(lab.shape)
+    scale = 1.0 / (ok.sum().float() if mean == "valid" else float(y.numel()))
+    loss = nll.sum() * scale
+    g = e / total
+    hot = torch.arange(v, device=z.device).unsqueeze(0) == y.unsqueeze(1)
+    g = torch.where(ok.unsqueeze(1), (g - hot.float()) * scale, torch.zeros_like(g))
+    dh = torch.matmul(g, wf).view(n, -1, c).transpose(1, 2).reshape(h.shape)
+    dw = torch.matmul(g.t(), x)
+    return loss, dh.to(h.dtype), dw.to(w.dtype), g.sum(0)
+
+
+def _plain_bwd(st):
+    coef, q, s = st["coef"], st["q"], st["s"]
+    n, c = q.shape[:2]
+    x = _kept(q, s, coef)
+    per = lambda t: t.view(1, c, 1, 1)
+    scale, shift, mean, inv = coef.unbind(1)
+    if st["ref"] is not None:
+        on = st["ref"] > 0
+    else:
+        # a checkpoint centred on the BatchNorm's zero holds the sign of its output exactly
+        at_zero = _centre(coef)[1]
+        on = torch.where(per(at_zero), q.float() * per(torch.sign(scale)) > 0, x * per(scale.double()) + per(shift.double()) > 0)
+    g = st["g"].float()
+    g = torch.where(on, g, g * SLOPE)
+    xm = (x - per(mean.double())).float()
+    s1, s2 = g.double().sum((0, 2, 3)), (g * xm).double().sum((0, 2, 3))
+    m = float(g.numel() // c)
+    du = per(scale) * (g - per((s1 / m).float()) - xm * per((inv.double() * inv.double() * s2 / m).float()))
+    return du.to(st["dtype"]), (s2 * inv.double()).float(), s1.float()
+
+
+def run(state):
+    op = state["op"]
+    if own:
+        from maxstyle_amd import ops
+        if op == "class_ce":
+            return ops.class_ce(state["h"], state["w"], state["b"], state["lab"], mean_over=state["mean"])
+        if op == "class_nll":
+            return ops.class_ce_fwd(state["h"], state["w"], state["b"], state["lab"])
+        if op == "act8_keep":
+            q, s = ops.act8_pack(state["x"], state["coef"])
+            return ops.act8_unpack(q, s, state["coef"], dtype=state["x"].dtype), s
+        return ops.act8_bn_act_bwd(state["g"], state["q"], state["s"], state["coef"], SLOPE, ref_q=state["ref"])
+    if op == "class_ce":
+        return _plain_ce(state["h"], state["w"], state["b"], state["lab"], state["mean"], True)
+    if op == "class_nll":
+        return _plain_ce(state["h"], state["w"], state["b"], state["lab"], state["mean"], False)
+    if op == "act8_keep":
+        q, s = _pack(state["x"], state["coef"])
+        return _kept(q, s, state["coef"]).to(state["x"].dtype), s
+    return _plain_bwd(state)
+
+
+# ----------------------------------------------------------------------------------------------------------------- work
+def work(case):
+    shape = _shape(case)
+    n = math.prod(shape)
+    size = {F32: 4, BF16: 2}
+    if case["op"].startswith("class"):
+        c, v = shape[1], case["classes"]
+        rows = n // c
+        hb, wb = n * size[case["h"]], v * c * size[case["w"]]
+        if case["op"] == "class_nll":
+            return {"bytes": hb + wb + 4 * v + 16 * rows, "flops": 2 * rows * v * c}
+        return {"bytes": 2 * hb + 2 * wb + 8 * v + 8 * rows, "flops": 6 * rows * v * c}
+    e = size[case["dtype"]]
+    if case["op"] == "act8_keep":
+        return {"bytes": n * (e + 1 + 1 + e), "flops": 6 * n}
+    return {"bytes": n * (e + 1 + e + (1 if case["ref"] else 0)), "flops": 12 * n}
+
+
+# ----------------------------------------------------------------------------------------------------------------- exact
+def _exact_ce(st, grad):
+    h, w, b, lab = st["h"].double(), st["w"].double(), st["b"].double(), st["lab"]
+    rows = h.movedim(1, -1).reshape(-1, h.shape[1])
+    target = lab.reshape(-1)
+    classes = w.shape[0]
+    valid = (target >= 0) & (target < classes)
+    norm = float(valid.sum()) if st["mean"] == "valid" else float(target.numel())
+    dw, db = torch.zeros_like(w), torch.zeros_like(b)
+    dx, nll = torch.zeros_like(rows), torch.zeros(rows.shape[0], dtype=torch.float64, device=h.device)
+    lse = torch.zeros_like(nll)
+    step = max(1, (1 << 27) // classes)
+    for i in range(0, rows.shape[0], step):
+        r, k = rows[i:i + step], valid[i:i + step]
+        z = r @ w.T + b
+        lse[i:i + step] = torch.logsumexp(z, 1)
+        logp = z - lse[i:i + step].unsqueeze(1)
+        pos = torch.nonzero(k)[:, 0]
+        t = target[i:i + step][pos]
+        nll[i:i + step][pos] = -logp[pos, t]
+        if grad:
+            p = torch.exp(logp)
+            p[pos, t] -= 1.0
+            p = p * (k.double() / norm).unsqueeze(1)
+            dx[i:i + step] = p @ w
+            dw += p.T @ r
+            db += p.sum(0)
+    if not grad:
+        return nll.reshape(lab.shape), lse.reshape(lab.shape)
+    dh = dx.reshape(h.shape[0], *h.shape[2:], h.shape[1]).movedim(-1, 1).contiguous()
+    return nll.sum() / norm, dh, dw, db
+
+
+def _exact_keep(st):
+    x, coef = st["x"].double(), st["coef"].double()
+    n, c = x.shape[:2]
+    zero = -coef[:, 1] / coef[:, 0]
+    mid = torch.where(((zero - coef[:, 2]) * coef[:, 3]).abs() <= 4, zero, coef[:, 2])[None, :, None]
+    planes = x.reshape(n, c, -1)
+    out, scales = torch.empty_like(planes), []
+    for i in range(0, planes.shape[2], BLOCK):
+        d = planes[:, :, i:i + BLOCK] - mid
+        s = (d.abs().amax(2, keepdim=True).float() / 127).double()          # the format keeps scales in fp32
+        k = torch.round(d / s)
+        k = torch.where(k == 0, torch.sign(d), k)
+        out[:, :, i:i + BLOCK] = mid + k * s
+        scales.append(s[:, :, 0])
+    return out.reshape(x.shape), torch.stack(scales, 2)
+
+
+def _exact_bwd(st):
+    coef, q = st["coef"].double(), st["q"]
+    n, c = q.shape[:2]
+    a, sh, mean, inv = (coef[:, i].reshape(1, c, 1) for i in range(4))
+    zero = -sh / a
+    at_zero = ((zero - mean) * inv).abs() <= 4
+    planes = q.reshape(n, c, -1).double()
+    idx = torch.arange(planes.shape[2], device=q.device) // BLOCK
+    d = planes * st["s"].double()[:, :, idx]
+    x = d + torch.where(at_zero, zero, mean)
+    z = torch.where(at_zero, a * d, a * x + sh) if st["ref"] is None else st["ref"].reshape(n, c, -1).double()
+    g = st["g"].double().reshape(n, c, -1) * torch.where(z > 0, 1.0, SLOPE)
+    count = n * planes.shape[2]
+    xhat = (x - mean) * inv
+    dbeta, dgamma = g.sum((0, 2)), (g * xhat).sum((0, 2))
+    du = a * (g - dbeta[None, :, None] / count - xhat * dgamma[None, :, None] / count)
+    return du.reshape(q.shape), dgamma, dbeta
+
+
+def exact(case, seed):
+    st = prepare(case, seed)
+    if case["op"] == "act8_keep":
+        return _exact_keep(st)
+    if case["op"] == "act8_bwd":
+        return _exact_bwd(st)
+    return _exact_ce(st, case["op"] == "class_ce")
