@@ -151,7 +151,7 @@ def _pack(x, coef):
     hw = d.shape[2]
     nb = (hw + BLOCK - 1) // BLOCK
     d = torch.cat([d, d.new_zeros(n, c, nb * BLOCK - hw)], 2).view(n, c, nb, BLOCK)
-    s = d.abs().amax(3).float() / 127.0
+    s = (d.abs().amax(3).float().double() / 127.0).float()
     q = torch.round(d / s.double().unsqueeze(3))
     q = torch.where((q == 0) & (d != 0), torch.sign(d), q)
     q = q.view(n, c, nb * BLOCK)[:, :, :hw].to(torch.int8).reshape(x.shape).contiguous()
@@ -296,7 +296,7 @@ def _exact_keep(st):
     out, scales = torch.empty_like(planes), []
     for i in range(0, planes.shape[2], BLOCK):
         d = planes[:, :, i:i + BLOCK] - mid
-        s = (d.abs().amax(2, keepdim=True).float() / 127).double()          # the format keeps scales in fp32
+        s = (d.abs().amax(2, keepdim=True).float().double() / 127).float().double()          # the format keeps the largest and the scale in fp32
         k = torch.round(d / s)
         k = torch.where(k == 0, torch.sign(d), k)
         out[:, :, i:i + BLOCK] = mid + k * s
