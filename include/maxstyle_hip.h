@@ -571,6 +571,51 @@ MS_STABLE int ms_head_ce(const float* h, const float* w, const float* b, const i
 MS_STABLE int ms_head_ce_ds(const float* h, const float* w, const float* b, const int64_t* labels, float* dh, float* logits, float* loss_out,
                   const int* loss_slot_dev, int N, int C, int K, int HW, float loss_sign, const float* grad_scale_dev, void* ws, size_t ws_bytes, void* stream);
 
+/* ---- head + softmax cross entropy over MANY classes, the logits never kept ------------------------------------------------------------------------
+ * ms_head_ce's operator without its limits (K <= 4, C <= 64), with all gradients in the one call:
+ *   z[p,v] = sum_c w[v,c] h[p,c] + b[v];  lse[p] = log sum_v exp z[p,v];  nll[p] = lse[p] - z[p,labels[p]], 0 where the label is outside [0,V)
+ *   loss = loss_sign * sum_p nll / (N*HW, or with mean_valid the rows whose label is a class; no such row: loss and gradients are 0)   (custom_loss.py:1043-1078)
+ *   dh = d loss/d h, dw = d loss/d w, db = d loss/d b, times *grad_scale_dev (NULL: 1); each may be NULL.
+ * h [N][C][HW] (rows of features [T][C]: N = T, HW = 1), w [V][C], b [V] or NULL, labels [N][HW]; dh like h, dw like w.  types: bit 0 h / dh are bf16, bit 1 w / dw
+ * are bf16, otherwise fp32; b, db, loss, nll, lse are fp32.  Up to 8192 channels, 2^20 classes, 2^30 rows.  A row whose label is not a class gives nothing to the
+ * loss and exactly 0 to every gradient, whatever its features hold; b may be -infinity for classes that are switched off.
+ * ms_class_ce_fwd: nll and lse of every row, ms_class_ce_bwd: the gradients for an upstream gradient of every row (grad [N][HW]) and the lse of that forward.
+ * Deterministic.  ws: ms_class_ce_ws_bytes(.., need_grad = 1 when any gradient is asked for), 16-byte aligned, free again when the stream has passed the call. */
+MS_STABLE size_t ms_class_ce_ws_bytes(int N, int C, int V, int HW, int types, int need_grad);
+MS_STABLE int ms_class_ce(const void* h, const void* w, const float* b, const int64_t* labels, float* loss_out, void* dh, void* dw, float* db, int N, int C, int V, int HW,
+                int types, float loss_sign, int mean_valid, const float* grad_scale_dev, void* ws, size_t ws_bytes, void* stream);
+MS_STABLE int ms_class_ce_fwd(const void* h, const void* w, const float* b, const int64_t* labels, float* nll, float* lse, int N, int C, int V, int HW, int types,
+                    void* ws, size_t ws_bytes, void* stream);
+MS_STABLE int ms_class_ce_bwd(const void* h, const void* w, const float* b, const int64_t* labels, const float* lse, const float* grad, void* dh, void* dw, float* db,
+                    int N, int C, int V, int HW, int types, void* ws, size_t ws_bytes, void* stream);
+
+/* ---- activation checkpoints in 8 bits ---------------------------------------------------------------------------------------------------------------
+ * A plane (n,c) of x [N][C][HW] in blocks of ms_act8_block() = 256 elements (the last may be shorter): with d = x - centre_c,
+ *   s = max|d| / 127 (fp32), q = rint(d / s), and the sign of d where that is 0 although d is not;  x' = centre_c + q s.       q [N][C][HW], s [N][C][ceil(HW/256)]
+ * coef4 (NULL: centre 0) is a BatchNorm record of ms_bn_finalize {scale, shift, mean, invstd} per channel: centre_c = -shift/scale where that lies within 4 standard
+ * deviations of the mean, else the mean - the sign of scale x + shift is then kept exactly.  A block below 2^-120 is kept as zeros, one with an infinity or NaN
+ * reads back as NaN.
+ *   ms_act8_bwd_reduce   ms_act_bwd_reduce out of a checkpoint: g' = g * (r > 0 ? 1 : slope), r = ref_q (the checkpoint, without a record, of the saved activation
+ *                        output: only its signs are read) or scale x' + shift when ref_q == NULL; part2 [C][ms_act8_bwd_parts()][2] = {sum g', sum g'(x' - mean)} for
+ *                        ms_bn_bwd_full; gout (g', may alias gin) and uout (x') may be NULL.  coef4 must be the record the checkpoint was made with.
+ *   ms_act8_bn_act_bwd   the whole backward of BatchNorm (batch statistics) + LeakyReLU: du, dgamma, dbeta (may not be NULL; du may alias g).
+ * Deterministic; any alignment and any HW. */
+MS_STABLE int ms_act8_block(void);
+MS_STABLE int ms_act8_pack(const float* x, const float* coef4, int8_t* q, float* s, int N, int C, int HW, void* stream);
+MS_STABLE int ms_act8_unpack(const int8_t* q, const float* s, const float* coef4, float* x, int N, int C, int HW, void* stream);
+MS_STABLE int ms_act8_bwd_parts(int N, int C, int HW);
+MS_STABLE int ms_act8_bwd_reduce(const float* gin, const int8_t* ref_q, const int8_t* q, const float* s, const float* coef4, float* gout, float* uout, float* part2,
+                       int N, int C, int HW, float slope, void* stream);
+MS_STABLE size_t ms_act8_bwd_ws_bytes(int N, int C, int HW);
+MS_STABLE int ms_act8_bn_act_bwd(const float* g, const int8_t* ref_q, const int8_t* q, const float* s, const float* coef4, float* du, float* dgamma, float* dbeta,
+                       int N, int C, int HW, float slope, void* ws, size_t ws_bytes, void* stream);
+MS_STABLE int ms_act8_pack_bf16(const uint16_t* x, const float* coef4, int8_t* q, float* s, int N, int C, int HW, void* stream);
+MS_STABLE int ms_act8_unpack_bf16(const int8_t* q, const float* s, const float* coef4, uint16_t* x, int N, int C, int HW, void* stream);
+MS_STABLE int ms_act8_bwd_reduce_bf16(const uint16_t* gin, const int8_t* ref_q, const int8_t* q, const float* s, const float* coef4, uint16_t* gout, uint16_t* uout, float* part2,
+                            int N, int C, int HW, float slope, void* stream);
+MS_STABLE int ms_act8_bn_act_bwd_bf16(const uint16_t* g, const int8_t* ref_q, const int8_t* q, const float* s, const float* coef4, uint16_t* du, float* dgamma, float* dbeta,
+                            int N, int C, int HW, float slope, void* ws, size_t ws_bytes, void* stream);
+
 /* ---- bf16 ACTIVATION STORAGE for the conv stack (SURVEY.md 8(b) "`_bf16` I/O variants with fp32 statistics") -----------------
  * Twins of the fp32 entry points above with the same argument lists and semantics; every ACTIVATION tensor (conv inputs / outputs, raw conv
  * outputs u, gradients, residuals, head inputs / outputs) is a tensor of bf16 bit patterns (uint16_t), everything else - packed weights, biases,

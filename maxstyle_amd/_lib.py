@@ -158,10 +158,23 @@ SIGNATURES = {
     "ms_head_ce_ws_bytes": (c_size, [c_int, c_int]),
     "ms_head_ce": (c_int, [c_f32p, c_f32p, c_f32p, c_i64p, c_f32p, c_f32p, c_f32p, c_void, c_int, c_int, c_int, c_int, c_float,
                            c_void, c_size, c_void]),
+    "ms_class_ce_ws_bytes": (c_size, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    "ms_class_ce": (c_int, [c_void, c_void, c_f32p, c_i64p, c_f32p, c_void, c_void, c_f32p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_f32p, c_void, c_size, c_void]),
+    "ms_class_ce_fwd": (c_int, [c_void, c_void, c_f32p, c_i64p, c_f32p, c_f32p, c_int, c_int, c_int, c_int, c_int, c_void, c_size, c_void]),
+    "ms_class_ce_bwd": (c_int, [c_void, c_void, c_f32p, c_i64p, c_f32p, c_f32p, c_void, c_void, c_f32p, c_int, c_int, c_int, c_int, c_int, c_void, c_size, c_void]),
+    "ms_act8_block": (c_int, []),
+    "ms_act8_pack": (c_int, [c_f32p, c_f32p, c_void, c_f32p, c_int, c_int, c_int, c_void]),
+    "ms_act8_unpack": (c_int, [c_void, c_f32p, c_f32p, c_f32p, c_int, c_int, c_int, c_void]),
+    "ms_act8_bwd_parts": (c_int, [c_int, c_int, c_int]),
+    "ms_act8_bwd_reduce": (c_int, [c_f32p, c_void, c_void, c_f32p, c_f32p, c_f32p, c_f32p, c_f32p, c_int, c_int, c_int, c_float, c_void]),
+    "ms_act8_bwd_ws_bytes": (c_size, [c_int, c_int, c_int]),
+    "ms_act8_bn_act_bwd": (c_int, [c_f32p, c_void, c_void, c_f32p, c_f32p, c_f32p, c_f32p, c_f32p, c_int, c_int, c_int, c_float, c_void, c_size, c_void]),
 }
 # bf16 activation storage for the conv stack: same argument lists as the fp32 entry points (device pointers travel as integers either way)
 for _n in ("ms_conv2d", "ms_conv2d_ride", "ms_conv2d_xfin", "ms_conv2d_actbwd_xfin", "ms_conv1x1_bnres", "ms_conv1x1_bnres_xfin", "ms_conv2d_actbwd", "ms_bn_act", "ms_bn_finalize_act", "ms_act_bwd_reduce", "ms_pool2_sum", "ms_pool2_actbwd", "ms_pool2_actbwd_pool", "ms_add_actbwd",
            "ms_head_fwd", "ms_head_fwd_styled", "ms_head_bwd", "ms_head_ce", "ms_head_ce_actbwd", "ms_head_ce_tail", "ms_conv_subpix", "ms_conv3x3_small_cout", "ms_conv3x3_small_cin", "ms_style_bwd_actbwd", "ms_style_bwd_actbwd_parts"):
+    SIGNATURES[_n + "_bf16"] = SIGNATURES[_n]
+for _n in ("ms_act8_pack", "ms_act8_unpack", "ms_act8_bwd_reduce", "ms_act8_bn_act_bwd"):
     SIGNATURES[_n + "_bf16"] = SIGNATURES[_n]
 for _n in ("ms_conv2d", "ms_conv2d_actbwd"):           # bf16 storage + bf16 matrix arithmetic (v_mfma_f32_16x16x16_bf16) where built
     SIGNATURES[_n + "_bf16m"] = SIGNATURES[_n]

@@ -1,0 +1,41 @@
+// Head + softmax cross entropy over many classes: shared definitions of the wide (matrix-product) and narrow (one-pass) forms.
+//
+//   z[p,v] = sum_c w[v,c] h[p,c] + b[v]      p = (n, hw): a pixel or row, P = N HW of them; V classes
+//   lse[p] = log sum_v exp z;  nll[p] = lse[p] - z[p,y_p] (0 where y_p is outside [0,V): the row takes no part)
+//   G[p,v] = g_p (exp(z - lse) - [v = y_p]);  dh[p,:] = sum_v G w[v,:];  dw[v,:] = sum_p G h[p,:];  db[v] = sum_p G
+//
+// Numbers on the matrix cores.  Products run on v_mfma_f32_16x16x32_f16 with fp32 accumulation.  Every row of h and of w is scaled by a power of two of its own
+// (ex[p], ew[v]: exact, put back in the epilogue) so that its largest element lies in [2^13, 2^14), then split into fp16 planes: an fp32 value into two
+// (11 + 11 bits, x = hi + lo to 2^-22 relative or 2^-39 of the row's largest), a bf16 value (8 bits) into one, exactly down to 2^-37 of the row's largest.
+// A product of two-plane operands is hi hi + hi lo + lo hi (lo lo is below 2^-22): three matrix instructions for fp32 x fp32, two for bf16 x fp32, one for
+// bf16 x bf16.  fp32's own matrix instruction does 1/16 of the fp16 rate, so three of these are 5 times its speed at its accuracy.
+#pragma once
+#include "ms_common.h"
+
+namespace ms {
+
+typedef _Float16 ms_h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 ms_h4 __attribute__((ext_vector_type(4)));
+typedef short ms_s4 __attribute__((ext_vector_type(4)));
+typedef float ms_f4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kCeTopExp = 13;         // scaled rows: largest magnitude in [2^13, 2^14)
+constexpr int kCePad = 256;           // rows of the packed operands are padded to whole tiles
+
+// the power of two that brings `amax` to [2^13, 2^14); 1 for a row of zeros or one with an infinity / NaN (it stays one), no smaller than 2^-100
+__device__ __forceinline__ int ce_exponent(float amax) {
+  const unsigned b = __float_as_uint(amax);
+  if (b >= 0x7F800000u || b == 0u) return 0;
+  const int e = (int)(b >> 23) - 127;                 // (a subnormal reads as -127: the clamp below)
+  return max(e - kCeTopExp, -100);
+}
+__device__ __forceinline__ float ce_pow2(int e) { return __uint_as_float((unsigned)(min(max(e, -126), 127) + 127) << 23); }
+
+// {hi, lo} planes of a scaled value
+__device__ __forceinline__ void ce_split(float x, _Float16& hi, _Float16& lo) {
+  hi = (_Float16)x;
+  lo = (_Float16)(x - (float)hi);
+}
+
+}  // namespace ms

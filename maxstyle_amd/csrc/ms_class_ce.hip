@@ -1,0 +1,628 @@
+// Head + softmax cross entropy over many classes, wide form: three matrix products (logits, dh, dw) over pieces of (rows x classes); see ms_class_ce.h.
+//
+// Passes of one training call (all on the caller's stream, nothing allocated, no atomics on floats):
+//   pack w, pack h      fp16 planes [rows][channels], power-of-two scales, padded to whole tiles
+//   logits -> stats     tile of z stays in registers: (max, sum exp) of each row and class tile, and the label's own z
+//   join                lse and nll of every row, loss in 64 bits
+//   per piece           G (logits again, written as fp16 planes), dh += G w, dw += G^T h; db from G's epilogue
+// The logits are never written; G exists for one piece at a time (kCePieceBytes: it stays in the 256 MB last-level cache between its writer and its two readers).
+#include <algorithm>
+#include "ms_class_ce.h"
+#include "maxstyle_hip.h"
+
+namespace ms {
+
+constexpr size_t kCePieceBytes = (size_t)96 << 20;
+
+// ------------------------------------------------------------------------------------------------------------------------------ small passes
+// scal[0]: rows that take part; scal[1]: max over rows of exponent(g_p) + ex[p]; scal[2]: max over classes of ew[v]   (integers: their order does not matter)
+__global__ void ce_init_kernel(int* scal) {
+  if (threadIdx.x == 0) { scal[0] = 0; scal[1] = -100000; scal[2] = -100000; }
+}
+
+// w [V][C] -> planes [Vp][Cp], fw[v] = 2^ew, bpad[v] = b or -inf behind the last class.  One wave a row.
+template <typename WT, int PL>
+__global__ __launch_bounds__(256) void ce_pack_rows_kernel(const void* __restrict__ w, const float* __restrict__ b, const int64_t* __restrict__ labels, int classes,
+                                                           _Float16* __restrict__ out, size_t plane, float* __restrict__ fw, float* __restrict__ bpad,
+                                                           int* __restrict__ lab32, int* __restrict__ scal, int rows, int rows_pad, int C, int Cp) {
+  // labels != nullptr: the rows are features, one that takes no part is packed as zeros (its h may hold anything); otherwise weights
+  using IO = ActIO<WT>;
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (r >= rows_pad) return;
+  bool live = r < rows;
+  if (labels != nullptr) {
+    int y = -1;
+    if (live) { const int64_t l = labels[r]; y = (l >= 0 && l < classes) ? (int)l : -1; }
+    live = y >= 0;
+    if (lane == 0) lab32[r] = y;
+  }
+  unsigned am = 0;
+  if (live) for (int c = lane; c < C; c += 64) am = max(am, __float_as_uint(IO::ld1(w, (size_t)r * C + c)) & 0x7FFFFFFFu);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) am = max(am, (unsigned)__shfl_xor((int)am, off, 64));
+  const int e = ce_exponent(__uint_as_float(am));
+  const float inv = ce_pow2(-e);
+  if (lane == 0) {
+    fw[r] = ce_pow2(e);
+    if (bpad != nullptr) bpad[r] = r < rows ? (b != nullptr ? b[r] : 0.f) : -__builtin_inff();
+    if (bpad != nullptr && r < rows) atomicMax(&scal[2], e);
+  }
+  for (int c = lane; c < Cp; c += 64) {
+    const float v = (live && c < C) ? IO::ld1(w, (size_t)r * C + c) * inv : 0.f;
+    _Float16 hi, lo;
+    ce_split(v, hi, lo);
+    out[(size_t)r * Cp + c] = hi;
+    if (PL == 2) out[plane + (size_t)r * Cp + c] = lo;
+  }
+}
+
+// h [N][C][HW] -> the same packed rows: a workgroup turns 64 pixels x 64 channels at a time through LDS (reads run along HW, writes along C).
+template <typename HT, int PL>
+__global__ __launch_bounds__(256) void ce_pack_planes_kernel(const void* __restrict__ h, const int64_t* __restrict__ labels, int classes, int drop, _Float16* __restrict__ out,
+                                                             size_t plane, float* __restrict__ fx, int* __restrict__ lab32, long P, long Pp, int C, int Cp, int HW) {
+  using IO = ActIO<HT>;
+  __shared__ _Float16 t[PL][64][64 + 8];
+  __shared__ unsigned smax[4][64];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const long p = (long)blockIdx.x * 64 + lane;
+  bool live = p < P;
+  if (labels != nullptr) {
+    int y = -1;
+    if (live) { const int64_t l = labels[p]; y = (l >= 0 && l < classes) ? (int)l : -1; }
+    if (wave == 0 && p < Pp) lab32[p] = y;
+    if (drop) live = y >= 0;
+  }
+  const long n = p / HW;
+  const size_t base = (size_t)n * C * HW + (size_t)(p - n * HW);
+  unsigned am = 0;
+  if (live) for (int c = wave; c < C; c += 4) am = max(am, __float_as_uint(IO::ld1(h, base + (size_t)c * HW)) & 0x7FFFFFFFu);
+  smax[wave][lane] = am;
+  __syncthreads();
+  am = max(max(smax[0][lane], smax[1][lane]), max(smax[2][lane], smax[3][lane]));
+  const int e = ce_exponent(__uint_as_float(am));
+  const float inv = ce_pow2(-e);
+  if (wave == 0 && p < Pp) fx[p] = ce_pow2(e);
+  for (int c0 = 0; c0 < Cp; c0 += 64) {
+    __syncthreads();
+    for (int c = wave; c < 64; c += 4) {
+      const float v = (live && c0 + c < C) ? IO::ld1(h, base + (size_t)(c0 + c) * HW) * inv : 0.f;
+      _Float16 hi, lo;
+      ce_split(v, hi, lo);
+      t[0][lane][c] = hi;
+      if (PL == 2) t[1][lane][c] = lo;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 64 * 8 * PL; i += 256) {
+      const int pl = i >> 9, row = (i >> 3) & 63, ch = (i & 7) * 8;
+      const long pr = (long)blockIdx.x * 64 + row;
+      if (pr < Pp) *reinterpret_cast<ms_h8*>(out + pl * plane + (size_t)pr * Cp + c0 + ch) = *reinterpret_cast<const ms_h8*>(&t[pl][row][ch]);
+    }
+  }
+}
+
+// rows that take part (for the mean over them)
+__global__ __launch_bounds__(256) void ce_count_kernel(const int64_t* __restrict__ labels, long P, int classes, int* __restrict__ scal) {
+  int k = 0;
+  for (long p = (long)blockIdx.x * 256 + threadIdx.x; p < P; p += (long)gridDim.x * 256) { const int64_t l = labels[p]; k += (l >= 0 && l < classes) ? 1 : 0; }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) k += __shfl_xor(k, off, 64);
+  if ((threadIdx.x & 63) == 0 && k) atomicAdd(&scal[0], k);
+}
+
+// The upstream gradient of every row: grad[p], or sign / rows (rows that take part) times *scale_dev; 0 where the label is not a class.
+__global__ __launch_bounds__(256) void ce_rowgrad_kernel(const float* __restrict__ grad, float sign, int mean_valid, const float* __restrict__ scale_dev, const int* __restrict__ lab32,
+                                                         const float* __restrict__ fx, float* __restrict__ gp, const float* __restrict__ lse_in, float* __restrict__ lse,
+                                                         int* __restrict__ scal, long P, long Pp) {
+  int e = -100000;
+  for (long p = (long)blockIdx.x * 256 + threadIdx.x; p < Pp; p += (long)gridDim.x * 256) {
+    float g = 0.f;
+    if (p < P && lab32[p] >= 0) {
+      if (grad != nullptr) g = grad[p];
+      else g = sign / (float)(mean_valid ? max(scal[0], 1) : P) * (scale_dev != nullptr ? *scale_dev : 1.f);
+      const unsigned b = __float_as_uint(g) & 0x7FFFFFFFu;
+      if (b != 0u && b < 0x7F800000u) e = max(e, (int)(b >> 23) - 126 + (int)(__float_as_uint(fx[p]) >> 23) - 127);
+    }
+    gp[p] = g;
+    if (lse_in != nullptr) lse[p] = p < P ? lse_in[p] : 0.f;        // (the caller's has no padding)
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) e = max(e, __shfl_xor(e, off, 64));
+  if ((threadIdx.x & 63) == 0 && e > -100000) atomicMax(&scal[1], e);
+}
+// 2^k that brings the largest |G| 2^(ex + ew) below 2^14; and its reciprocal
+__device__ __forceinline__ int ce_gexp(const int* __restrict__ scal) {
+  const int a = scal[1], b = scal[2];
+  return (a < -50000 || b < -50000) ? 0 : min(max(kCeTopExp - (a + b), -120), 120);
+}
+
+// part[t][p] = {max, sum exp} over one class range -> lse, nll; loss partials in 64 bits
+__global__ __launch_bounds__(256) void ce_join_kernel(const float2* __restrict__ part, int nparts, size_t stride, const float* __restrict__ zlab, const int* __restrict__ lab32,
+                                                      float* __restrict__ lse, float* __restrict__ lse_out, float* __restrict__ nll_out, double* __restrict__ lsum, long P, long Pp) {
+  __shared__ double redd[16];
+  const long p = (long)blockIdx.x * 256 + threadIdx.x;
+  double acc = 0.0;
+  if (p < Pp) {
+    float m = -__builtin_inff();
+    for (int t = 0; t < nparts; ++t) { const float o = part[(size_t)t * stride + p].x; m = (o > m || o != o) ? o : m; }
+    const float ms_ = (m == -__builtin_inff()) ? 0.f : m;
+    float l = 0.f;
+    for (int t = 0; t < nparts; ++t) { const float2 o = part[(size_t)t * stride + p]; l += o.y * __builtin_amdgcn_exp2f((o.x - ms_) * kLog2e); }
+    const float lg = logf(l), s = m + lg;
+    lse[p] = s;
+    if (p < P) {
+      if (lse_out != nullptr) lse_out[p] = s;
+      const float v = lab32[p] >= 0 ? (m - zlab[p]) + lg : 0.f;        // (max - z) + log sum: nothing cancels where the label has the maximum
+      if (nll_out != nullptr) nll_out[p] = v;
+      acc = (double)v;
+    }
+  }
+  acc = block_sum_d(acc, redd);
+  if (threadIdx.x == 0) lsum[blockIdx.x] = acc;
+}
+__global__ __launch_bounds__(256) void ce_loss_kernel(const double* __restrict__ lsum, int n, float sign, int mean_valid, const int* __restrict__ scal, long P, float* __restrict__ loss) {
+  __shared__ double redd[16];
+  double a = 0.0;
+  for (int i = threadIdx.x; i < n; i += 256) a += lsum[i];
+  a = block_sum_d(a, redd);
+  if (threadIdx.x == 0) loss[0] = (float)((double)sign * a / (double)(mean_valid ? max(scal[0], 1) : P));
+}
+
+// ------------------------------------------------------------------------------------------------------------------------------ matrix products
+struct CeOperand { const _Float16* p; size_t plane; int ld; int cols; };      // ROW: [mn][k], ld = row stride; COL: [k][mn], cols = valid columns
+struct CeGemm {
+  CeOperand a, b;
+  int nseg, pa[3], pb[3];         // plane pairs summed into one accumulator
+  int ksteps;                     // K / 64 of one pair
+  int mt, nt, split;
+  // logits epilogues
+  const float *fw, *bpad, *fx; const int* lab; const float* lse; const float* gp; const int* scal;
+  float2* part; size_t part_stride; float* zlab;
+  _Float16* g; size_t g_plane; int g_ld; float* dbpart; size_t db_stride;
+  int v0; long p0;                // first class / row of this piece
+  // plain epilogue
+  float* out; size_t out_split; int out_ld;
+};
+enum { CE_STATS = 0, CE_GRAD = 1, CE_GRAD2 = 2, CE_OUT = 3 };
+
+constexpr int kCeBK = 64;
+
+// Stage one 64-deep slab of an operand tile into LDS by DMA: 1 KB an instruction, the source address permuted so that the fragment reads below are free of bank conflicts.
+//   ROW: [T rows][64 k]: 16-byte chunk j of row r lies at chunk j ^ (r & 7)
+//   COL: [64 k][T columns]: 32-byte unit u of row k lies at unit u ^ f(k), f = (k & 3) | ((k >> 3) & 1) << 2
+template <int T, bool COL, int NW>
+__device__ __forceinline__ void ce_stage(const CeOperand& o, const _Float16* base, int mn0, int wave, int lane, unsigned lds) {
+  constexpr int kInstr = T * kCeBK * 2 / 1024;
+  const ms_i32x4 rs = ms_dma_rsrc(base);
+#pragma unroll
+  for (int t = 0; t < kInstr / NW; ++t) {
+    const int ins = t * NW + wave;
+    int voff;
+    if (!COL) {
+      const int row = ins * 8 + (lane >> 3), ch = (lane & 7) ^ (row & 7);
+      voff = (int)(((unsigned)row * (unsigned)o.ld + ch * 8) * 2u);
+    } else {
+      constexpr int kRows = 1024 / (T * 2), kCh = T / 8;
+      const int k = ins * kRows + lane / kCh, ch = lane % kCh;
+      const int unit = (ch >> 1) ^ ((k & 3) | (((k >> 3) & 1) << 2));
+      const int col = min(mn0 + unit * 16 + (ch & 1) * 8, o.cols - 8);        // columns behind the operand's last are read twice and never used
+      voff = (int)(((unsigned)k * (unsigned)o.ld + (unsigned)col) * 2u);
+    }
+    ms_lds_dma16(rs, __builtin_amdgcn_readfirstlane(lds + ins * 1024), voff, 0);
+  }
+}
+template <int T, bool COL>
+__device__ __forceinline__ ms_h8 ce_frag(const _Float16* tile, int mn, int ks, int lane) {      // mn: first of 16, inside the tile
+  const int q = lane >> 4, i = lane & 15;
+  if (!COL) {
+    return *reinterpret_cast<const ms_h8*>(tile + (mn + i) * kCeBK + (((ks * 4 + q) ^ (i & 7)) * 8));
+  } else {
+    const int f = (i >> 2) | ((q & 1) << 2);
+    const int k = ks * 32 + q * 8 + (i >> 2);
+    const _Float16* a = tile + k * T + (((mn >> 4) ^ f) * 16) + (i & 3) * 4;
+    typedef __attribute__((address_space(3))) ms_s4* lp;
+    union { ms_s4 s[2]; ms_h8 h; } u;
+    u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(ms_s4*)a);
+    u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(ms_s4*)(a + 4 * T));
+    return u.h;
+  }
+}
+
+// One BM x BN tile, (BM / WM) x (BN / WN) per wave, LDS double-buffered: slab t + 1 is on its way while slab t is multiplied; one barrier a slab.
+template <int BM, int BN, int WM, int WN, bool ACOL, bool BCOL, int EPI>
+__global__ __launch_bounds__(WM * WN * 64) void ce_gemm_kernel(CeGemm g) {
+  constexpr int NW = WM * WN, TM = BM / WM, TN = BN / WN, MI = TM / 16, NJ = TN / 16;
+  __shared__ __attribute__((aligned(1024))) _Float16 sm[2][(BM + BN) * kCeBK];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q = lane >> 4, li = lane & 15;
+  const int wm = wave / WN, wn = wave % WN;
+  // Tiles of one XCD (workgroups are dealt to the 8 of them in turn) are neighbours: they share operand panels in that XCD's L2.
+  int id = blockIdx.x;
+  const int tiles = g.mt * g.nt * g.split, per = tiles >> 3;
+  if (id < per * 8) id = (id & 7) * per + (id >> 3);
+  const int sp = id / (g.mt * g.nt);
+  id -= sp * g.mt * g.nt;
+  // groups of 8 class tiles wide: 8 x (up to 8) tiles in a row use 16 panels
+  constexpr int GRP = 8;
+  const int gsz = GRP * g.nt, gi = id / gsz, gm = min(GRP, g.mt - gi * GRP), gr = id - gi * gsz;
+  const int mt = gi * GRP + gr % gm, nt = gr / gm;
+  const int m0 = mt * BM, n0 = nt * BN;
+  const int steps = g.ksteps * g.nseg;
+  const int k0 = (int)((long)steps * sp / g.split), k1 = (int)((long)steps * (sp + 1) / g.split);
+
+  ms_f4 acc[MI][NJ];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[i][j] = ms_f4{0.f, 0.f, 0.f, 0.f};
+
+  const unsigned lds0 = ms_lds_addr(&sm[0][0]);
+  auto stage = [&](int t) {
+    const int seg = t / g.ksteps, kk = t - seg * g.ksteps;
+    const unsigned buf = lds0 + (unsigned)(t & 1) * (unsigned)((BM + BN) * kCeBK * 2);
+    const _Float16* a = g.a.p + (size_t)g.pa[seg] * g.a.plane + (ACOL ? (size_t)kk * kCeBK * g.a.ld : (size_t)m0 * g.a.ld + (size_t)kk * kCeBK);
+    const _Float16* b = g.b.p + (size_t)g.pb[seg] * g.b.plane + (BCOL ? (size_t)kk * kCeBK * g.b.ld : (size_t)n0 * g.b.ld + (size_t)kk * kCeBK);
+    ce_stage<BM, ACOL, NW>(g.a, a, m0, wave, lane, buf);
+    ce_stage<BN, BCOL, NW>(g.b, b, n0, wave, lane, buf + BM * kCeBK * 2);
+  };
+  if (k0 < k1) stage(k0);
+  for (int t = k0; t < k1; ++t) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();                    // slab t has landed for every wave, and nobody reads the buffer that slab t + 1 goes to
+    if (t + 1 < k1) stage(t + 1);
+    const _Float16* sa = &sm[t & 1][0];
+    const _Float16* sb = sa + BM * kCeBK;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      ms_h8 fa[MI], fb[NJ];
+#pragma unroll
+      for (int i = 0; i < MI; ++i) fa[i] = ce_frag<BM, ACOL>(sa, wm * TM + i * 16, ks, lane);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) fb[j] = ce_frag<BN, BCOL>(sb, wn * TN + j * 16, ks, lane);
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[i], fb[j], acc[i][j], 0, 0, 0);
+    }
+  }
+
+  // Fragment layout of the result: column n = lane & 15, rows m = 4 (lane >> 4) + 0..3.
+  if (EPI == CE_OUT) {
+    float* o = g.out + (size_t)sp * g.out_split;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int m = m0 + wm * TM + i * 16 + q * 4 + r;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) o[(size_t)m * g.out_ld + n0 + wn * TN + j * 16 + li] = acc[i][j][r];
+      }
+    return;
+  }
+
+  const int vbase = m0 + wm * TM + q * 4;           // class inside the piece
+  float fxp[NJ];
+  int lab[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    const size_t p = (size_t)g.p0 + n0 + wn * TN + j * 16 + li;
+    fxp[j] = g.fx[p]; lab[j] = g.lab[p] - g.v0;
+    if (g.lab[p] < 0) lab[j] = -1;
+  }
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const float4 f = *reinterpret_cast<const float4*>(g.fw + g.v0 + vbase + i * 16), b = *reinterpret_cast<const float4*>(g.bpad + g.v0 + vbase + i * 16);
+    const float ff[4] = {f.x, f.y, f.z, f.w}, bb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[i][j][r] = acc[i][j][r] * ff[r] * fxp[j] + bb[r];
+  }
+  if (EPI == CE_STATS) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const size_t p = (size_t)g.p0 + n0 + wn * TN + j * 16 + li;
+      float mx = -__builtin_inff();
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          mx = fmaxf(mx, acc[i][j][r]);
+          if (vbase + i * 16 + r == lab[j]) g.zlab[p] = acc[i][j][r];
+        }
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float ms_ = mx == -__builtin_inff() ? 0.f : mx;
+      float l = 0.f;
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) l += __builtin_amdgcn_exp2f((acc[i][j][r] - ms_) * kLog2e);
+      l += __shfl_xor(l, 16, 64);
+      l += __shfl_xor(l, 32, 64);
+      if (q == 0) g.part[(size_t)(mt * WM + wm) * g.part_stride + p] = make_float2(mx, l);
+    }
+    return;
+  }
+  if (EPI == CE_GRAD || EPI == CE_GRAD2) {
+    const float gn = ce_pow2(ce_gexp(g.scal));
+    float gp[NJ], ls[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const size_t p = (size_t)g.p0 + n0 + wn * TN + j * 16 + li;
+      gp[j] = g.gp[p]; ls[j] = g.lse[p];
+    }
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const float4 f = *reinterpret_cast<const float4*>(g.fw + g.v0 + vbase + i * 16);
+      const float ff[4] = {f.x, f.y, f.z, f.w};
+      float db[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        ms_h4 hi, lo;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float s = __builtin_amdgcn_exp2f((acc[i][j][r] - ls[j]) * kLog2e) - (vbase + i * 16 + r == lab[j] ? 1.f : 0.f);
+          s = gp[j] == 0.f ? 0.f : s * gp[j];          // a row that takes no part gives zeros, whatever its logits are
+          db[r] += s;
+          _Float16 a, b;
+          ce_split(s * fxp[j] * gn * ff[r], a, b);
+          hi[r] = a; lo[r] = b;
+        }
+        const size_t at = (size_t)(n0 + wn * TN + j * 16 + li) * g.g_ld + vbase + i * 16;
+        *reinterpret_cast<ms_h4*>(g.g + at) = hi;
+        if (EPI == CE_GRAD2) *reinterpret_cast<ms_h4*>(g.g + g.g_plane + at) = lo;
+      }
+      if (g.dbpart != nullptr) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+#pragma unroll
+          for (int off = 1; off < 16; off <<= 1) db[r] += __shfl_xor(db[r], off, 64);
+        }
+        if (li == 0) *reinterpret_cast<float4*>(g.dbpart + (size_t)(nt * WN + wn) * g.db_stride + vbase + i * 16) = make_float4(db[0], db[1], db[2], db[3]);
+      }
+    }
+  }
+}
+
+// Sum of a product's K-splits -> dh or dw.  part [split][M][ld] with M = channels, columns = rows (dh) or M = classes, columns = channels (dw).
+//   first: nothing is there yet, else the fp32 running sum `acc` is added;  last: written to `out` in its type, else back to `acc`.
+template <typename OT, bool DH>
+__global__ __launch_bounds__(256) void ce_reduce_kernel(const float* __restrict__ part, size_t out_split, int ld, int split, const float* __restrict__ f, const int* __restrict__ scal,
+                                                        float* __restrict__ acc, void* __restrict__ out, int first, int last, long rows, long r0, int cols, int HW, int C) {
+  const float gi = ce_pow2(-ce_gexp(scal));
+  const long total = rows * cols;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
+    size_t src, dst;
+    float fac;
+    if (DH) {                  // rows = pixels of this piece (fastest), cols = channels; with HW = 1 the channels are fastest in the output
+      long p, c;
+      if (HW > 1) { c = i / rows; p = i - c * rows; } else { p = i / cols; c = i - p * cols; }
+      src = (size_t)c * ld + p;
+      const long gpix = r0 + p, n = gpix / HW;
+      dst = ((size_t)n * C + c) * HW + (gpix - n * HW);
+      fac = gi / f[gpix];
+    } else {                   // rows = classes of this piece, cols = channels
+      const long v = i / cols, c = i - v * cols;
+      src = (size_t)v * ld + c;
+      dst = (size_t)(r0 + v) * C + c;
+      fac = gi / f[r0 + v];
+    }
+    float s = 0.f;
+    for (int k = 0; k < split; ++k) s += part[k * out_split + src];
+    s *= fac;
+    if (!first) s += acc[dst];
+    if (last) ActIO<OT>::st1(out, dst, s); else acc[dst] = s;
+  }
+}
+__global__ __launch_bounds__(256) void ce_db_kernel(const float* __restrict__ part, int n, size_t stride, float* __restrict__ db, int first, int V, int v0) {
+  const int v = blockIdx.x * 256 + threadIdx.x;
+  if (v >= V) return;
+  double s = first ? 0.0 : (double)db[v0 + v];
+  for (int i = 0; i < n; ++i) s += (double)part[(size_t)i * stride + v];
+  db[v0 + v] = (float)s;
+}
+
+// ------------------------------------------------------------------------------------------------------------------------------ host
+struct CePlan {
+  long P, Pp; int Vp, Cp, HW;
+  int xp, wp, gpl;               // planes of h, w, G
+  int pb, vb;                    // rows / classes of a piece
+  int nparts;
+  int split_x, split_w;
+  size_t o_x, o_w, o_fx, o_fw, o_b, o_lab, o_lse, o_zl, o_gp, o_part, o_scal, o_lsum, o_g, o_db, o_px, o_pw, o_ax, o_aw, total;
+};
+static size_t ce_al(size_t n) { return (n + 255) & ~(size_t)255; }
+static long ce_up(long a, long b) { return (a + b - 1) / b * b; }
+
+static CePlan ce_plan(int N, int C, int V, int HW, int types, bool grad) {
+  CePlan k{};
+  k.P = (long)N * HW; k.HW = HW;
+  k.Pp = ce_up(k.P, kCePad); k.Vp = (int)ce_up(V, kCePad); k.Cp = (int)ce_up(C, kCeBK);
+  k.xp = (types & 1) ? 1 : 2; k.wp = (types & 2) ? 1 : 2;
+  k.gpl = (k.xp == 2 || k.wp == 2) ? 2 : 1;
+  k.vb = std::min(k.Vp, 8192);
+  k.pb = (int)std::min<long>(k.Pp, std::max<long>(kCePad, (long)(kCePieceBytes / ((size_t)k.vb * 2 * k.gpl)) / kCePad * kCePad));
+  k.nparts = k.Vp / 128 * 2;
+  size_t o = 0;
+  auto take = [&](size_t n) { const size_t at = o; o += ce_al(n); return at; };
+  k.o_x = take((size_t)k.xp * k.Pp * k.Cp * 2);
+  k.o_w = take((size_t)k.wp * k.Vp * k.Cp * 2);
+  k.o_fx = take(k.Pp * 4); k.o_fw = take((size_t)k.Vp * 4); k.o_b = take((size_t)k.Vp * 4);
+  k.o_lab = take(k.Pp * 4); k.o_lse = take(k.Pp * 4); k.o_zl = take(k.Pp * 4); k.o_gp = take(k.Pp * 4);
+  k.o_scal = take(64);
+  k.o_lsum = take((size_t)(k.Pp / 256) * 8);
+  const size_t stats = (size_t)k.nparts * k.Pp * 8;
+  if (!grad) { k.o_part = take(stats); k.total = o; return k; }
+  // The statistics are read before the first piece of G is written: they share its memory.
+  k.o_part = o;
+  k.o_g = take(std::max((size_t)k.gpl * k.pb * k.vb * 2, stats));
+  k.o_db = take((size_t)(k.pb / 256 * 4) * k.vb * 4);
+  // K-splits: enough tiles for the chip (256 CUs, two workgroups each at 128 x 128), at least 8 slabs of 64 each
+  const long cp = ce_up(k.Cp, 128);
+  auto split = [&](long tiles, long ksteps) { return (int)std::max<long>(1, std::min<long>(std::min<long>(512 / std::max<long>(tiles, 1), ksteps / 8), 64)); };
+  k.split_x = split(cp / 128 * (k.pb / 128), k.vb / 64);
+  k.split_w = split(cp / 128 * (k.vb / 128), k.pb / 64);
+  k.o_px = take((size_t)k.split_x * cp * k.pb * 4);
+  k.o_pw = take((size_t)k.split_w * k.vb * cp * 4);
+  k.o_ax = take((k.vb < k.Vp && (types & 1)) ? (size_t)k.P * C * 4 : 0);
+  k.o_aw = take((k.pb < k.Pp && (types & 2)) ? (size_t)V * C * 4 : 0);
+  k.total = o;
+  return k;
+}
+
+static int ce_check(int N, int C, int V, int HW, int types, const char* who) {
+  if (N < 1 || C < 1 || V < 1 || HW < 1 || types < 0 || types > 3) { set_error("%s: invalid shape", who); return MS_ERR_INVALID; }
+  if (C > 8192 || V > (1 << 20) || (long long)N * HW > (1LL << 30)) { set_error("%s: supported up to 8192 channels, 2^20 classes, 2^30 rows", who); return MS_ERR_INVALID; }
+  return MS_OK;
+}
+
+template <int EPI, bool ACOL, bool BCOL>
+static int ce_gemm(const CeGemm& g, hipStream_t st, const char* what) {
+  MS_LAUNCH((ce_gemm_kernel<128, 128, 2, 2, ACOL, BCOL, EPI>), dim3(g.mt * g.nt * g.split), dim3(256), 0, st, g);
+  return check_launch(what);
+}
+static void ce_pairs(CeGemm& g, int a, int b) {       // planes of the two operands -> products
+  g.nseg = 1; g.pa[0] = g.pb[0] = 0;
+  if (b == 2) { g.pa[g.nseg] = 0; g.pb[g.nseg++] = 1; }
+  if (a == 2) { g.pa[g.nseg] = 1; g.pb[g.nseg++] = 0; }
+}
+
+struct CeArgs {
+  const void *h, *w; const float* b; const int64_t* labels;
+  float *loss, *nll, *lse; const float *lse_in, *grad; void *dh, *dw; float* db;
+  float sign; int mean_valid; const float* scale_dev;
+  int N, C, V, HW, types; void* ws; size_t ws_bytes; hipStream_t st;
+};
+
+static int ce_run(const CeArgs& a, const char* who) {
+  if (int e = ce_check(a.N, a.C, a.V, a.HW, a.types, who)) return e;
+  if (a.h == nullptr || a.w == nullptr || a.labels == nullptr) { set_error("%s: null pointer", who); return MS_ERR_INVALID; }
+  const bool need_grad = a.dh != nullptr || a.dw != nullptr || a.db != nullptr;
+  const CePlan k = ce_plan(a.N, a.C, a.V, a.HW, a.types, need_grad);
+  if (a.ws == nullptr || a.ws_bytes < k.total) { set_error("%s: workspace too small", who); return MS_ERR_WORKSPACE; }
+  if (!aligned16(a.ws)) { set_error("%s: workspace not 16-byte aligned", who); return MS_ERR_ALIGN; }
+  char* ws = (char*)a.ws;
+  auto f32 = [&](size_t o) { return (float*)(ws + o); };
+  _Float16 *x = (_Float16*)(ws + k.o_x), *w = (_Float16*)(ws + k.o_w);
+  const size_t xpl = (size_t)k.Pp * k.Cp, wpl = (size_t)k.Vp * k.Cp;
+  int *lab = (int*)(ws + k.o_lab), *scal = (int*)(ws + k.o_scal);
+  float *fx = f32(k.o_fx), *fw = f32(k.o_fw), *bp = f32(k.o_b), *lse = f32(k.o_lse), *zl = f32(k.o_zl), *gp = f32(k.o_gp);
+  hipStream_t st = a.st;
+  MS_LAUNCH(ce_init_kernel, dim3(1), dim3(64), 0, st, scal);
+  if (int e = check_launch("ce_init")) return e;
+  if (a.types & 2) MS_LAUNCH((ce_pack_rows_kernel<ms_bf16, 1>), dim3(k.Vp / 4), dim3(256), 0, st, a.w, a.b, (const int64_t*)nullptr, 0, w, wpl, fw, bp, (int*)nullptr, scal, a.V, k.Vp, a.C, k.Cp);
+  else MS_LAUNCH((ce_pack_rows_kernel<float, 2>), dim3(k.Vp / 4), dim3(256), 0, st, a.w, a.b, (const int64_t*)nullptr, 0, w, wpl, fw, bp, (int*)nullptr, scal, a.V, k.Vp, a.C, k.Cp);
+  if (int e = check_launch("ce_pack_w")) return e;
+  const dim3 gx((unsigned)(k.Pp / 64));
+  if (a.types & 1) MS_LAUNCH((ce_pack_planes_kernel<ms_bf16, 1>), gx, dim3(256), 0, st, a.h, a.labels, a.V, need_grad ? 1 : 0, x, xpl, fx, lab, k.P, k.Pp, a.C, k.Cp, a.HW);
+  else MS_LAUNCH((ce_pack_planes_kernel<float, 2>), gx, dim3(256), 0, st, a.h, a.labels, a.V, need_grad ? 1 : 0, x, xpl, fx, lab, k.P, k.Pp, a.C, k.Cp, a.HW);
+  if (int e = check_launch("ce_pack_h")) return e;
+  if (a.mean_valid) {
+    MS_LAUNCH(ce_count_kernel, dim3((unsigned)std::min<long>(cdiv((int)std::min<long>(k.P, 1 << 30), 1024), 1024)), dim3(256), 0, st, a.labels, k.P, a.V, scal);
+    if (int e = check_launch("ce_count")) return e;
+  }
+  CeGemm g{};
+  g.fw = fw; g.bpad = bp; g.fx = fx; g.lab = lab; g.lse = lse; g.gp = gp; g.scal = scal; g.zlab = zl;
+  if (a.lse_in == nullptr) {
+    // logits -> statistics: M = classes, N = rows
+    g.a = CeOperand{w, wpl, k.Cp, 0}; g.b = CeOperand{x, xpl, k.Cp, 0};
+    ce_pairs(g, k.wp, k.xp);
+    g.ksteps = k.Cp / kCeBK; g.mt = k.Vp / 128; g.nt = (int)(k.Pp / 128); g.split = 1;
+    g.part = (float2*)(ws + k.o_part); g.part_stride = (size_t)k.Pp;
+    if (int e = ce_gemm<CE_STATS, false, false>(g, st, "ce_stats")) return e;
+    MS_LAUNCH(ce_join_kernel, dim3((unsigned)(k.Pp / 256)), dim3(256), 0, st, (const float2*)g.part, k.nparts, g.part_stride, zl, lab, lse, a.lse, a.nll, (double*)(ws + k.o_lsum), k.P, k.Pp);
+    if (int e = check_launch("ce_join")) return e;
+    if (a.loss != nullptr) {
+      MS_LAUNCH(ce_loss_kernel, dim3(1), dim3(256), 0, st, (const double*)(ws + k.o_lsum), (int)(k.Pp / 256), a.sign, a.mean_valid, scal, k.P, a.loss);
+      if (int e = check_launch("ce_loss")) return e;
+    }
+  }
+  if (!need_grad) return MS_OK;
+  MS_LAUNCH(ce_rowgrad_kernel, dim3((unsigned)std::min<long>(k.Pp / 256, 1024)), dim3(256), 0, st, a.grad, a.sign, a.mean_valid, a.scale_dev, lab, fx, gp, a.lse_in, lse, scal, k.P, k.Pp);
+  if (int e = check_launch("ce_rowgrad")) return e;
+  const long cp = ce_up(k.Cp, 128);
+  for (long p0 = 0; p0 < k.Pp; p0 += k.pb) {
+    const int pn = (int)std::min<long>(k.pb, k.Pp - p0);
+    for (int v0 = 0; v0 < k.Vp; v0 += k.vb) {
+      const int vn = std::min(k.vb, k.Vp - v0);
+      CeGemm d = g;
+      d.a = CeOperand{w + (size_t)v0 * k.Cp, wpl, k.Cp, 0}; d.b = CeOperand{x + (size_t)p0 * k.Cp, xpl, k.Cp, 0};
+      ce_pairs(d, k.wp, k.xp);
+      d.ksteps = k.Cp / kCeBK; d.mt = vn / 128; d.nt = pn / 128; d.split = 1; d.v0 = v0; d.p0 = p0;
+      _Float16* G = (_Float16*)(ws + k.o_g);
+      const size_t gpl = (size_t)k.pb * k.vb;
+      d.g = G; d.g_plane = gpl; d.g_ld = k.vb;
+      d.dbpart = a.db != nullptr ? f32(k.o_db) : nullptr; d.db_stride = k.vb;
+      if (k.gpl == 2) { if (int e = ce_gemm<CE_GRAD2, false, false>(d, st, "ce_grad")) return e; }
+      else { if (int e = ce_gemm<CE_GRAD, false, false>(d, st, "ce_grad")) return e; }
+      if (a.db != nullptr) {
+        const int vr = std::min(vn, a.V - v0);
+        if (vr > 0) {
+          MS_LAUNCH(ce_db_kernel, dim3(cdiv(vr, 256)), dim3(256), 0, st, f32(k.o_db), pn / 128 * 2, (size_t)k.vb, a.db, p0 == 0 ? 1 : 0, vr, v0);
+          if (int e = check_launch("ce_db")) return e;
+        }
+      }
+      if (a.dh != nullptr) {        // dh^T [channels][rows] = w^T G^T
+        CeGemm o{};
+        o.a = CeOperand{w + (size_t)v0 * k.Cp, wpl, k.Cp, k.Cp}; o.b = CeOperand{G, gpl, k.vb, 0};
+        ce_pairs(o, (a.types & 1) ? 1 : k.wp, (a.types & 1) ? 1 : 2);
+        o.ksteps = vn / kCeBK; o.mt = (int)(cp / 128); o.nt = pn / 128; o.split = k.split_x;
+        o.out = f32(k.o_px); o.out_ld = k.pb; o.out_split = (size_t)cp * k.pb;
+        if (int e = ce_gemm<CE_OUT, true, false>(o, st, "ce_dh")) return e;
+        const long rows = std::min<long>(pn, k.P - p0);
+        const int first = v0 == 0, last = v0 + vn >= k.Vp;
+        const dim3 grid((unsigned)std::min<long>((rows * a.C + 255) / 256, 8192));
+        float* ac = (a.types & 1) ? f32(k.o_ax) : (float*)a.dh;
+        if (a.types & 1) MS_LAUNCH((ce_reduce_kernel<ms_bf16, true>), grid, dim3(256), 0, st, o.out, o.out_split, o.out_ld, o.split, fx, scal, ac, a.dh, first, last, rows, p0, a.C, a.HW, a.C);
+        else MS_LAUNCH((ce_reduce_kernel<float, true>), grid, dim3(256), 0, st, o.out, o.out_split, o.out_ld, o.split, fx, scal, ac, a.dh, first, last, rows, p0, a.C, a.HW, a.C);
+        if (int e = check_launch("ce_dh_sum")) return e;
+      }
+      const int vr = std::min(vn, a.V - v0);
+      if (a.dw != nullptr && vr > 0) {        // dw [classes][channels] = G^T h
+        CeGemm o{};
+        o.a = CeOperand{G, gpl, k.vb, k.vb}; o.b = CeOperand{x + (size_t)p0 * k.Cp, xpl, k.Cp, k.Cp};
+        ce_pairs(o, (a.types & 2) ? 1 : 2, (a.types & 2) ? 1 : k.xp);
+        o.ksteps = pn / kCeBK; o.mt = vn / 128; o.nt = (int)(cp / 128); o.split = k.split_w;
+        o.out = f32(k.o_pw); o.out_ld = (int)cp; o.out_split = (size_t)k.vb * cp;
+        if (int e = ce_gemm<CE_OUT, true, true>(o, st, "ce_dw")) return e;
+        const int first = p0 == 0, last = p0 + pn >= k.Pp;
+        const dim3 grid((unsigned)std::min<long>(((long)vr * a.C + 255) / 256, 8192));
+        float* ac = (a.types & 2) ? f32(k.o_aw) : (float*)a.dw;
+        if (a.types & 2) MS_LAUNCH((ce_reduce_kernel<ms_bf16, false>), grid, dim3(256), 0, st, o.out, o.out_split, o.out_ld, o.split, fw, scal, ac, a.dw, first, last, (long)vr, (long)v0, a.C, 1, a.C);
+        else MS_LAUNCH((ce_reduce_kernel<float, false>), grid, dim3(256), 0, st, o.out, o.out_split, o.out_ld, o.split, fw, scal, ac, a.dw, first, last, (long)vr, (long)v0, a.C, 1, a.C);
+        if (int e = check_launch("ce_dw_sum")) return e;
+      }
+    }
+  }
+  return MS_OK;
+}
+}  // namespace ms
+
+extern "C" size_t ms_class_ce_ws_bytes(int N, int C, int V, int HW, int types, int need_grad) {
+  if (ms::ce_check(N, C, V, HW, types, "ms_class_ce_ws_bytes")) return 0;
+  return ms::ce_plan(N, C, V, HW, types, need_grad != 0).total;
+}
+extern "C" int ms_class_ce(const void* h, const void* w, const float* b, const int64_t* labels, float* loss_out, void* dh, void* dw, float* db, int N, int C, int V, int HW,
+                           int types, float loss_sign, int mean_valid, const float* grad_scale_dev, void* ws, size_t ws_bytes, void* stream) {
+  if (loss_out == nullptr) { ms::set_error("ms_class_ce: loss_out is NULL"); return MS_ERR_INVALID; }
+  ms::CeArgs a{};
+  a.h = h; a.w = w; a.b = b; a.labels = labels; a.loss = loss_out; a.dh = dh; a.dw = dw; a.db = db;
+  a.sign = loss_sign; a.mean_valid = mean_valid ? 1 : 0; a.scale_dev = grad_scale_dev;
+  a.N = N; a.C = C; a.V = V; a.HW = HW; a.types = types; a.ws = ws; a.ws_bytes = ws_bytes; a.st = (hipStream_t)stream;
+  return ms::ce_run(a, "ms_class_ce");
+}
+extern "C" int ms_class_ce_fwd(const void* h, const void* w, const float* b, const int64_t* labels, float* nll, float* lse, int N, int C, int V, int HW, int types,
+                               void* ws, size_t ws_bytes, void* stream) {
+  if (nll == nullptr || lse == nullptr) { ms::set_error("ms_class_ce_fwd: null pointer"); return MS_ERR_INVALID; }
+  ms::CeArgs a{};
+  a.h = h; a.w = w; a.b = b; a.labels = labels; a.nll = nll; a.lse = lse; a.sign = 1.f;
+  a.N = N; a.C = C; a.V = V; a.HW = HW; a.types = types; a.ws = ws; a.ws_bytes = ws_bytes; a.st = (hipStream_t)stream;
+  return ms::ce_run(a, "ms_class_ce_fwd");
+}
+extern "C" int ms_class_ce_bwd(const void* h, const void* w, const float* b, const int64_t* labels, const float* lse, const float* grad, void* dh, void* dw, float* db,
+                               int N, int C, int V, int HW, int types, void* ws, size_t ws_bytes, void* stream) {
+  if (lse == nullptr || grad == nullptr || (dh == nullptr && dw == nullptr && db == nullptr)) { ms::set_error("ms_class_ce_bwd: null pointer"); return MS_ERR_INVALID; }
+  ms::CeArgs a{};
+  a.h = h; a.w = w; a.b = b; a.labels = labels; a.lse_in = lse; a.grad = grad; a.dh = dh; a.dw = dw; a.db = db; a.sign = 1.f;
+  a.N = N; a.C = C; a.V = V; a.HW = HW; a.types = types; a.ws = ws; a.ws_bytes = ws_bytes; a.st = (hipStream_t)stream;
+  return ms::ce_run(a, "ms_class_ce_bwd");
+}

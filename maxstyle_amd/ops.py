@@ -401,3 +401,221 @@ def mse_loss(x, target):
     ws = torch.empty(lib.ms_mse_ws_bytes(), dtype=torch.uint8, device=x.device)
     check(lib.ms_mse_loss(x.data_ptr(), target.data_ptr(), n, 0.5 / n, 0.0, out.data_ptr(), 0, ws.data_ptr(), ws.numel(), _stream()), "ms_mse_loss")
     return out[0]
+
+
+# ---------------------------------------------------------------------------------------------------------
+# head + cross entropy over many classes (the logits are never kept)
+# ---------------------------------------------------------------------------------------------------------
+def _class_ce_args(h, w, b, labels):
+    """Checks of the ms_class_ce family: (N, C, V, HW, types) of h [N,C,*spatial] (rows of features: [T,C]), w [V,C] or [V,C,1,1], b [V] | None, labels [N,*spatial]."""
+    for name, t in (("h", h), ("w", w)):
+        if not t.is_cuda:
+            raise RuntimeError("maxstyle_amd ops run on the MI355X only: got a CPU tensor (there is no CPU fallback)")
+        if t.dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError(f"class_ce: {name} is fp32 or bf16; got {t.dtype}")
+        if not t.is_contiguous():
+            raise ValueError(f"class_ce: {name} must be contiguous")
+    if h.dim() < 2:
+        raise ValueError("class_ce: h is [N,C,*spatial] or rows [T,C]")
+    if w.dim() < 2 or w.shape[1] != h.shape[1] or w.numel() != w.shape[0] * w.shape[1]:
+        raise ValueError(f"class_ce: w must be [V,{h.shape[1]}] (or a 1x1 convolution's weight); got {tuple(w.shape)}")
+    if b is not None:
+        _need_cuda_f32(b)
+        if b.numel() != w.shape[0]:
+            raise ValueError(f"class_ce: b has {b.numel()} elements for {w.shape[0]} classes")
+    if labels.dtype != torch.int64 or not labels.is_cuda or not labels.is_contiguous():
+        raise TypeError("labels must be a contiguous CUDA int64 tensor [N,*spatial]")
+    if tuple(labels.shape) != (h.shape[0],) + tuple(h.shape[2:]):
+        raise ValueError(f"class_ce: labels must be {(h.shape[0],) + tuple(h.shape[2:])}; got {tuple(labels.shape)}")
+    if h.numel() == 0 or w.numel() == 0:
+        raise ValueError("class_ce: empty input")
+    for t in (w, b, labels):
+        if t is not None and t.device != h.device:
+            raise ValueError("class_ce: all tensors must be on one device")
+    N, C = h.shape[:2]
+    return N, C, w.shape[0], labels.numel() // N, int(h.dtype == torch.bfloat16) | 2 * int(w.dtype == torch.bfloat16)
+
+
+def _class_ce_ws(N, C, V, HW, types, need_grad, device):
+    # a block of its own for every call: the caching allocator hands it out again in stream order, and a captured graph keeps its own (two graphs share nothing)
+    nbytes = lib.ms_class_ce_ws_bytes(N, C, V, HW, types, 1 if need_grad else 0)
+    if nbytes == 0:
+        check(-1, "ms_class_ce_ws_bytes")
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def class_ce(h, w, b, labels, loss_sign=1.0, mean_over="all", need_dh=True, need_dw=True, grad_scale=None):
+    """`head_ce` for any number of classes and channels, with every gradient: loss = loss_sign * mean cross entropy of (w h + b) against `labels`, and its gradients, without
+    the logits ever being stored (ms_class_ce).  Returns (loss [0-dim], dh, dw, db); what is not asked for (need_dh / need_dw; db without b) is None.
+
+    h [N,C,*spatial] or rows [T,C], fp32 or bf16; w [V,C] (or [V,C,1,1]), fp32 or bf16; b [V] fp32 or None; labels [N,*spatial] int64.  A label outside [0,V) takes its
+    row out: nothing in the loss, exactly 0 in the gradients, whatever its features hold.  mean_over: "all" rows (cross_entropy_2D's mean) or the "valid" ones.
+    grad_scale: an upstream gradient, a 1-element fp32 CUDA tensor (read on the device).  Runs on the current stream, can be captured into a graph, gives the same bits
+    every time."""
+    if mean_over not in ("all", "valid"):
+        raise ValueError("class_ce: mean_over is 'all' or 'valid'")
+    N, C, V, HW, types = _class_ce_args(h, w, b, labels)
+    if grad_scale is not None:
+        _need_cuda_f32(grad_scale)
+        if grad_scale.numel() != 1 or grad_scale.device != h.device:
+            raise ValueError("class_ce: grad_scale is one fp32 value on the device of h")
+    with torch.cuda.device(h.device):
+        loss = torch.empty((), device=h.device, dtype=torch.float32)
+        dh = torch.empty_like(h) if need_dh else None
+        dw = torch.empty_like(w) if need_dw else None
+        db = torch.empty_like(b) if (need_dw and b is not None) else None
+        ws = _class_ce_ws(N, C, V, HW, types, need_dh or need_dw, h.device)
+        check(lib.ms_class_ce(h.data_ptr(), w.data_ptr(), _ptr(b), labels.data_ptr(), loss.data_ptr(), _ptr(dh), _ptr(dw), _ptr(db), N, C, V, HW, types, float(loss_sign),
+                              1 if mean_over == "valid" else 0, _ptr(grad_scale), ws.data_ptr(), ws.numel(), _stream()), "ms_class_ce")
+    return loss, dh, dw, db
+
+
+def class_ce_fwd(h, w, b, labels):
+    """Cross entropy of every row and the log-sum of its exponentials, (nll, lse) [N,*spatial] fp32 (ms_class_ce_fwd); arguments as class_ce.  nll is 0 where the label
+    is not a class."""
+    N, C, V, HW, types = _class_ce_args(h, w, b, labels)
+    with torch.cuda.device(h.device):
+        nll = torch.empty(labels.shape, device=h.device, dtype=torch.float32)
+        lse = torch.empty_like(nll)
+        ws = _class_ce_ws(N, C, V, HW, types, False, h.device)
+        check(lib.ms_class_ce_fwd(h.data_ptr(), w.data_ptr(), _ptr(b), labels.data_ptr(), nll.data_ptr(), lse.data_ptr(), N, C, V, HW, types, ws.data_ptr(), ws.numel(),
+                                  _stream()), "ms_class_ce_fwd")
+    return nll, lse
+
+
+def class_ce_bwd(h, w, b, labels, lse, grad, need_dh=True, need_dw=True):
+    """Gradients (dh, dw, db) of sum(grad * nll) for class_ce_fwd's nll, from its inputs and its lse (ms_class_ce_bwd).  grad [N,*spatial] fp32."""
+    N, C, V, HW, types = _class_ce_args(h, w, b, labels)
+    _need_cuda_f32(lse, grad)
+    for t in (lse, grad):
+        if t.shape != labels.shape or t.device != h.device:
+            raise ValueError("class_ce_bwd: lse and grad have the shape and the device of labels")
+    if not (need_dh or need_dw):
+        return None, None, None
+    with torch.cuda.device(h.device):
+        dh = torch.empty_like(h) if need_dh else None
+        dw = torch.empty_like(w) if need_dw else None
+        db = torch.empty_like(b) if (need_dw and b is not None) else None
+        ws = _class_ce_ws(N, C, V, HW, types, True, h.device)
+        check(lib.ms_class_ce_bwd(h.data_ptr(), w.data_ptr(), _ptr(b), labels.data_ptr(), lse.data_ptr(), grad.data_ptr(), _ptr(dh), _ptr(dw), _ptr(db), N, C, V, HW, types,
+                                  ws.data_ptr(), ws.numel(), _stream()), "ms_class_ce_bwd")
+    return dh, dw, db
+
+
+# ---------------------------------------------------------------------------------------------------------
+# activation checkpoints in 8 bits
+# ---------------------------------------------------------------------------------------------------------
+ACT8_BLOCK = 256             # elements of a plane that share one scale (ms_act8_block)
+
+
+def _act8_dims(shape, who):
+    if len(shape) < 3:
+        raise ValueError(f"{who}: activations are [N,C,*spatial]")
+    N, C = int(shape[0]), int(shape[1])
+    HW = 1
+    for n in shape[2:]:
+        HW *= int(n)
+    if N * C * HW == 0:
+        raise ValueError(f"{who}: empty input")
+    return N, C, HW
+
+
+def _act8_coef(coef4, C, device, who):
+    if coef4 is not None:
+        _need_cuda_f32(coef4)
+        if tuple(coef4.shape) != (C, 4) or coef4.device != device:
+            raise ValueError(f"{who}: coef4 is the [C,4] record of bn_finalize, on the activations' device")
+        if coef4.data_ptr() % 16:
+            raise ValueError(f"{who}: coef4 must be 16-byte aligned")
+
+
+def _act8_kept(q, s, who):
+    for t, dt in ((q, torch.int8), (s, torch.float32)):
+        if not t.is_cuda:
+            raise RuntimeError("maxstyle_amd ops run on the MI355X only: got a CPU tensor (there is no CPU fallback)")
+        if t.dtype != dt or not t.is_contiguous():
+            raise TypeError(f"{who}: a checkpoint is (q int8, s fp32), contiguous, as act8_pack returns it")
+    N, C, HW = _act8_dims(q.shape, who)
+    if tuple(s.shape) != (N, C, (HW + ACT8_BLOCK - 1) // ACT8_BLOCK) or s.device != q.device:
+        raise ValueError(f"{who}: s must be [N,C,ceil(HW/{ACT8_BLOCK})] on the device of q; got {tuple(s.shape)}")
+    return N, C, HW
+
+
+def act8_pack(x, coef4=None, q=None, s=None):
+    """8-bit checkpoint (q int8 [N,C,*spatial], s fp32 [N,C,ceil(HW/256)]) of an activation x, fp32 or bf16 (ms_act8_pack): 8.125 bits an element, |x' - x| <= half a
+    step of its 256-element block's largest deviation / 127, signs kept exactly.  coef4: the BatchNorm record (bn_finalize) of a raw convolution output: the checkpoint is
+    then centred on the BatchNorm's zero, so that LeakyReLU's mask is exact; None: for activation outputs (zeros and signs are exact).  q, s: buffers to write into."""
+    bf = _need_cuda_act(x)
+    N, C, HW = _act8_dims(x.shape, "act8_pack")
+    _act8_coef(coef4, C, x.device, "act8_pack")
+    with torch.cuda.device(x.device):
+        q = torch.empty(x.shape, dtype=torch.int8, device=x.device) if q is None else q
+        s = torch.empty(N, C, (HW + ACT8_BLOCK - 1) // ACT8_BLOCK, dtype=torch.float32, device=x.device) if s is None else s
+        if _act8_kept(q, s, "act8_pack") != (N, C, HW) or q.device != x.device:
+            raise ValueError("act8_pack: q must have the shape and the device of x")
+        check(_fn("ms_act8_pack", bf)(x.data_ptr(), _ptr(coef4), q.data_ptr(), s.data_ptr(), N, C, HW, _stream()), "ms_act8_pack")
+    return q, s
+
+
+def act8_unpack(q, s, coef4=None, dtype=torch.float32, out=None):
+    """The activation that a checkpoint of act8_pack stands for, in fp32 or bf16; coef4: the record it was made with (ms_act8_unpack)."""
+    N, C, HW = _act8_kept(q, s, "act8_unpack")
+    _act8_coef(coef4, C, q.device, "act8_unpack")
+    with torch.cuda.device(q.device):
+        out = torch.empty(q.shape, dtype=dtype, device=q.device) if out is None else out
+        bf = _need_cuda_act(out)
+        if out.shape != q.shape or out.device != q.device:
+            raise ValueError("act8_unpack: out must have the shape and the device of q")
+        check(_fn("ms_act8_unpack", bf)(q.data_ptr(), s.data_ptr(), _ptr(coef4), out.data_ptr(), N, C, HW, _stream()), "ms_act8_unpack")
+    return out
+
+
+def _act8_bwd_args(g, q, s, coef4, slope, ref_q, who):
+    bf = _need_cuda_act(g)
+    N, C, HW = _act8_kept(q, s, who)
+    if coef4 is None:
+        raise ValueError(f"{who}: needs the BatchNorm record the checkpoint was made with")
+    _act8_coef(coef4, C, q.device, who)
+    if g.shape != q.shape or g.device != q.device:
+        raise ValueError(f"{who}: the gradient must have the shape and the device of q")
+    if ref_q is not None and (ref_q.dtype != torch.int8 or ref_q.shape != q.shape or not ref_q.is_contiguous() or ref_q.device != q.device):
+        raise ValueError(f"{who}: ref_q is the int8 part of the activation output's checkpoint, shaped like q")
+    if not 0.0 <= slope <= 1.0:
+        raise ValueError(f"{who}: 0 <= slope <= 1")
+    return bf, N, C, HW
+
+
+def act8_bwd_reduce(gin, q, s, coef4, slope, ref_q=None, gout=None, uout=None, part=None):
+    """act_bwd_reduce out of a checkpoint (ms_act8_bwd_reduce): (gout, part, nparts) with gout = gin * (r > 0 ? 1 : slope); r from ref_q's signs or the checkpoint's own.
+    uout: a tensor that receives the kept activation on the way."""
+    bf, N, C, HW = _act8_bwd_args(gin, q, s, coef4, slope, ref_q, "act8_bwd_reduce")
+    _need_cuda_f32(part)
+    with torch.cuda.device(gin.device):
+        nparts = lib.ms_act8_bwd_parts(N, C, HW)
+        gout = torch.empty_like(gin) if gout is None else gout
+        part = torch.empty(C, nparts, 2, device=gin.device, dtype=torch.float32) if part is None else part
+        for t in (gout, uout):
+            if t is not None and (t.shape != gin.shape or t.dtype != gin.dtype or not t.is_contiguous() or t.device != gin.device):
+                raise ValueError("act8_bwd_reduce: gout and uout are contiguous and like gin")
+        if part.numel() < C * nparts * 2 or part.device != gin.device:
+            raise ValueError(f"act8_bwd_reduce: part must hold [C,{nparts},2]")
+        check(_fn("ms_act8_bwd_reduce", bf)(gin.data_ptr(), _ptr(ref_q), q.data_ptr(), s.data_ptr(), coef4.data_ptr(), gout.data_ptr(), _ptr(uout), part.data_ptr(), N, C, HW,
+                                            float(slope), _stream()), "ms_act8_bwd_reduce")
+    return gout, part, nparts
+
+
+def act8_bn_act_bwd(g, q, s, coef4, slope, ref_q=None, out=None):
+    """Backward of BatchNorm (batch statistics) + LeakyReLU from the 8-bit checkpoint (q, s) of the BatchNorm's input (ms_act8_bn_act_bwd): returns (du, dgamma, dbeta).
+    g: gradient of the activation's output, fp32 or bf16; coef4: the bn_finalize record the checkpoint was made with; ref_q: the int8 part of the checkpoint of the saved
+    activation output where something was added in front of the activation (a residual block's tail) - without it the mask comes from the checkpoint itself."""
+    bf, N, C, HW = _act8_bwd_args(g, q, s, coef4, slope, ref_q, "act8_bn_act_bwd")
+    with torch.cuda.device(g.device):
+        out = torch.empty_like(g) if out is None else out
+        if out.shape != g.shape or out.dtype != g.dtype or not out.is_contiguous() or out.device != g.device:
+            raise ValueError("act8_bn_act_bwd: out is contiguous and like g")
+        dg = torch.empty(C, device=g.device, dtype=torch.float32)
+        db = torch.empty_like(dg)
+        ws = torch.empty(max(lib.ms_act8_bwd_ws_bytes(N, C, HW), 64), dtype=torch.uint8, device=g.device)
+        check(_fn("ms_act8_bn_act_bwd", bf)(g.data_ptr(), _ptr(ref_q), q.data_ptr(), s.data_ptr(), coef4.data_ptr(), out.data_ptr(), dg.data_ptr(), db.data_ptr(), N, C, HW,
+                                            float(slope), ws.data_ptr(), ws.numel(), _stream()), "ms_act8_bn_act_bwd")
+    return out, dg, db
