@@ -8,6 +8,7 @@
 // The logits are never written; G exists for one piece at a time (kCePieceBytes: it stays in the 256 MB last-level cache between its writer and its two readers).
 #include <algorithm>
 #include "ms_class_ce.h"
+#include "ms_class_ce_narrow.h"
 #include "maxstyle_hip.h"
 
 namespace ms {
@@ -486,17 +487,11 @@ static void ce_pairs(CeGemm& g, int a, int b) {       // planes of the two opera
   if (a == 2) { g.pa[g.nseg] = 1; g.pb[g.nseg++] = 0; }
 }
 
-struct CeArgs {
-  const void *h, *w; const float* b; const int64_t* labels;
-  float *loss, *nll, *lse; const float *lse_in, *grad; void *dh, *dw; float* db;
-  float sign; int mean_valid; const float* scale_dev;
-  int N, C, V, HW, types; void* ws; size_t ws_bytes; hipStream_t st;
-};
-
 static int ce_run(const CeArgs& a, const char* who) {
   if (int e = ce_check(a.N, a.C, a.V, a.HW, a.types, who)) return e;
   if (a.h == nullptr || a.w == nullptr || a.labels == nullptr) { set_error("%s: null pointer", who); return MS_ERR_INVALID; }
   const bool need_grad = a.dh != nullptr || a.dw != nullptr || a.db != nullptr;
+  if (ce_narrow_ok(a.N, a.C, a.V, a.HW)) return ce_narrow_run(a, need_grad, who);
   const CePlan k = ce_plan(a.N, a.C, a.V, a.HW, a.types, need_grad);
   if (a.ws == nullptr || a.ws_bytes < k.total) { set_error("%s: workspace too small", who); return MS_ERR_WORKSPACE; }
   if (!aligned16(a.ws)) { set_error("%s: workspace not 16-byte aligned", who); return MS_ERR_ALIGN; }
@@ -599,6 +594,7 @@ static int ce_run(const CeArgs& a, const char* who) {
 
 extern "C" size_t ms_class_ce_ws_bytes(int N, int C, int V, int HW, int types, int need_grad) {
   if (ms::ce_check(N, C, V, HW, types, "ms_class_ce_ws_bytes")) return 0;
+  if (ms::ce_narrow_ok(N, C, V, HW)) return ms::ce_narrow_ws_bytes(N, C, V, HW, types, need_grad != 0);
   return ms::ce_plan(N, C, V, HW, types, need_grad != 0).total;
 }
 extern "C" int ms_class_ce(const void* h, const void* w, const float* b, const int64_t* labels, float* loss_out, void* dh, void* dw, float* db, int N, int C, int V, int HW,
