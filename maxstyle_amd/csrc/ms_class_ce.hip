@@ -13,7 +13,7 @@
 
 namespace ms {
 
-constexpr size_t kCePieceBytes = (size_t)96 << 20;
+constexpr size_t kCePieceBytes = (size_t)128 << 20;
 
 // ------------------------------------------------------------------------------------------------------------------------------ small passes
 // scal[0]: rows that take part; scal[1]: max over rows of exponent(g_p) + ex[p]; scal[2]: max over classes of ew[v]   (integers: their order does not matter)
@@ -21,12 +21,12 @@ __global__ void ce_init_kernel(int* scal) {
   if (threadIdx.x == 0) { scal[0] = 0; scal[1] = -100000; scal[2] = -100000; }
 }
 
-// w [V][C] -> planes [Vp][Cp], fw[v] = 2^ew, bpad[v] = b or -inf behind the last class.  One wave a row.
-template <typename WT, int PL>
-__global__ __launch_bounds__(256) void ce_pack_rows_kernel(const void* __restrict__ w, const float* __restrict__ b, const int64_t* __restrict__ labels, int classes,
+// Rows [rows][C] -> planes [rows_pad][Cp] and each row's 2^e.  One wave a row; 8 channels a lane where the rows are made of whole vectors.
+//   weights: bpad[v] = b or -inf behind the last class; features (labels != nullptr): a row that takes no part is packed as zeros when `drop` is set (it may hold anything)
+template <typename WT, int PL, bool VEC>
+__global__ __launch_bounds__(256) void ce_pack_rows_kernel(const void* __restrict__ w, const float* __restrict__ b, const int64_t* __restrict__ labels, int classes, int drop,
                                                            _Float16* __restrict__ out, size_t plane, float* __restrict__ fw, float* __restrict__ bpad,
                                                            int* __restrict__ lab32, int* __restrict__ scal, int rows, int rows_pad, int C, int Cp) {
-  // labels != nullptr: the rows are features, one that takes no part is packed as zeros (its h may hold anything); otherwise weights
   using IO = ActIO<WT>;
   const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (r >= rows_pad) return;
@@ -34,11 +34,22 @@ __global__ __launch_bounds__(256) void ce_pack_rows_kernel(const void* __restric
   if (labels != nullptr) {
     int y = -1;
     if (live) { const int64_t l = labels[r]; y = (l >= 0 && l < classes) ? (int)l : -1; }
-    live = y >= 0;
+    live = live && (!drop || y >= 0);
     if (lane == 0) lab32[r] = y;
   }
+  const size_t base = (size_t)r * C;
   unsigned am = 0;
-  if (live) for (int c = lane; c < C; c += 64) am = max(am, __float_as_uint(IO::ld1(w, (size_t)r * C + c)) & 0x7FFFFFFFu);
+  auto see = [&](float v) { am = max(am, __float_as_uint(v) & 0x7FFFFFFFu); };
+  if (live) {
+    if (VEC) {
+      for (int c = lane * 8; c < C; c += 512) {
+        const float4 u = IO::ld4(w, base + c), v = IO::ld4(w, base + c + 4);
+        see(u.x); see(u.y); see(u.z); see(u.w); see(v.x); see(v.y); see(v.z); see(v.w);
+      }
+    } else {
+      for (int c = lane; c < C; c += 64) see(IO::ld1(w, base + c));
+    }
+  }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) am = max(am, (unsigned)__shfl_xor((int)am, off, 64));
   const int e = ce_exponent(__uint_as_float(am));
@@ -46,58 +57,63 @@ __global__ __launch_bounds__(256) void ce_pack_rows_kernel(const void* __restric
   if (lane == 0) {
     fw[r] = ce_pow2(e);
     if (bpad != nullptr) bpad[r] = r < rows ? (b != nullptr ? b[r] : 0.f) : -__builtin_inff();
-    if (bpad != nullptr && r < rows) atomicMax(&scal[2], e);
+    // (looked at first: 32768 rows' atomics on one word took 370 us, this 10)
+    if (bpad != nullptr && r < rows && e > __hip_atomic_load(&scal[2], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(&scal[2], e);
   }
-  for (int c = lane; c < Cp; c += 64) {
-    const float v = (live && c < C) ? IO::ld1(w, (size_t)r * C + c) * inv : 0.f;
-    _Float16 hi, lo;
-    ce_split(v, hi, lo);
-    out[(size_t)r * Cp + c] = hi;
-    if (PL == 2) out[plane + (size_t)r * Cp + c] = lo;
+  for (int c = lane * 8; c < Cp; c += 512) {
+    float v[8];
+    if (VEC) {
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f), d = a;
+      if (live && c < C) { a = IO::ld4(w, base + c); d = IO::ld4(w, base + c + 4); }
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = d.x; v[5] = d.y; v[6] = d.z; v[7] = d.w;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = (live && c + k < C) ? IO::ld1(w, base + c + k) : 0.f;
+    }
+    ms_h8 hi, lo;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) { _Float16 x, y; ce_split(v[k] * inv, x, y); hi[k] = x; lo[k] = y; }
+    *reinterpret_cast<ms_h8*>(out + (size_t)r * Cp + c) = hi;
+    if (PL == 2) *reinterpret_cast<ms_h8*>(out + plane + (size_t)r * Cp + c) = lo;
   }
 }
 
-// h [N][C][HW] -> the same packed rows: a workgroup turns 64 pixels x 64 channels at a time through LDS (reads run along HW, writes along C).
+// h [N][C][HW], HW > 1 -> the same packed rows.  A workgroup takes 64 pixels: a wave reads 64 neighbouring pixels of a channel at a time and writes 8 channels of each.
 template <typename HT, int PL>
-__global__ __launch_bounds__(256) void ce_pack_planes_kernel(const void* __restrict__ h, const int64_t* __restrict__ labels, int classes, int drop, _Float16* __restrict__ out,
-                                                             size_t plane, float* __restrict__ fx, int* __restrict__ lab32, long P, long Pp, int C, int Cp, int HW) {
+__global__ __launch_bounds__(1024) void ce_pack_planes_kernel(const void* __restrict__ h, const int64_t* __restrict__ labels, int classes, int drop, _Float16* __restrict__ out,
+                                                              size_t plane, float* __restrict__ fx, int* __restrict__ lab32, long P, long Pp, int C, int Cp, int HW) {
   using IO = ActIO<HT>;
-  __shared__ _Float16 t[PL][64][64 + 8];
-  __shared__ unsigned smax[4][64];
+  __shared__ unsigned smax[16][64];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const long p = (long)blockIdx.x * 64 + lane;
-  bool live = p < P;
-  if (labels != nullptr) {
-    int y = -1;
-    if (live) { const int64_t l = labels[p]; y = (l >= 0 && l < classes) ? (int)l : -1; }
-    if (wave == 0 && p < Pp) lab32[p] = y;
-    if (drop) live = y >= 0;
-  }
-  const long n = p / HW;
-  const size_t base = (size_t)n * C * HW + (size_t)(p - n * HW);
+  int y = -1;
+  if (p < P) { const int64_t l = labels[p]; y = (l >= 0 && l < classes) ? (int)l : -1; }
+  if (wave == 0) lab32[p] = y;
+  const bool live = p < P && (!drop || y >= 0);
+  const int n = (int)p / HW;
+  const size_t base = (size_t)n * C * HW + (size_t)((int)p - n * HW);
   unsigned am = 0;
-  if (live) for (int c = wave; c < C; c += 4) am = max(am, __float_as_uint(IO::ld1(h, base + (size_t)c * HW)) & 0x7FFFFFFFu);
+  for (int c0 = wave * 8; c0 < C; c0 += 128) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) if (live && c0 + k < C) am = max(am, __float_as_uint(IO::ld1(h, base + (size_t)(c0 + k) * HW)) & 0x7FFFFFFFu);
+  }
   smax[wave][lane] = am;
   __syncthreads();
-  am = max(max(smax[0][lane], smax[1][lane]), max(smax[2][lane], smax[3][lane]));
+#pragma unroll
+  for (int k = 0; k < 16; ++k) am = max(am, smax[k][lane]);
   const int e = ce_exponent(__uint_as_float(am));
   const float inv = ce_pow2(-e);
-  if (wave == 0 && p < Pp) fx[p] = ce_pow2(e);
-  for (int c0 = 0; c0 < Cp; c0 += 64) {
-    __syncthreads();
-    for (int c = wave; c < 64; c += 4) {
-      const float v = (live && c0 + c < C) ? IO::ld1(h, base + (size_t)(c0 + c) * HW) * inv : 0.f;
-      _Float16 hi, lo;
-      ce_split(v, hi, lo);
-      t[0][lane][c] = hi;
-      if (PL == 2) t[1][lane][c] = lo;
+  if (wave == 0) fx[p] = ce_pow2(e);
+  for (int c0 = wave * 8; c0 < Cp; c0 += 128) {
+    ms_h8 hi, lo;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      _Float16 x, z;
+      ce_split((live && c0 + k < C) ? IO::ld1(h, base + (size_t)(c0 + k) * HW) * inv : 0.f, x, z);
+      hi[k] = x; lo[k] = z;
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 64 * 8 * PL; i += 256) {
-      const int pl = i >> 9, row = (i >> 3) & 63, ch = (i & 7) * 8;
-      const long pr = (long)blockIdx.x * 64 + row;
-      if (pr < Pp) *reinterpret_cast<ms_h8*>(out + pl * plane + (size_t)pr * Cp + c0 + ch) = *reinterpret_cast<const ms_h8*>(&t[pl][row][ch]);
-    }
+    *reinterpret_cast<ms_h8*>(out + (size_t)p * Cp + c0) = hi;
+    if (PL == 2) *reinterpret_cast<ms_h8*>(out + plane + (size_t)p * Cp + c0) = lo;
   }
 }
 
@@ -136,29 +152,35 @@ __device__ __forceinline__ int ce_gexp(const int* __restrict__ scal) {
   return (a < -50000 || b < -50000) ? 0 : min(max(kCeTopExp - (a + b), -120), 120);
 }
 
-// part[t][p] = {max, sum exp} over one class range -> lse, nll; loss partials in 64 bits
-__global__ __launch_bounds__(256) void ce_join_kernel(const float2* __restrict__ part, int nparts, size_t stride, const float* __restrict__ zlab, const int* __restrict__ lab32,
-                                                      float* __restrict__ lse, float* __restrict__ lse_out, float* __restrict__ nll_out, double* __restrict__ lsum, long P, long Pp) {
-  __shared__ double redd[16];
-  const long p = (long)blockIdx.x * 256 + threadIdx.x;
+// part[t][p] = {max, sum exp} over one class range -> lse, nll; loss partials in 64 bits.  64 rows a workgroup, 16 threads each over the class ranges.
+__device__ __forceinline__ void ce_merge(float& m, float& l, float mo, float lo) {
+  const float mn = fmaxf(m, mo), mm = mn == -__builtin_inff() ? 0.f : mn;
+  l = l * __builtin_amdgcn_exp2f((m - mm) * kLog2e) + lo * __builtin_amdgcn_exp2f((mo - mm) * kLog2e);
+  m = mn;
+}
+__global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict__ part, int nparts, size_t stride, const float* __restrict__ zlab, const int* __restrict__ lab32,
+                                                       float* __restrict__ lse, float* __restrict__ lse_out, float* __restrict__ nll_out, double* __restrict__ lsum, long P) {
+  __shared__ float2 sh[16][64];
+  const int el = threadIdx.x & 63, grp = threadIdx.x >> 6;
+  const long p = (long)blockIdx.x * 64 + el;          // (padded)
+  float m = -__builtin_inff(), l = 0.f;
+#pragma unroll 4
+  for (int t = grp; t < nparts; t += 16) { const float2 o = part[(size_t)t * stride + p]; ce_merge(m, l, o.x, o.y); }
+  sh[grp][el] = make_float2(m, l);
+  __syncthreads();
+  if (grp != 0) return;
+  for (int k = 1; k < 16; ++k) ce_merge(m, l, sh[k][el].x, sh[k][el].y);
+  const float lg = logf(l), s = m + lg;
+  lse[p] = s;
   double acc = 0.0;
-  if (p < Pp) {
-    float m = -__builtin_inff();
-    for (int t = 0; t < nparts; ++t) { const float o = part[(size_t)t * stride + p].x; m = (o > m || o != o) ? o : m; }
-    const float ms_ = (m == -__builtin_inff()) ? 0.f : m;
-    float l = 0.f;
-    for (int t = 0; t < nparts; ++t) { const float2 o = part[(size_t)t * stride + p]; l += o.y * __builtin_amdgcn_exp2f((o.x - ms_) * kLog2e); }
-    const float lg = logf(l), s = m + lg;
-    lse[p] = s;
-    if (p < P) {
-      if (lse_out != nullptr) lse_out[p] = s;
-      const float v = lab32[p] >= 0 ? (m - zlab[p]) + lg : 0.f;        // (max - z) + log sum: nothing cancels where the label has the maximum
-      if (nll_out != nullptr) nll_out[p] = v;
-      acc = (double)v;
-    }
+  if (p < P) {
+    if (lse_out != nullptr) lse_out[p] = s;
+    const float v = lab32[p] >= 0 ? (m - zlab[p]) + lg : 0.f;        // (max - z) + log sum: nothing cancels where the label has the maximum
+    if (nll_out != nullptr) nll_out[p] = v;
+    acc = (double)v;
   }
-  acc = block_sum_d(acc, redd);
-  if (threadIdx.x == 0) lsum[blockIdx.x] = acc;
+  acc = wave_sum_d(acc);
+  if (el == 0) lsum[blockIdx.x] = acc;
 }
 __global__ __launch_bounds__(256) void ce_loss_kernel(const double* __restrict__ lsum, int n, float sign, int mean_valid, const int* __restrict__ scal, long P, float* __restrict__ loss) {
   __shared__ double redd[16];
@@ -384,42 +406,44 @@ __global__ __launch_bounds__(WM * WN * 64) void ce_gemm_kernel(CeGemm g) {
   }
 }
 
-// Sum of a product's K-splits -> dh or dw.  part [split][M][ld] with M = channels, columns = rows (dh) or M = classes, columns = channels (dw).
+// Sum of a product's K-splits -> dh or dw.  part [split][rows][ld]:
+//   PLANES  rows = channels, columns = pixels of this piece, written as [n][channel][hw];  f = 2^ex of the column
+//   else    rows = classes (dw) or feature rows (dh with HW = 1) of this piece, columns = channels, written as [row][channel];  f = 2^ew / 2^ex of the row
 //   first: nothing is there yet, else the fp32 running sum `acc` is added;  last: written to `out` in its type, else back to `acc`.
-template <typename OT, bool DH>
+template <typename OT, bool PLANES>
 __global__ __launch_bounds__(256) void ce_reduce_kernel(const float* __restrict__ part, size_t out_split, int ld, int split, const float* __restrict__ f, const int* __restrict__ scal,
-                                                        float* __restrict__ acc, void* __restrict__ out, int first, int last, long rows, long r0, int cols, int HW, int C) {
+                                                        float* __restrict__ acc, void* __restrict__ out, int first, int last, int rows, int cols, long r0, int HW, int C) {
   const float gi = ce_pow2(-ce_gexp(scal));
-  const long total = rows * cols;
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
-    size_t src, dst;
-    float fac;
-    if (DH) {                  // rows = pixels of this piece (fastest), cols = channels; with HW = 1 the channels are fastest in the output
-      long p, c;
-      if (HW > 1) { c = i / rows; p = i - c * rows; } else { p = i / cols; c = i - p * cols; }
-      src = (size_t)c * ld + p;
-      const long gpix = r0 + p, n = gpix / HW;
-      dst = ((size_t)n * C + c) * HW + (gpix - n * HW);
-      fac = gi / f[gpix];
-    } else {                   // rows = classes of this piece, cols = channels
-      const long v = i / cols, c = i - v * cols;
-      src = (size_t)v * ld + c;
-      dst = (size_t)(r0 + v) * C + c;
-      fac = gi / f[r0 + v];
-    }
+  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (row >= rows) return;
+  for (int c = blockIdx.y * 64 + lane; c < cols; c += gridDim.y * 64) {
+    const float* src = part + (size_t)row * ld + c;
     float s = 0.f;
-    for (int k = 0; k < split; ++k) s += part[k * out_split + src];
-    s *= fac;
+    for (int k = 0; k < split; ++k) s += src[k * out_split];
+    size_t dst;
+    if (PLANES) {
+      const int p = (int)r0 + c, n = p / HW;
+      dst = ((size_t)n * C + row) * HW + (p - n * HW);
+      s *= gi / f[p];
+    } else {
+      dst = (size_t)(r0 + row) * C + c;
+      s *= gi / f[r0 + row];
+    }
     if (!first) s += acc[dst];
     if (last) ActIO<OT>::st1(out, dst, s); else acc[dst] = s;
   }
 }
-__global__ __launch_bounds__(256) void ce_db_kernel(const float* __restrict__ part, int n, size_t stride, float* __restrict__ db, int first, int V, int v0) {
-  const int v = blockIdx.x * 256 + threadIdx.x;
-  if (v >= V) return;
-  double s = first ? 0.0 : (double)db[v0 + v];
-  for (int i = 0; i < n; ++i) s += (double)part[(size_t)i * stride + v];
-  db[v0 + v] = (float)s;
+__global__ __launch_bounds__(1024) void ce_db_kernel(const float* __restrict__ part, int n, size_t stride, float* __restrict__ db, int first, int V, int v0) {
+  __shared__ double sh[16][64];
+  const int el = threadIdx.x & 63, grp = threadIdx.x >> 6, v = blockIdx.x * 64 + el;
+  double s = 0.0;
+#pragma unroll 4
+  for (int i = grp; i < n; i += 16) s += (double)part[(size_t)i * stride + v];      // (columns padded to whole tiles)
+  sh[grp][el] = s;
+  __syncthreads();
+  if (grp != 0 || v >= V) return;
+  for (int k = 1; k < 16; ++k) s += sh[k][el];
+  db[v0 + v] = (float)(first ? s : s + (double)db[v0 + v]);
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------ host
@@ -440,8 +464,10 @@ static CePlan ce_plan(int N, int C, int V, int HW, int types, bool grad) {
   k.Pp = ce_up(k.P, kCePad); k.Vp = (int)ce_up(V, kCePad); k.Cp = (int)ce_up(C, kCeBK);
   k.xp = (types & 1) ? 1 : 2; k.wp = (types & 2) ? 1 : 2;
   k.gpl = (k.xp == 2 || k.wp == 2) ? 2 : 1;
-  k.vb = std::min(k.Vp, 8192);
-  k.pb = (int)std::min<long>(k.Pp, std::max<long>(kCePad, (long)(kCePieceBytes / ((size_t)k.vb * 2 * k.gpl)) / kCePad * kCePad));
+  // Pieces of G: up to 8192 classes, and as many rows as kCePieceBytes holds, both cut evenly (6 pieces of 90 % fill the chip better than 5 whole ones and a scrap).
+  auto even = [](long n, long most) { return ce_up((n + (n + most - 1) / most - 1) / ((n + most - 1) / most), kCePad); };
+  k.vb = (int)even(k.Vp, 8192);
+  k.pb = (int)even(k.Pp, std::max<long>(kCePad, (long)(kCePieceBytes / ((size_t)k.vb * 2 * k.gpl)) / kCePad * kCePad));
   k.nparts = k.Vp / 128 * 2;
   size_t o = 0;
   auto take = [&](size_t n) { const size_t at = o; o += ce_al(n); return at; };
@@ -450,7 +476,7 @@ static CePlan ce_plan(int N, int C, int V, int HW, int types, bool grad) {
   k.o_fx = take(k.Pp * 4); k.o_fw = take((size_t)k.Vp * 4); k.o_b = take((size_t)k.Vp * 4);
   k.o_lab = take(k.Pp * 4); k.o_lse = take(k.Pp * 4); k.o_zl = take(k.Pp * 4); k.o_gp = take(k.Pp * 4);
   k.o_scal = take(64);
-  k.o_lsum = take((size_t)(k.Pp / 256) * 8);
+  k.o_lsum = take((size_t)(k.Pp / 64) * 8);
   const size_t stats = (size_t)k.nparts * k.Pp * 8;
   if (!grad) { k.o_part = take(stats); k.total = o; return k; }
   // The statistics are read before the first piece of G is written: they share its memory.
@@ -503,17 +529,29 @@ static int ce_run(const CeArgs& a, const char* who) {
   float *fx = f32(k.o_fx), *fw = f32(k.o_fw), *bp = f32(k.o_b), *lse = f32(k.o_lse), *zl = f32(k.o_zl), *gp = f32(k.o_gp);
   hipStream_t st = a.st;
   MS_LAUNCH(ce_init_kernel, dim3(1), dim3(64), 0, st, scal);
-  if (int e = check_launch("ce_init")) return e;
-  if (a.types & 2) MS_LAUNCH((ce_pack_rows_kernel<ms_bf16, 1>), dim3(k.Vp / 4), dim3(256), 0, st, a.w, a.b, (const int64_t*)nullptr, 0, w, wpl, fw, bp, (int*)nullptr, scal, a.V, k.Vp, a.C, k.Cp);
-  else MS_LAUNCH((ce_pack_rows_kernel<float, 2>), dim3(k.Vp / 4), dim3(256), 0, st, a.w, a.b, (const int64_t*)nullptr, 0, w, wpl, fw, bp, (int*)nullptr, scal, a.V, k.Vp, a.C, k.Cp);
-  if (int e = check_launch("ce_pack_w")) return e;
-  const dim3 gx((unsigned)(k.Pp / 64));
-  if (a.types & 1) MS_LAUNCH((ce_pack_planes_kernel<ms_bf16, 1>), gx, dim3(256), 0, st, a.h, a.labels, a.V, need_grad ? 1 : 0, x, xpl, fx, lab, k.P, k.Pp, a.C, k.Cp, a.HW);
-  else MS_LAUNCH((ce_pack_planes_kernel<float, 2>), gx, dim3(256), 0, st, a.h, a.labels, a.V, need_grad ? 1 : 0, x, xpl, fx, lab, k.P, k.Pp, a.C, k.Cp, a.HW);
-  if (int e = check_launch("ce_pack_h")) return e;
+  if (int e = check_launch("class_ce_init")) return e;
+  auto pack_rows = [&](const void* src, bool bf, const float* b, const int64_t* labels, _Float16* out, size_t pl, float* f, float* bpad, int rows, int rows_pad) {
+    const bool vec = a.C % 8 == 0 && aligned16(src);
+    const dim3 grid(rows_pad / 4), block(256);
+    const int drop = need_grad ? 1 : 0;
+    if (bf && vec) MS_LAUNCH((ce_pack_rows_kernel<ms_bf16, 1, true>), grid, block, 0, st, src, b, labels, a.V, drop, out, pl, f, bpad, lab, scal, rows, rows_pad, a.C, k.Cp);
+    else if (bf) MS_LAUNCH((ce_pack_rows_kernel<ms_bf16, 1, false>), grid, block, 0, st, src, b, labels, a.V, drop, out, pl, f, bpad, lab, scal, rows, rows_pad, a.C, k.Cp);
+    else if (vec) MS_LAUNCH((ce_pack_rows_kernel<float, 2, true>), grid, block, 0, st, src, b, labels, a.V, drop, out, pl, f, bpad, lab, scal, rows, rows_pad, a.C, k.Cp);
+    else MS_LAUNCH((ce_pack_rows_kernel<float, 2, false>), grid, block, 0, st, src, b, labels, a.V, drop, out, pl, f, bpad, lab, scal, rows, rows_pad, a.C, k.Cp);
+    return check_launch("class_ce_pack");
+  };
+  if (int e = pack_rows(a.w, (a.types & 2) != 0, a.b, nullptr, w, wpl, fw, bp, a.V, k.Vp)) return e;
+  if (a.HW == 1) {
+    if (int e = pack_rows(a.h, (a.types & 1) != 0, nullptr, a.labels, x, xpl, fx, nullptr, a.N, (int)k.Pp)) return e;
+  } else {
+    const dim3 gx((unsigned)(k.Pp / 64));
+    if (a.types & 1) MS_LAUNCH((ce_pack_planes_kernel<ms_bf16, 1>), gx, dim3(1024), 0, st, a.h, a.labels, a.V, need_grad ? 1 : 0, x, xpl, fx, lab, k.P, k.Pp, a.C, k.Cp, a.HW);
+    else MS_LAUNCH((ce_pack_planes_kernel<float, 2>), gx, dim3(1024), 0, st, a.h, a.labels, a.V, need_grad ? 1 : 0, x, xpl, fx, lab, k.P, k.Pp, a.C, k.Cp, a.HW);
+    if (int e = check_launch("class_ce_pack")) return e;
+  }
   if (a.mean_valid) {
     MS_LAUNCH(ce_count_kernel, dim3((unsigned)std::min<long>(cdiv((int)std::min<long>(k.P, 1 << 30), 1024), 1024)), dim3(256), 0, st, a.labels, k.P, a.V, scal);
-    if (int e = check_launch("ce_count")) return e;
+    if (int e = check_launch("class_ce_count")) return e;
   }
   CeGemm g{};
   g.fw = fw; g.bpad = bp; g.fx = fx; g.lab = lab; g.lse = lse; g.gp = gp; g.scal = scal; g.zlab = zl;
@@ -523,17 +561,17 @@ static int ce_run(const CeArgs& a, const char* who) {
     ce_pairs(g, k.wp, k.xp);
     g.ksteps = k.Cp / kCeBK; g.mt = k.Vp / 128; g.nt = (int)(k.Pp / 128); g.split = 1;
     g.part = (float2*)(ws + k.o_part); g.part_stride = (size_t)k.Pp;
-    if (int e = ce_gemm<CE_STATS, false, false>(g, st, "ce_stats")) return e;
-    MS_LAUNCH(ce_join_kernel, dim3((unsigned)(k.Pp / 256)), dim3(256), 0, st, (const float2*)g.part, k.nparts, g.part_stride, zl, lab, lse, a.lse, a.nll, (double*)(ws + k.o_lsum), k.P, k.Pp);
-    if (int e = check_launch("ce_join")) return e;
+    if (int e = ce_gemm<CE_STATS, false, false>(g, st, "class_ce_stats")) return e;
+    MS_LAUNCH(ce_join_kernel, dim3((unsigned)(k.Pp / 64)), dim3(1024), 0, st, (const float2*)g.part, k.nparts, g.part_stride, zl, lab, lse, a.lse, a.nll, (double*)(ws + k.o_lsum), k.P);
+    if (int e = check_launch("class_ce_join")) return e;
     if (a.loss != nullptr) {
-      MS_LAUNCH(ce_loss_kernel, dim3(1), dim3(256), 0, st, (const double*)(ws + k.o_lsum), (int)(k.Pp / 256), a.sign, a.mean_valid, scal, k.P, a.loss);
-      if (int e = check_launch("ce_loss")) return e;
+      MS_LAUNCH(ce_loss_kernel, dim3(1), dim3(256), 0, st, (const double*)(ws + k.o_lsum), (int)(k.Pp / 64), a.sign, a.mean_valid, scal, k.P, a.loss);
+      if (int e = check_launch("class_ce_loss")) return e;
     }
   }
   if (!need_grad) return MS_OK;
   MS_LAUNCH(ce_rowgrad_kernel, dim3((unsigned)std::min<long>(k.Pp / 256, 1024)), dim3(256), 0, st, a.grad, a.sign, a.mean_valid, a.scale_dev, lab, fx, gp, a.lse_in, lse, scal, k.P, k.Pp);
-  if (int e = check_launch("ce_rowgrad")) return e;
+  if (int e = check_launch("class_ce_rowgrad")) return e;
   const long cp = ce_up(k.Cp, 128);
   for (long p0 = 0; p0 < k.Pp; p0 += k.pb) {
     const int pn = (int)std::min<long>(k.pb, k.Pp - p0);
@@ -547,44 +585,53 @@ static int ce_run(const CeArgs& a, const char* who) {
       const size_t gpl = (size_t)k.pb * k.vb;
       d.g = G; d.g_plane = gpl; d.g_ld = k.vb;
       d.dbpart = a.db != nullptr ? f32(k.o_db) : nullptr; d.db_stride = k.vb;
-      if (k.gpl == 2) { if (int e = ce_gemm<CE_GRAD2, false, false>(d, st, "ce_grad")) return e; }
-      else { if (int e = ce_gemm<CE_GRAD, false, false>(d, st, "ce_grad")) return e; }
+      if (k.gpl == 2) { if (int e = ce_gemm<CE_GRAD2, false, false>(d, st, "class_ce_grad")) return e; }
+      else { if (int e = ce_gemm<CE_GRAD, false, false>(d, st, "class_ce_grad")) return e; }
       if (a.db != nullptr) {
         const int vr = std::min(vn, a.V - v0);
         if (vr > 0) {
-          MS_LAUNCH(ce_db_kernel, dim3(cdiv(vr, 256)), dim3(256), 0, st, f32(k.o_db), pn / 128 * 2, (size_t)k.vb, a.db, p0 == 0 ? 1 : 0, vr, v0);
-          if (int e = check_launch("ce_db")) return e;
+          MS_LAUNCH(ce_db_kernel, dim3(cdiv(vr, 64)), dim3(1024), 0, st, f32(k.o_db), pn / 128 * 2, (size_t)k.vb, a.db, p0 == 0 ? 1 : 0, vr, v0);
+          if (int e = check_launch("class_ce_db")) return e;
         }
       }
-      if (a.dh != nullptr) {        // dh^T [channels][rows] = w^T G^T
+      if (a.dh != nullptr) {        // dh^T [channels][pixels] = w^T G^T, or dh [rows][channels] = G w where the channels are neighbours
+        const bool rows_form = a.HW == 1;
         CeGemm o{};
-        o.a = CeOperand{w + (size_t)v0 * k.Cp, wpl, k.Cp, k.Cp}; o.b = CeOperand{G, gpl, k.vb, 0};
-        ce_pairs(o, (a.types & 1) ? 1 : k.wp, (a.types & 1) ? 1 : 2);
-        o.ksteps = vn / kCeBK; o.mt = (int)(cp / 128); o.nt = pn / 128; o.split = k.split_x;
-        o.out = f32(k.o_px); o.out_ld = k.pb; o.out_split = (size_t)cp * k.pb;
-        if (int e = ce_gemm<CE_OUT, true, false>(o, st, "ce_dh")) return e;
-        const long rows = std::min<long>(pn, k.P - p0);
-        const int first = v0 == 0, last = v0 + vn >= k.Vp;
-        const dim3 grid((unsigned)std::min<long>((rows * a.C + 255) / 256, 8192));
+        const CeOperand ow{w + (size_t)v0 * k.Cp, wpl, k.Cp, k.Cp}, og{G, gpl, k.vb, 0};
+        const int pw = (a.types & 1) ? 1 : k.wp, pg = (a.types & 1) ? 1 : 2;
+        o.ksteps = vn / kCeBK; o.split = std::min(k.split_x, std::max(1, o.ksteps / 8));
+        o.out = f32(k.o_px); o.out_split = (size_t)cp * k.pb;
+        const int rows = (int)std::min<long>(pn, k.P - p0), first = v0 == 0, last = v0 + vn >= k.Vp;
         float* ac = (a.types & 1) ? f32(k.o_ax) : (float*)a.dh;
-        if (a.types & 1) MS_LAUNCH((ce_reduce_kernel<ms_bf16, true>), grid, dim3(256), 0, st, o.out, o.out_split, o.out_ld, o.split, fx, scal, ac, a.dh, first, last, rows, p0, a.C, a.HW, a.C);
-        else MS_LAUNCH((ce_reduce_kernel<float, true>), grid, dim3(256), 0, st, o.out, o.out_split, o.out_ld, o.split, fx, scal, ac, a.dh, first, last, rows, p0, a.C, a.HW, a.C);
-        if (int e = check_launch("ce_dh_sum")) return e;
+        if (rows_form) {
+          o.a = og; o.b = ow; ce_pairs(o, pg, pw); o.mt = pn / 128; o.nt = (int)(cp / 128); o.out_ld = (int)cp;
+          if (int e = ce_gemm<CE_OUT, false, true>(o, st, "class_ce_dh")) return e;
+          const dim3 grid((unsigned)cdiv(rows, 4), (unsigned)std::min(cdiv(a.C, 64), 4));
+          if (a.types & 1) MS_LAUNCH((ce_reduce_kernel<ms_bf16, false>), grid, dim3(256), 0, st, o.out, o.out_split, o.out_ld, o.split, fx, scal, ac, a.dh, first, last, rows, a.C, p0, 1, a.C);
+          else MS_LAUNCH((ce_reduce_kernel<float, false>), grid, dim3(256), 0, st, o.out, o.out_split, o.out_ld, o.split, fx, scal, ac, a.dh, first, last, rows, a.C, p0, 1, a.C);
+        } else {
+          o.a = ow; o.b = og; ce_pairs(o, pw, pg); o.mt = (int)(cp / 128); o.nt = pn / 128; o.out_ld = k.pb;
+          if (int e = ce_gemm<CE_OUT, true, false>(o, st, "class_ce_dh")) return e;
+          const dim3 grid((unsigned)cdiv(a.C, 4), (unsigned)std::min(cdiv(rows, 64), 64));
+          if (a.types & 1) MS_LAUNCH((ce_reduce_kernel<ms_bf16, true>), grid, dim3(256), 0, st, o.out, o.out_split, o.out_ld, o.split, fx, scal, ac, a.dh, first, last, a.C, rows, p0, a.HW, a.C);
+          else MS_LAUNCH((ce_reduce_kernel<float, true>), grid, dim3(256), 0, st, o.out, o.out_split, o.out_ld, o.split, fx, scal, ac, a.dh, first, last, a.C, rows, p0, a.HW, a.C);
+        }
+        if (int e = check_launch("class_ce_dh_sum")) return e;
       }
       const int vr = std::min(vn, a.V - v0);
       if (a.dw != nullptr && vr > 0) {        // dw [classes][channels] = G^T h
         CeGemm o{};
         o.a = CeOperand{G, gpl, k.vb, k.vb}; o.b = CeOperand{x + (size_t)p0 * k.Cp, xpl, k.Cp, k.Cp};
         ce_pairs(o, (a.types & 2) ? 1 : 2, (a.types & 2) ? 1 : k.xp);
-        o.ksteps = pn / kCeBK; o.mt = vn / 128; o.nt = (int)(cp / 128); o.split = k.split_w;
+        o.ksteps = pn / kCeBK; o.mt = vn / 128; o.nt = (int)(cp / 128); o.split = std::min(k.split_w, std::max(1, o.ksteps / 8));
         o.out = f32(k.o_pw); o.out_ld = (int)cp; o.out_split = (size_t)k.vb * cp;
-        if (int e = ce_gemm<CE_OUT, true, true>(o, st, "ce_dw")) return e;
+        if (int e = ce_gemm<CE_OUT, true, true>(o, st, "class_ce_dw")) return e;
         const int first = p0 == 0, last = p0 + pn >= k.Pp;
-        const dim3 grid((unsigned)std::min<long>(((long)vr * a.C + 255) / 256, 8192));
+        const dim3 grid((unsigned)cdiv(vr, 4), (unsigned)std::min(cdiv(a.C, 64), 4));
         float* ac = (a.types & 2) ? f32(k.o_aw) : (float*)a.dw;
-        if (a.types & 2) MS_LAUNCH((ce_reduce_kernel<ms_bf16, false>), grid, dim3(256), 0, st, o.out, o.out_split, o.out_ld, o.split, fw, scal, ac, a.dw, first, last, (long)vr, (long)v0, a.C, 1, a.C);
-        else MS_LAUNCH((ce_reduce_kernel<float, false>), grid, dim3(256), 0, st, o.out, o.out_split, o.out_ld, o.split, fw, scal, ac, a.dw, first, last, (long)vr, (long)v0, a.C, 1, a.C);
-        if (int e = check_launch("ce_dw_sum")) return e;
+        if (a.types & 2) MS_LAUNCH((ce_reduce_kernel<ms_bf16, false>), grid, dim3(256), 0, st, o.out, o.out_split, o.out_ld, o.split, fw, scal, ac, a.dw, first, last, vr, a.C, (long)v0, 1, a.C);
+        else MS_LAUNCH((ce_reduce_kernel<float, false>), grid, dim3(256), 0, st, o.out, o.out_split, o.out_ld, o.split, fw, scal, ac, a.dw, first, last, vr, a.C, (long)v0, 1, a.C);
+        if (int e = check_launch("class_ce_dw_sum")) return e;
       }
     }
   }

@@ -92,13 +92,13 @@ __global__ __launch_bounds__(256) void cn_prep_kernel(const void* __restrict__ w
 }
 
 // {rows that take part, max ew} from the prep pass's slots (at most 256: one a thread)
-__device__ __forceinline__ int2 cn_slots(const int2* __restrict__ slots, int n, int* red /*8*/) {
+__device__ __forceinline__ int2 cn_slots(const int2* __restrict__ slots, int n, int* red /* 2 x waves */) {
   int2 s = threadIdx.x < (unsigned)n ? slots[threadIdx.x] : make_int2(0, -100000);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) { s.x += __shfl_xor(s.x, off, 64); s.y = max(s.y, __shfl_xor(s.y, off, 64)); }
-  if ((threadIdx.x & 63) == 0) { red[threadIdx.x >> 6] = s.x; red[4 + (threadIdx.x >> 6)] = s.y; }
+  if ((threadIdx.x & 63) == 0) { red[2 * (threadIdx.x >> 6)] = s.x; red[2 * (threadIdx.x >> 6) + 1] = s.y; }
   __syncthreads();
-  return make_int2(red[0] + red[1] + red[2] + red[3], max(max(red[4], red[5]), max(red[6], red[7])));
+  return make_int2(red[0] + red[2] + red[4] + red[6], max(max(red[1], red[3]), max(red[5], red[7])));      // (the slots lie in the first four waves)
 }
 
 template <int WP, int KS>
@@ -577,33 +577,42 @@ __global__ __launch_bounds__(256) void cn_classes_kernel(CnwArgs a) {
   }
 }
 
-// dw, db: sums of the splits; the loss (last workgroup)
+// dw, db: sums of the splits in a fixed order; the loss (last workgroup).  A workgroup sums 64 elements, 16 threads each.
 template <typename WT>
-__global__ __launch_bounds__(256) void cn_join_kernel(const float* __restrict__ dwp, const float* __restrict__ dbp, size_t dw_split, int db_split, int splits, void* __restrict__ dw,
-                                                      float* __restrict__ db, int V, int C, int kC, const double* __restrict__ lsum, int nl, const int2* __restrict__ slots, int nslots,
-                                                      float sign, int mean_valid, long P, float* __restrict__ loss) {
+__global__ __launch_bounds__(1024) void cn_join_kernel(const float* __restrict__ dwp, const float* __restrict__ dbp, size_t dw_split, int db_split, int splits, void* __restrict__ dw,
+                                                       float* __restrict__ db, int V, int C, int kC, int dw_blocks, const double* __restrict__ lsum, int nl, const int2* __restrict__ slots,
+                                                       int nslots, float sign, int mean_valid, long P, float* __restrict__ loss) {
   __shared__ double redd[16];
-  __shared__ int redi[8];
+  __shared__ int redi[32];
+  __shared__ float part[16][64];
   if (blockIdx.x == gridDim.x - 1 && loss != nullptr) {
     const int2 s = cn_slots(slots, nslots, redi);
     double a = 0.0;
-    for (int i = threadIdx.x; i < nl; i += 256) a += lsum[i];
+    for (int i = threadIdx.x; i < nl; i += 1024) a += lsum[i];
     a = block_sum_d(a, redd);
     if (threadIdx.x == 0) loss[0] = (float)((double)sign * a / (double)(mean_valid ? max(s.x, 1) : P));
     return;
   }
-  const int i = blockIdx.x * 256 + threadIdx.x, total = dw != nullptr ? V * C : 0;
+  const bool isw = blockIdx.x < (unsigned)dw_blocks;
+  const int el = threadIdx.x & 63, grp = threadIdx.x >> 6;
+  const int i = (isw ? blockIdx.x : blockIdx.x - dw_blocks) * 64 + el, total = isw ? V * kC : V;
+  const float* src = isw ? dwp : dbp;
+  const size_t stride = isw ? dw_split : (size_t)db_split;
+  float a = 0.f;
   if (i < total) {
-    const int v = i / C, c = i - v * C;
-    const float* s = dwp + (size_t)v * kC + c;
-    float a = 0.f;
-    for (int k = 0; k < splits; ++k) a += s[k * dw_split];
-    ActIO<WT>::st1(dw, i, a);
-  } else if (db != nullptr && i - total < V) {
-    const int v = i - total;
-    double a = 0.0;
-    for (int k = 0; k < splits; ++k) a += (double)dbp[(size_t)k * db_split + v];
-    db[v] = (float)a;
+#pragma unroll 8
+    for (int k = grp; k < splits; k += 16) a += src[k * stride + i];
+  }
+  part[grp][el] = a;
+  __syncthreads();
+  if (grp != 0 || i >= total) return;
+#pragma unroll
+  for (int k = 1; k < 16; ++k) a += part[k][el];
+  if (isw) {
+    const int v = i / kC, c = i - v * kC;
+    if (c < C) ActIO<WT>::st1(dw, (size_t)v * C + c, a);
+  } else {
+    db[i] = a;
   }
 }
 
@@ -628,7 +637,7 @@ static CnPlan cn_plan(int N, int C, int V, int HW, int types, bool grad) {
   k.wpx = std::min(k.wpx, k.tp / 32);
   k.vblocks = cdiv(k.units, 4 / k.wpx);
   k.tiles = (int)((k.P + k.tp - 1) / k.tp);
-  k.splits = (int)std::max<long>(1, std::min<long>(k.tiles, 768 / std::min(k.vblocks, 768)));
+  k.splits = (int)std::max<long>(1, std::min<long>(k.tiles, 512 / std::min(k.vblocks, 512)));
   size_t o = 0;
   auto take = [&](size_t n) { const size_t at = o; o += (n + 255) & ~(size_t)255; return at; };
   k.o_img = take((size_t)k.nch * ((size_t)((types & 2) ? 1 : 2) * 64 * k.KS * 64 + 1024));
@@ -696,10 +705,10 @@ static int cn_run(const CeArgs& a, const CnPlan& k) {
     if (int e = check_launch("class_ce_classes")) return e;
   }
   if (need_dw || a.loss != nullptr) {
-    const long n = (a.dw != nullptr ? (long)a.V * a.C : 0) + (a.db != nullptr ? a.V : 0);
-    const unsigned blocks = (unsigned)((n + 255) / 256) + (a.loss != nullptr ? 1u : 0u);
-    MS_LAUNCH((cn_join_kernel<WT>), dim3(blocks), block, 0, st, (const float*)(ws + k.o_dw), (const float*)(ws + k.o_db), (size_t)k.Vp * KS * 32, k.Vp, k.splits * k.wpx, a.dw, a.db,
-              a.V, a.C, KS * 32, p.lsum, (int)k.wgs, slots, k.nslots, a.sign, a.mean_valid, k.P, a.loss);
+    const int wb = a.dw != nullptr ? cdiv(a.V * KS * 32, 64) : 0;
+    const unsigned blocks = (unsigned)(wb + (a.db != nullptr ? cdiv(a.V, 64) : 0) + (a.loss != nullptr ? 1 : 0));
+    MS_LAUNCH((cn_join_kernel<WT>), dim3(blocks), dim3(1024), 0, st, (const float*)(ws + k.o_dw), (const float*)(ws + k.o_db), (size_t)k.Vp * KS * 32, k.Vp, k.splits * k.wpx, a.dw, a.db,
+              a.V, a.C, KS * 32, wb, p.lsum, (int)k.wgs, slots, k.nslots, a.sign, a.mean_valid, k.P, a.loss);
     if (int e = check_launch("class_ce_join")) return e;
   }
   return MS_OK;
