@@ -144,7 +144,7 @@ __global__ __launch_bounds__(256) void ce_rowgrad_kernel(const float* __restrict
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) e = max(e, __shfl_xor(e, off, 64));
-  if ((threadIdx.x & 63) == 0 && e > -100000) atomicMax(&scal[1], e);
+  if ((threadIdx.x & 63) == 0 && e > __hip_atomic_load(&scal[1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(&scal[1], e);
 }
 // 2^k that brings the largest |G| 2^(ex + ew) below 2^14; and its reciprocal
 __device__ __forceinline__ int ce_gexp(const int* __restrict__ scal) {

@@ -1,13 +1,14 @@
 // Head + softmax cross entropy over many classes, narrow form (C <= 128): no operand and no product ever leaves the chip; see ms_class_ce.h.
 //
-//   prep    w -> fp16 planes in the order the LDS wants them, 64 classes a chunk (an "image": the next kernel's DMA copies it as it lies); rows that take part counted
-//   pixels  a wave keeps NJ x 16 pixels' features in registers (one read of h), runs over the classes twice: (max, sum exp) first, then G = exp(z - lse) - hot,
-//           which is already in the register layout the second product wants, and dh += w^T G.  One read of h, one write of dh, w from L2.
+//   prep    w -> fp16 planes in the order the LDS wants them, 64 classes a chunk with one power-of-two scale (an "image": the next kernel's DMA copies it as it
+//           lies); rows that take part counted
+//   pixels  a wave keeps NJ x 16 pixels' features in registers (one read of h) and runs over the classes once: e = exp(z - m) against a running maximum m is already
+//           in the register layout the second product wants, o += w^T e, l += e; at the end dh = g (o / l - w[label]).  One read of h, one write of dh, w from L2.
 //   classes roles exchanged: a wave keeps NJ x 16 classes' weights in registers and runs over pixels: z again, G, dw += h G^T, db += G.  Pixels are split over
 //           workgroups; the partial dw are summed by
 //   join    in a fixed order, with the loss.
-// 10 P V C products instead of 8 (z is formed three times), but nothing of size P V is stored.  The vector unit, not the matrix cores, sets the time: about 6 operations
-// a logit for the statistics, 11 for each G (exp2 counts 4).
+// 8 P V C products, and nothing of size P V is stored.  The vector unit, not the matrix cores, sets the time: about 8 operations a logit in the pixel pass and 10 in
+// the class pass, and an exp2, which counts 4.
 #include <algorithm>
 #include "ms_class_ce.h"
 #include "ms_class_ce_narrow.h"
@@ -22,7 +23,7 @@ constexpr int kCnPrep = 256;          // most workgroups of the prep pass
 template <int KS> __device__ __forceinline__ int cn_swz(int r) { return KS == 1 ? (r >> 1) & 3 : (KS == 3 ? (r >> 2) & 3 : r & 7); }
 template <int KS, int WP> struct CnImage {
   static constexpr int kPlane = kCnClasses * KS * 32;                    // halves of one plane
-  static constexpr int kBytes = WP * kPlane * 2 + 1024;                  // + 64 x {2^ew log2(e)}, 64 x {b log2(e)}, 64 x {ew}
+  static constexpr int kBytes = WP * kPlane * 2 + 1024;                  // + 64 x {b log2(e)}, 2^e log2(e), 2^e of the chunk
 };
 
 // transposing read: lane (q, i) gets column mn + i of rows k .. k + 3, k = k0 + 4 q (swizzled tile of KS * 32 columns)
@@ -37,68 +38,69 @@ __device__ __forceinline__ ms_h8 cn_tr2(const _Float16* tile, int k0, int k1, in
   return u.h;
 }
 
-// slots[block] = {rows that take part, max ew}; scal[1] is made ready for the pixel pass
+// One workgroup a chunk of classes (the first nch), and all of them count: slots[block] = rows that take part.  scal[1] is made ready for the pixel pass.
+// One scale for 64 classes: a weight is held to 2^-22, or 2^-39 of the chunk's largest - an absolute error that no logit notices.
 template <typename WT, int WP, int KS>
 __global__ __launch_bounds__(256) void cn_prep_kernel(const void* __restrict__ w, const float* __restrict__ b, const int64_t* __restrict__ labels, long P, int count,
-                                                      char* __restrict__ img, int2* __restrict__ slots, int* __restrict__ scal, int V, int Vp, int C) {
+                                                      char* __restrict__ img, int* __restrict__ slots, int nslots, int* __restrict__ scal, int V, int nch, int C) {
   using IO = ActIO<WT>;
   using IM = CnImage<KS, WP>;
-  __shared__ int red[2][4];
+  __shared__ int red[4];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   if (blockIdx.x == 0 && threadIdx.x == 0) scal[1] = -100000;
-  int emax = -100000;
-  for (int v = blockIdx.x * 4 + wave; v < Vp; v += gridDim.x * 4) {
-    float x[2];
+  if ((int)blockIdx.x < nch) {
+    const int v0 = blockIdx.x * 64;
+    constexpr int kPer = 64 * KS * 32 / 256;
+    float x[kPer];
     unsigned am = 0;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int c = lane + 64 * k;
-      x[k] = (v < V && c < C) ? IO::ld1(w, (size_t)v * C + c) : 0.f;
-      am = max(am, __float_as_uint(x[k]) & 0x7FFFFFFFu);
+    for (int k = 0; k < kPer; ++k) {
+      const int i = k * 256 + threadIdx.x, r = i / (KS * 32), c = i % (KS * 32);
+      x[k] = (v0 + r < V && c < C) ? IO::ld1(w, (size_t)(v0 + r) * C + c) : 0.f;
+      const unsigned bits = __float_as_uint(x[k]) & 0x7FFFFFFFu;
+      am = max(am, bits < 0x7F800000u ? bits : 0u);          // (an infinity or NaN spoils its own class only)
     }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) am = max(am, (unsigned)__shfl_xor((int)am, off, 64));
+    if (lane == 0) red[wave] = (int)am;
+    __syncthreads();
+    am = max(max((unsigned)red[0], (unsigned)red[1]), max((unsigned)red[2], (unsigned)red[3]));
+    __syncthreads();
     const int e = ce_exponent(__uint_as_float(am));
     const float inv = ce_pow2(-e);
-    char* im = img + (size_t)(v >> 6) * IM::kBytes;
+    char* im = img + (size_t)blockIdx.x * IM::kBytes;
     _Float16* pl = (_Float16*)im;
-    const int r = v & 63;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int c = lane + 64 * k;
-      if (c < KS * 32) {
-        _Float16 hi, lo;
-        ce_split(x[k] * inv, hi, lo);
-        const int at = r * (KS * 32) + (((c >> 3) ^ cn_swz<KS>(r)) * 8) + (c & 7);
-        pl[at] = hi;
-        if (WP == 2) pl[IM::kPlane + at] = lo;
-      }
+    for (int k = 0; k < kPer; ++k) {
+      const int i = k * 256 + threadIdx.x, r = i / (KS * 32), c = i % (KS * 32);
+      _Float16 hi, lo;
+      ce_split(x[k] * inv, hi, lo);
+      const int at = r * (KS * 32) + (((c >> 3) ^ cn_swz<KS>(r)) * 8) + (c & 7);
+      pl[at] = hi;
+      if (WP == 2) pl[IM::kPlane + at] = lo;
     }
-    if (lane == 0) {
-      float* t = (float*)(im + WP * IM::kPlane * 2);
-      t[r] = ce_pow2(e) * kLog2e;
-      t[64 + r] = v < V ? (b != nullptr ? b[v] * kLog2e : 0.f) : -__builtin_inff();
-      t[128 + r] = (float)e;
-      if (v < V) emax = max(emax, e);
-    }
+    float* t = (float*)(im + WP * IM::kPlane * 2);
+    if (threadIdx.x < 64) t[threadIdx.x] = v0 + (int)threadIdx.x < V ? (b != nullptr ? b[v0 + threadIdx.x] * kLog2e : 0.f) : -__builtin_inff();
+    if (threadIdx.x == 64) { t[64] = ce_pow2(e) * kLog2e; t[65] = ce_pow2(e); }
   }
+  if (!count || (int)blockIdx.x >= nslots) return;
   int k = 0;
-  if (count) for (long p = (long)blockIdx.x * 256 + threadIdx.x; p < P; p += (long)gridDim.x * 256) { const int64_t l = labels[p]; k += (l >= 0 && l < V) ? 1 : 0; }
+  for (long p = (long)blockIdx.x * 256 + threadIdx.x; p < P; p += (long)nslots * 256) { const int64_t l = labels[p]; k += (l >= 0 && l < V) ? 1 : 0; }
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) { k += __shfl_xor(k, off, 64); emax = max(emax, __shfl_xor(emax, off, 64)); }
-  if (lane == 0) { red[0][wave] = k; red[1][wave] = emax; }
+  for (int off = 32; off > 0; off >>= 1) k += __shfl_xor(k, off, 64);
+  if (lane == 0) red[wave] = k;
   __syncthreads();
-  if (threadIdx.x == 0) slots[blockIdx.x] = make_int2(red[0][0] + red[0][1] + red[0][2] + red[0][3], max(max(red[1][0], red[1][1]), max(red[1][2], red[1][3])));
+  if (threadIdx.x == 0) slots[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
 }
 
-// {rows that take part, max ew} from the prep pass's slots (at most 256: one a thread)
-__device__ __forceinline__ int2 cn_slots(const int2* __restrict__ slots, int n, int* red /* 2 x waves */) {
-  int2 s = threadIdx.x < (unsigned)n ? slots[threadIdx.x] : make_int2(0, -100000);
+// rows that take part, from the prep pass's slots (at most 256: one a thread of the first four waves)
+__device__ __forceinline__ int cn_count(const int* __restrict__ slots, int n, int* red /* a word a wave */) {
+  int s = threadIdx.x < (unsigned)n ? slots[threadIdx.x] : 0;
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) { s.x += __shfl_xor(s.x, off, 64); s.y = max(s.y, __shfl_xor(s.y, off, 64)); }
-  if ((threadIdx.x & 63) == 0) { red[2 * (threadIdx.x >> 6)] = s.x; red[2 * (threadIdx.x >> 6) + 1] = s.y; }
+  for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
-  return make_int2(red[0] + red[2] + red[4] + red[6], max(max(red[1], red[3]), max(red[5], red[7])));      // (the slots lie in the first four waves)
+  return red[0] + red[1] + red[2] + red[3];
 }
 
 template <int WP, int KS>
@@ -109,59 +111,59 @@ __device__ __forceinline__ void cn_stage(const char* img, int chunk, unsigned ld
 }
 
 struct CnArgs {
-  const void *h; const int64_t* labels; const char* img; const int2* slots; int nslots; int* scal;
+  const void *h, *w; const int64_t* labels; const char* img; const int* slots; int nslots; int* scal;
   float *nll, *lse_out; const float *lse_in, *grad, *scale_dev; float sign; int mean_valid, drop;
   void* dh; double* lsum;
   float *fx, *lse2, *gp; int* lab;          // what the class pass needs of every row (NULL: it does not run)
   long P; int C, HW, V, nch;
 };
 
-template <typename HT, int HP, int WP, int KS, int NJ>
-__global__ __launch_bounds__(256) void cn_pixels_kernel(CnArgs a) {
+// The running maximum m is moved only when a logit exceeds it by more than 1 (in log2), for a whole wave at once: e = 2^(14 + z - m) then stays below 2^15 in fp16, and
+// most classes after the first cost no rescaling.  With the log-sum given (lse_in) m is that, and never moves.
+template <typename HT, typename WT, int KS, int NJ, bool DH>
+__global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
   using IO = ActIO<HT>;
+  constexpr int HP = sizeof(HT) == 4 ? 2 : 1, WP = sizeof(WT) == 4 ? 2 : 1, CT = KS * 2;
   using IM = CnImage<KS, WP>;
-  constexpr int CT = KS * 2;
   __shared__ __attribute__((aligned(1024))) char sm[2][IM::kBytes];
-  __shared__ int redi[8];
+  __shared__ int redi[4];
   __shared__ double redd[16];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q = lane >> 4, li = lane & 15;
   const unsigned lds0 = ms_lds_addr(&sm[0][0]);
-  const bool stats = a.lse_in == nullptr, grads = a.dh != nullptr;
-  const int nch = a.nch, T = (stats ? nch : 0) + (grads ? nch : 0);
-  const bool resident = nch <= 2;           // both chunks stay: the second run over the classes loads nothing
-  auto chunk_of = [&](int t) { return t >= nch ? t - nch : t; };
-  auto buf_of = [&](int t) { return resident ? chunk_of(t) : (t & 1); };
-  if (T > 0) cn_stage<WP, KS>(a.img, 0, lds0, wave, lane);
+  const bool online = a.lse_in == nullptr;
+  const int nch = (online || DH) ? a.nch : 0;
+  if (nch > 0) cn_stage<WP, KS>(a.img, 0, lds0, wave, lane);
 
-  // ---- this wave's pixels: scaled fp16 planes in the layout of a matrix operand (column = pixel li, 8 channels 32 ks + 8 q + j)
+  // ---- this wave's pixels: scaled fp16 planes in the layout of a matrix operand (column = pixel li, 8 channels 32 ks + 8 q + k)
   ms_h8 x[HP][KS][NJ];
   float fx[NJ];
   int lab[NJ];
-  long pix[NJ];
-  size_t base[NJ];
+  const int pw = (int)blockIdx.x * (4 * NJ * 16) + wave * (NJ * 16) + li;      // (at most 2^30 rows)
+  const int P = (int)a.P;
+  // every load unconditional, at a clamped address, and all of them in flight together (loads behind branches wait for one another: 20 us more at 400k pixels x 64 channels)
+  float v[NJ][KS][8];
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
-    const long p = (long)blockIdx.x * (4 * NJ * 16) + wave * (NJ * 16) + j * 16 + li;
-    pix[j] = p;
-    int y = -1;
-    if (p < a.P) { const int64_t l = a.labels[p]; y = (l >= 0 && l < a.V) ? (int)l : -1; }
-    lab[j] = y;
-    const bool live = p < a.P && (!a.drop || y >= 0);
-    const int n = (int)p / a.HW;                     // (at most 2^30 rows)
-    base[j] = (size_t)n * a.C * a.HW + (size_t)((int)p - n * a.HW);
-    float v[KS][8];
+    const int p = min(pw + j * 16, P - 1), n = p / a.HW;
+    const size_t base = (size_t)n * a.C * a.HW + (size_t)(p - n * a.HW);
+    const int64_t lb = a.labels[p];
+    lab[j] = (lb >= 0 && lb < a.V && pw + j * 16 < P) ? (int)lb : -1;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[j][ks][k] = IO::ld1(a.h, base + (size_t)min(ks * 32 + q * 8 + k, a.C - 1) * a.HW);
+  }
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    const bool live = pw + j * 16 < P && (!a.drop || lab[j] >= 0);
     unsigned am = 0;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const int c = ks * 32 + q * 8 + k;
-        v[ks][k] = (live && c < a.C) ? IO::ld1(a.h, base[j] + (size_t)c * a.HW) : 0.f;
+        if (!live || ks * 32 + q * 8 + k >= a.C) v[j][ks][k] = 0.f;
+        am = max(am, __float_as_uint(v[j][ks][k]) & 0x7FFFFFFFu);
       }
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-      for (int k = 0; k < 8; ++k) am = max(am, __float_as_uint(v[ks][k]) & 0x7FFFFFFFu);
     am = max(am, (unsigned)__shfl_xor((int)am, 16, 64));
     am = max(am, (unsigned)__shfl_xor((int)am, 32, 64));
     const int e = ce_exponent(__uint_as_float(am));
@@ -172,196 +174,134 @@ __global__ __launch_bounds__(256) void cn_pixels_kernel(CnArgs a) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         _Float16 hi, lo;
-        ce_split(v[ks][k] * inv, hi, lo);
+        ce_split(v[j][ks][k] * inv, hi, lo);
         x[0][ks][j][k] = hi;
         if (HP == 2) x[HP - 1][ks][j][k] = lo;
       }
   }
-  const int2 prep = cn_slots(a.slots, a.nslots, redi);
 
-  // one pair of 16-class tiles: z (without the row's scale) of classes t0 + 4 q + r
-  auto logits = [&](const _Float16* wp, int t0, ms_f4 (&s)[2][NJ]) {
+  float m[NJ], l[NJ], zl[NJ];          // in units of log2; m is the same in the four lanes of a pixel, l and zl are each lane's part
+  ms_f4 o[CT][NJ];
+  float scale = 1.f;                   // 2^e of the chunk that o is measured in
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+  for (int j = 0; j < NJ; ++j) {
+    m[j] = -__builtin_inff(); l[j] = 0.f; zl[j] = 0.f;
+    if (!online) m[j] = pw + j * 16 < P ? a.lse_in[pw + j * 16] * kLog2e : 0.f;
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) s[t][j] = ms_f4{0.f, 0.f, 0.f, 0.f};
-      const int r = t0 + t * 16 + li;
+    for (int c = 0; c < CT; ++c) o[c][j] = ms_f4{0.f, 0.f, 0.f, 0.f};
+  }
+  for (int t = 0; t < nch; ++t) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();                   // chunk t has landed for every wave, and nobody reads the buffer that chunk t + 1 goes to
+    if (t + 1 < nch) cn_stage<WP, KS>(a.img, t + 1, lds0 + (unsigned)((t + 1) & 1) * (unsigned)IM::kBytes, wave, lane);
+    const _Float16* wp = (const _Float16*)sm[t & 1];
+    const float* tb = (const float*)(sm[t & 1] + WP * IM::kPlane * 2);
+    const float wl2 = tb[64];
+    if (DH) {
+      const float sc = tb[65];
+      if (sc != scale) {               // (chunks of like weights share a scale)
+        const float f = scale / sc;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const int at = r * (KS * 32) + (((ks * 4 + q) ^ cn_swz<KS>(r)) * 8);
-        const ms_h8 hi = *reinterpret_cast<const ms_h8*>(wp + at);
+        for (int c = 0; c < CT; ++c)
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) s[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, x[0][ks][j], s[t][j], 0, 0, 0);
-        if (HP == 2) {
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) s[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, x[HP - 1][ks][j], s[t][j], 0, 0, 0);
-        }
-        if (WP == 2) {
-          const ms_h8 lo = *reinterpret_cast<const ms_h8*>(wp + IM::kPlane + at);
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) s[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, x[0][ks][j], s[t][j], 0, 0, 0);
-        }
+          for (int j = 0; j < NJ; ++j) o[c][j] *= f;
+        scale = sc;
       }
     }
-  };
-
-  float m[NJ], l[NJ], zl[NJ];          // in units of log2
+    float fs[NJ];
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) { m[j] = -__builtin_inff(); l[j] = 0.f; zl[j] = 0.f; }
-  int t = 0;
-  auto next_chunk = [&]() {            // chunk t is in LDS for every wave; chunk t + 1 starts
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (t + 1 < T && !(resident && t + 1 >= nch)) cn_stage<WP, KS>(a.img, chunk_of(t + 1), lds0 + (unsigned)buf_of(t + 1) * (unsigned)IM::kBytes, wave, lane);
-  };
-  if (stats) {
-    for (; t < nch; ++t) {
-      next_chunk();
-      const _Float16* wp = (const _Float16*)sm[buf_of(t)];
-      const float* tb = (const float*)(sm[buf_of(t)] + WP * IM::kPlane * 2);
+    for (int j = 0; j < NJ; ++j) fs[j] = fx[j] * wl2;
 #pragma unroll 1
-      for (int h2 = 0; h2 < 2; ++h2) {
-        if (t * kCnClasses + h2 * 32 >= a.V) break;
-        ms_f4 s[2][NJ];
-        logits(wp, h2 * 32, s);
-        bool any = false;
+    for (int h2 = 0; h2 < 2; ++h2) {
+      if (t * kCnClasses + h2 * 32 >= a.V) break;
+      // z of two tiles of 16 classes: 4 q + r of each
+      ms_f4 s[2][NJ];
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) any |= (lab[j] >> 5) == t * 2 + h2;
+      for (int tt = 0; tt < 2; ++tt) {
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt) {
-          const float4 f = *reinterpret_cast<const float4*>(tb + h2 * 32 + tt * 16 + q * 4), b = *reinterpret_cast<const float4*>(tb + 64 + h2 * 32 + tt * 16 + q * 4);
-          const float ff[4] = {f.x, f.y, f.z, f.w}, bb[4] = {b.x, b.y, b.z, b.w};
+        for (int j = 0; j < NJ; ++j) s[tt][j] = ms_f4{0.f, 0.f, 0.f, 0.f};
+        const int r = h2 * 32 + tt * 16 + li;
 #pragma unroll
-          for (int j = 0; j < NJ; ++j)
+        for (int ks = 0; ks < KS; ++ks) {
+          const int at = r * (KS * 32) + (((ks * 4 + q) ^ cn_swz<KS>(r)) * 8);
+          const ms_h8 hi = *reinterpret_cast<const ms_h8*>(wp + at);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[tt][j][r] = __builtin_fmaf(s[tt][j][r] * ff[r], fx[j], bb[r]);
+          for (int j = 0; j < NJ; ++j) s[tt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, x[0][ks][j], s[tt][j], 0, 0, 0);
+          if (HP == 2) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) s[tt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, x[HP - 1][ks][j], s[tt][j], 0, 0, 0);
+          }
+          if (WP == 2) {
+            const ms_h8 lo = *reinterpret_cast<const ms_h8*>(wp + IM::kPlane + at);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) s[tt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, x[0][ks][j], s[tt][j], 0, 0, 0);
+          }
         }
-        if (__any(any)) {
+      }
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) {
+      for (int tt = 0; tt < 2; ++tt) {
+        const float4 b = *reinterpret_cast<const float4*>(tb + h2 * 32 + tt * 16 + q * 4);
+        const float bb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[tt][j][r] = __builtin_fmaf(s[tt][j][r], fs[j], bb[r]);
+      }
+      if (online) {
+        bool grow = false;
+        float mx[NJ];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          if (__any((lab[j] >> 5) == t * 2 + h2)) {          // some pixel's label is among these 32 classes
             const int y = lab[j] - (t * kCnClasses + h2 * 32 + q * 4);
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
               for (int r = 0; r < 4; ++r) zl[j] = y == tt * 16 + r ? s[tt][j][r] : zl[j];
           }
+          mx[j] = fmaxf(fmaxf(fmaxf(s[0][j][0], s[0][j][1]), fmaxf(s[0][j][2], s[0][j][3])), fmaxf(fmaxf(s[1][j][0], s[1][j][1]), fmaxf(s[1][j][2], s[1][j][3])));
+          grow |= mx[j] > m[j] + 1.f;
         }
+        if (__any(grow)) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          float mx = fmaxf(fmaxf(fmaxf(s[0][j][0], s[0][j][1]), fmaxf(s[0][j][2], s[0][j][3])), fmaxf(fmaxf(s[1][j][0], s[1][j][1]), fmaxf(s[1][j][2], s[1][j][3])));
-          mx = fmaxf(m[j], mx);
-          const float mm = mx == -__builtin_inff() ? 0.f : mx;
-          float sum = l[j] * __builtin_amdgcn_exp2f(m[j] - mm);
+          for (int j = 0; j < NJ; ++j) {
+            float mn = fmaxf(m[j], mx[j]);
+            mn = fmaxf(mn, __shfl_xor(mn, 16, 64));
+            mn = fmaxf(mn, __shfl_xor(mn, 32, 64));
+            const float f = m[j] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m[j] - mn);
+            m[j] = mn;
+            l[j] *= f;
+            if (DH) {
 #pragma unroll
-          for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(s[tt][j][r] - mm);
-          l[j] = sum; m[j] = mx;
-        }
-      }
-    }
-  }
-  // ---- rows: join the four class quarters, loss, what the class pass needs
-  const float cnt = (float)(a.mean_valid ? max(prep.x, 1) : a.P);
-  float gp[NJ], lse2[NJ];
-  double acc_l = 0.0;
-  int emax = -100000;
-#pragma unroll
-  for (int j = 0; j < NJ; ++j) {
-    const long p = pix[j];
-    if (stats) {
-#pragma unroll
-      for (int off = 16; off <= 32; off <<= 1) {
-        const float mo = __shfl_xor(m[j], off, 64), lo = __shfl_xor(l[j], off, 64), mn = fmaxf(m[j], mo), mm = mn == -__builtin_inff() ? 0.f : mn;
-        l[j] = l[j] * __builtin_amdgcn_exp2f(m[j] - mm) + lo * __builtin_amdgcn_exp2f(mo - mm);
-        m[j] = mn;
-        zl[j] += __shfl_xor(zl[j], off, 64);          // (one lane of the four holds it, the others 0)
-      }
-      const float lg = __builtin_amdgcn_logf(l[j]);   // log2
-      lse2[j] = m[j] + lg;
-      const float ln2 = 0.693147180559945309f, nll = lab[j] >= 0 ? ((m[j] - zl[j]) + lg) * ln2 : 0.f;
-      if (q == 0 && p < a.P) {
-        if (a.nll != nullptr) { a.nll[p] = nll; a.lse_out[p] = lse2[j] * ln2; }
-        acc_l += (double)nll;
-      }
-    } else {
-      lse2[j] = p < a.P ? a.lse_in[p] * kLog2e : 0.f;
-    }
-    gp[j] = 0.f;
-    if (lab[j] >= 0) gp[j] = a.grad != nullptr ? a.grad[p] : a.sign / cnt * (a.scale_dev != nullptr ? *a.scale_dev : 1.f);
-    if (a.fx != nullptr) {
-      const unsigned gb = __float_as_uint(gp[j]) & 0x7FFFFFFFu;
-      if (gb != 0u && gb < 0x7F800000u) emax = max(emax, (int)(gb >> 23) - 126 + (int)(__float_as_uint(fx[j]) >> 23) - 127);
-      if (q == 0) {                                   // (arrays padded to whole workgroups)
-        a.fx[p] = fx[j]; a.gp[p] = gp[j]; a.lab[p] = lab[j];
-        a.lse2[p] = gp[j] == 0.f ? __builtin_inff() : lse2[j];      // a row that takes no part: exp2(z - inf) = 0 whatever z is
-      }
-    }
-  }
-  if (a.lsum != nullptr) {
-    acc_l = block_sum_d(acc_l, redd);
-    if (threadIdx.x == 0) a.lsum[blockIdx.x] = acc_l;
-  }
-  if (a.fx != nullptr) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) emax = max(emax, __shfl_xor(emax, off, 64));
-    if (lane == 0 && emax > -100000) atomicMax(&a.scal[1], emax);
-  }
-  if (!grads) return;
-
-  // ---- dh = w^T G.  G is scaled by 2^(ew - max ew + 13) class by class: the power of two rides on the exponent's argument.
-  ms_f4 o[CT][NJ];
-#pragma unroll
-  for (int c = 0; c < CT; ++c)
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) o[c][j] = ms_f4{0.f, 0.f, 0.f, 0.f};
-  const float top = (float)(kCeTopExp - prep.y);
-  constexpr bool kG2 = HP == 2;          // planes of G (and of w, below): two for an fp32 dh
-#pragma unroll 1
-  for (; t < T; ++t) {
-    next_chunk();
-    const int ch = chunk_of(t);
-    const _Float16* wp = (const _Float16*)sm[buf_of(t)];
-    const float* tb = (const float*)(sm[buf_of(t)] + WP * IM::kPlane * 2);
-#pragma unroll 1
-    for (int h2 = 0; h2 < 2; ++h2) {
-      if (ch * kCnClasses + h2 * 32 >= a.V) break;
-      ms_f4 s[2][NJ];
-      logits(wp, h2 * 32, s);
-      ms_h8 gh[NJ], gl[NJ];
-      bool any = false;
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) any |= (lab[j] >> 5) == ch * 2 + h2;
-      any = __any(any);
-#pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
-        const float4 f = *reinterpret_cast<const float4*>(tb + h2 * 32 + tt * 16 + q * 4), b = *reinterpret_cast<const float4*>(tb + 64 + h2 * 32 + tt * 16 + q * 4),
-                     ew = *reinterpret_cast<const float4*>(tb + 128 + h2 * 32 + tt * 16 + q * 4);
-        const float ff[4] = {f.x, f.y, f.z, f.w}, bb[4] = {b.x, b.y, b.z, b.w}, ee[4] = {ew.x + top, ew.y + top, ew.z + top, ew.w + top};
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          float g[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) g[r] = __builtin_amdgcn_exp2f((__builtin_fmaf(s[tt][j][r] * ff[r], fx[j], bb[r]) - lse2[j]) + ee[r]);
-          if (any) {
-            const int y = lab[j] - (ch * kCnClasses + h2 * 32 + tt * 16 + q * 4);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) g[r] -= y == r ? __builtin_amdgcn_exp2f(ee[r]) : 0.f;
+              for (int c = 0; c < CT; ++c) o[c][j] *= f;
+            }
           }
+        }
+      }
+      ms_h8 gh[NJ], gl[NJ];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const float mm = (m[j] == -__builtin_inff() ? 0.f : m[j]) - 14.f;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            _Float16 hi, lo;
-            ce_split(g[r], hi, lo);
-            gh[j][tt * 4 + r] = hi; gl[j][tt * 4 + r] = lo;
+            const float e = __builtin_amdgcn_exp2f(s[tt][j][r] - mm);
+            l[j] += e;
+            if (DH) {
+              _Float16 hi, lo;
+              ce_split(e, hi, lo);
+              gh[j][tt * 4 + r] = hi; gl[j][tt * 4 + r] = lo;
+            }
           }
-        }
       }
+      if (DH) {
+        // Two planes of e also for a bf16 dh: o / l - w[label] nearly cancels where the network is sure, and has to be right to more than e's 11 bits there.
 #pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        const ms_h8 wh = cn_tr2<KS>(wp, h2 * 32, h2 * 32 + 16, c * 16, lane);
+        for (int c = 0; c < CT; ++c) {
+          const ms_h8 wh = cn_tr2<KS>(wp, h2 * 32, h2 * 32 + 16, c * 16, lane);
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) o[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh, gh[j], o[c][j], 0, 0, 0);
-        if (kG2) {
+          for (int j = 0; j < NJ; ++j) o[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh, gh[j], o[c][j], 0, 0, 0);
 #pragma unroll
           for (int j = 0; j < NJ; ++j) o[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh, gl[j], o[c][j], 0, 0, 0);
           if (WP == 2) {
@@ -373,18 +313,66 @@ __global__ __launch_bounds__(256) void cn_pixels_kernel(CnArgs a) {
       }
     }
   }
-  const float back = ce_pow2(prep.y - kCeTopExp);
+  // ---- rows: loss, what the class pass needs, dh
+  const float cnt = (float)(a.mean_valid ? max(cn_count(a.slots, a.nslots, redi), 1) : P);
+  double acc_l = 0.0;
+  int emax = -100000;
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
-    if (pix[j] >= a.P) continue;
-    const float f = gp[j] * back;
-#pragma unroll
-    for (int c = 0; c < CT; ++c)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int cc = c * 16 + q * 4 + r;
-        if (cc < a.C) IO::st1(a.dh, base[j] + (size_t)cc * a.HW, gp[j] == 0.f ? 0.f : o[c][j][r] * f);
+    const int p = pw + j * 16;
+    float lse2 = m[j], fac = 1.f / 16384.f;
+    if (online) {
+      l[j] += __shfl_xor(l[j], 16, 64);
+      l[j] += __shfl_xor(l[j], 32, 64);
+      zl[j] += __shfl_xor(zl[j], 16, 64);             // (one lane of the four holds it, the others 0)
+      zl[j] += __shfl_xor(zl[j], 32, 64);
+      fac = 1.f / l[j];
+      const float lg = __builtin_amdgcn_logf(l[j]) - 14.f;      // log2
+      lse2 = m[j] + lg;
+      const float ln2 = 0.693147180559945309f, nll = lab[j] >= 0 ? ((m[j] - zl[j]) + lg) * ln2 : 0.f;
+      if (q == 0 && p < P) {
+        if (a.nll != nullptr) { a.nll[p] = nll; a.lse_out[p] = lse2 * ln2; }
+        acc_l += (double)nll;
       }
+    }
+    float gp = 0.f;
+    if (lab[j] >= 0) gp = a.grad != nullptr ? a.grad[p] : a.sign / cnt * (a.scale_dev != nullptr ? *a.scale_dev : 1.f);
+    if (a.fx != nullptr) {
+      const unsigned gb = __float_as_uint(gp) & 0x7FFFFFFFu;
+      if (gb != 0u && gb < 0x7F800000u) emax = max(emax, (int)(gb >> 23) - 126 + (int)(__float_as_uint(fx[j]) >> 23) - 127);
+      if (q == 0) {                                   // (arrays padded to whole workgroups)
+        a.fx[p] = fx[j]; a.gp[p] = gp; a.lab[p] = lab[j];
+        a.lse2[p] = gp == 0.f ? __builtin_inff() : lse2;        // a row that takes no part: exp2(z - inf) = 0 whatever z is
+      }
+    }
+    if (DH) {
+      const int pc = min(p, P - 1), n = pc / a.HW;
+      const size_t base = (size_t)n * a.C * a.HW + (size_t)(pc - n * a.HW), wrow = (size_t)max(lab[j], 0) * a.C;
+      const float f = scale * fac;
+      float wl[CT][4];
+#pragma unroll
+      for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) wl[c][r] = ActIO<WT>::ld1(a.w, wrow + min(c * 16 + q * 4 + r, a.C - 1));
+#pragma unroll
+      for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int cc = c * 16 + q * 4 + r;
+          const float d = gp == 0.f ? 0.f : gp * (o[c][j][r] * f - wl[c][r]);
+          if (cc < a.C && p < P) IO::st1(a.dh, base + (size_t)cc * a.HW, d);
+        }
+    }
+  }
+  if (a.lsum != nullptr) {
+    acc_l = block_sum_d(acc_l, redd);
+    if (threadIdx.x == 0) a.lsum[blockIdx.x] = acc_l;
+  }
+  if (a.fx != nullptr) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) emax = max(emax, __shfl_xor(emax, off, 64));
+    // (looked at first: the atomics of 16384 waves on one word took 180 us)
+    if (lane == 0 && emax > __hip_atomic_load(&a.scal[1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(&a.scal[1], emax);
   }
 }
 
@@ -396,9 +384,10 @@ struct CnwArgs {
 };
 
 // Pixel tile in LDS: [plane][channel][TP pixels], 16-byte chunk j of row c at j ^ (c & 7).
-template <typename HT, int HP, int WP, int KS, int NJ, int TP, bool VEC>
-__global__ __launch_bounds__(256) void cn_classes_kernel(CnwArgs a) {
+template <typename HT, typename WT, int KS, int NJ, int TP, bool VEC>
+__global__ __launch_bounds__(256, 2) void cn_classes_kernel(CnwArgs a) {
   using IO = ActIO<HT>;
+  constexpr int HP = sizeof(HT) == 4 ? 2 : 1, WP = sizeof(WT) == 4 ? 2 : 1;
   using IM = CnImage<KS, WP>;
   constexpr int CT = KS * 2, kC = KS * 32, kTasks = kC * (TP / 8) / 256;
   __shared__ __attribute__((aligned(1024))) _Float16 xs[HP * kC * TP];
@@ -414,14 +403,15 @@ __global__ __launch_bounds__(256) void cn_classes_kernel(CnwArgs a) {
 
   // this wave's classes
   ms_h8 w[WP][KS][NJ];
-  float fw[NJ], bw[NJ], db[NJ];
+  float bw[NJ], db[NJ];
+  const float wl2 = busy ? ((const float*)(a.img + (size_t)(v0 >> 6) * IM::kBytes + WP * IM::kPlane * 2))[64] : 0.f;      // (the classes of a wave lie in one chunk)
   ms_f4 o[CT][NJ];
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
     const int v = min(v0 + j * 16 + li, ((a.V + 63) & ~63) - 1), r = v & 63;      // (a class behind the last chunk repeats its last row and is not stored)
     const char* im = a.img + (size_t)(v >> 6) * IM::kBytes;
     const float* tb = (const float*)(im + WP * IM::kPlane * 2);
-    fw[j] = tb[r]; bw[j] = tb[64 + r]; db[j] = 0.f;
+    bw[j] = tb[r]; db[j] = 0.f;
 #pragma unroll
     for (int pl = 0; pl < WP; ++pl)
 #pragma unroll
@@ -523,19 +513,25 @@ __global__ __launch_bounds__(256) void cn_classes_kernel(CnwArgs a) {
           const float4 f = *reinterpret_cast<const float4*>(&rows[0][pr]), ls = *reinterpret_cast<const float4*>(&rows[1][pr]), rr = *reinterpret_cast<const float4*>(&rows[2][pr]),
                        gg = *reinterpret_cast<const float4*>(&rows[3][pr]);
           const int4 yy = *reinterpret_cast<const int4*>(&labs[pr]);
-          const float ff[4] = {f.x, f.y, f.z, f.w}, l4[4] = {ls.x, ls.y, ls.z, ls.w}, r4[4] = {rr.x, rr.y, rr.z, rr.w}, g4[4] = {gg.x, gg.y, gg.z, gg.w};
-          const int y4[4] = {yy.x, yy.y, yy.z, yy.w};
+          const float ff[4] = {f.x * wl2, f.y * wl2, f.z * wl2, f.w * wl2}, l4[4] = {ls.x, ls.y, ls.z, ls.w}, r4[4] = {rr.x, rr.y, rr.z, rr.w}, g4[4] = {gg.x, gg.y, gg.z, gg.w};
+          const int y4[4] = {yy.x - v0 - li, yy.y - v0 - li, yy.z - v0 - li, yy.w - v0 - li};
 #pragma unroll
-          for (int j = 0; j < NJ; ++j)
+          for (int j = 0; j < NJ; ++j) {
+            float e[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][j][r], ff[r], bw[j]) - l4[r]);
+            if (__any(y4[0] == j * 16 || y4[1] == j * 16 || y4[2] == j * 16 || y4[3] == j * 16)) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r) e[r] -= y4[r] == j * 16 ? 1.f : 0.f;
+            }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][j][r] * ff[r], fw[j], bw[j]) - l4[r]);
-              e -= y4[r] == v0 + j * 16 + li ? 1.f : 0.f;
-              db[j] = __builtin_fmaf(e, g4[r], db[j]);
+              db[j] = __builtin_fmaf(e[r], g4[r], db[j]);
               _Float16 x, y;
-              ce_split(e * r4[r], x, y);
+              ce_split(e[r] * r4[r], x, y);
               gh[j][tt * 4 + r] = x; gl[j][tt * 4 + r] = y;
             }
+          }
         }
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
@@ -580,17 +576,17 @@ __global__ __launch_bounds__(256) void cn_classes_kernel(CnwArgs a) {
 // dw, db: sums of the splits in a fixed order; the loss (last workgroup).  A workgroup sums 64 elements, 16 threads each.
 template <typename WT>
 __global__ __launch_bounds__(1024) void cn_join_kernel(const float* __restrict__ dwp, const float* __restrict__ dbp, size_t dw_split, int db_split, int splits, void* __restrict__ dw,
-                                                       float* __restrict__ db, int V, int C, int kC, int dw_blocks, const double* __restrict__ lsum, int nl, const int2* __restrict__ slots,
+                                                       float* __restrict__ db, int V, int C, int kC, int dw_blocks, const double* __restrict__ lsum, int nl, const int* __restrict__ slots,
                                                        int nslots, float sign, int mean_valid, long P, float* __restrict__ loss) {
   __shared__ double redd[16];
-  __shared__ int redi[32];
+  __shared__ int redi[16];
   __shared__ float part[16][64];
   if (blockIdx.x == gridDim.x - 1 && loss != nullptr) {
-    const int2 s = cn_slots(slots, nslots, redi);
+    const int s = mean_valid ? cn_count(slots, nslots, redi) : 0;
     double a = 0.0;
     for (int i = threadIdx.x; i < nl; i += 1024) a += lsum[i];
     a = block_sum_d(a, redd);
-    if (threadIdx.x == 0) loss[0] = (float)((double)sign * a / (double)(mean_valid ? max(s.x, 1) : P));
+    if (threadIdx.x == 0) loss[0] = (float)((double)sign * a / (double)(mean_valid ? max(s, 1) : P));
     return;
   }
   const bool isw = blockIdx.x < (unsigned)dw_blocks;
@@ -629,7 +625,7 @@ static CnPlan cn_plan(int N, int C, int V, int HW, int types, bool grad) {
   if (k.nj == 4 && k.P < 256L * 256) k.nj = 2;
   k.wgs = (k.P + k.nj * 64 - 1) / (k.nj * 64);
   k.Pp = (k.P + 255) / 256 * 256;
-  k.nslots = (int)std::min<long>(kCnPrep, std::max<long>(cdiv(k.Vp, 4), std::min<long>(k.P / 1024 + 1, kCnPrep)));
+  k.nslots = (int)std::min<long>(kCnPrep, k.P / 1024 + 1);
   k.njw = k.KS <= 2 && V > 32 ? 4 : 2;
   k.units = cdiv(V, 16 * k.njw);
   k.tp = k.KS <= 2 ? 128 : 64;
@@ -641,7 +637,7 @@ static CnPlan cn_plan(int N, int C, int V, int HW, int types, bool grad) {
   size_t o = 0;
   auto take = [&](size_t n) { const size_t at = o; o += (n + 255) & ~(size_t)255; return at; };
   k.o_img = take((size_t)k.nch * ((size_t)((types & 2) ? 1 : 2) * 64 * k.KS * 64 + 1024));
-  k.o_slots = take(kCnPrep * 8); k.o_scal = take(64); k.o_lsum = take((size_t)k.wgs * 8);
+  k.o_slots = take(kCnPrep * 4); k.o_scal = take(64); k.o_lsum = take((size_t)k.wgs * 8);
   if (grad) {
     k.o_fx = take(k.Pp * 4); k.o_lse = take(k.Pp * 4); k.o_gp = take(k.Pp * 4); k.o_lab = take(k.Pp * 4);
     k.o_dw = take((size_t)k.splits * k.wpx * k.Vp * k.KS * 32 * 4);
@@ -660,27 +656,28 @@ size_t ce_narrow_ws_bytes(int N, int C, int V, int HW, int types, bool grad) { r
 
 template <typename HT, typename WT, int KS>
 static int cn_run(const CeArgs& a, const CnPlan& k) {
-  constexpr int HP = sizeof(HT) == 4 ? 2 : 1, WP = sizeof(WT) == 4 ? 2 : 1;
+  constexpr int WP = sizeof(WT) == 4 ? 2 : 1;
   const bool need_dw = a.dw != nullptr || a.db != nullptr, need_grad = need_dw || a.dh != nullptr;
   char* ws = (char*)a.ws;
   hipStream_t st = a.st;
-  int2* slots = (int2*)(ws + k.o_slots);
+  int* slots = (int*)(ws + k.o_slots);
   int* scal = (int*)(ws + k.o_scal);
-  MS_LAUNCH((cn_prep_kernel<WT, WP, KS>), dim3(k.nslots), dim3(256), 0, st, a.w, a.b, a.labels, k.P, a.mean_valid, ws + k.o_img, slots, scal, a.V, k.Vp, a.C);
+  MS_LAUNCH((cn_prep_kernel<WT, WP, KS>), dim3(std::max(k.nch, a.mean_valid ? k.nslots : 1)), dim3(256), 0, st, a.w, a.b, a.labels, k.P, a.mean_valid, ws + k.o_img, slots, k.nslots, scal, a.V,
+            k.nch, a.C);
   if (int e = check_launch("class_ce_prep")) return e;
   CnArgs p{};
-  p.h = a.h; p.labels = a.labels; p.img = ws + k.o_img; p.slots = slots; p.nslots = k.nslots; p.scal = scal;
+  p.h = a.h; p.w = a.w; p.labels = a.labels; p.img = ws + k.o_img; p.slots = slots; p.nslots = k.nslots; p.scal = scal;
   p.nll = a.nll; p.lse_out = a.lse; p.lse_in = a.lse_in; p.grad = a.grad; p.scale_dev = a.scale_dev; p.sign = a.sign; p.mean_valid = a.mean_valid; p.drop = need_grad ? 1 : 0;
   p.dh = a.dh; p.lsum = a.loss != nullptr ? (double*)(ws + k.o_lsum) : nullptr;
   if (need_dw) { p.fx = (float*)(ws + k.o_fx); p.lse2 = (float*)(ws + k.o_lse); p.gp = (float*)(ws + k.o_gp); p.lab = (int*)(ws + k.o_lab); }
   p.P = k.P; p.C = a.C; p.HW = a.HW; p.V = a.V; p.nch = k.nch;
   const dim3 grid((unsigned)k.wgs), block(256);
   if constexpr (KS <= 2) {
-    if (k.nj == 4) MS_LAUNCH((cn_pixels_kernel<HT, HP, WP, KS, 4>), grid, block, 0, st, p);
-    else MS_LAUNCH((cn_pixels_kernel<HT, HP, WP, KS, 2>), grid, block, 0, st, p);
-  } else {
-    MS_LAUNCH((cn_pixels_kernel<HT, HP, WP, KS, 2>), grid, block, 0, st, p);
+    if (k.nj == 4 && a.dh != nullptr) MS_LAUNCH((cn_pixels_kernel<HT, WT, KS, 4, true>), grid, block, 0, st, p);
+    else if (k.nj == 4) MS_LAUNCH((cn_pixels_kernel<HT, WT, KS, 4, false>), grid, block, 0, st, p);
   }
+  if (k.nj == 2 && a.dh != nullptr) MS_LAUNCH((cn_pixels_kernel<HT, WT, KS, 2, true>), grid, block, 0, st, p);
+  else if (k.nj == 2) MS_LAUNCH((cn_pixels_kernel<HT, WT, KS, 2, false>), grid, block, 0, st, p);
   if (int e = check_launch("class_ce_pixels")) return e;
   if (need_dw) {
     CnwArgs c{};
@@ -692,15 +689,15 @@ static int cn_run(const CeArgs& a, const CnPlan& k) {
     constexpr int TP = KS <= 2 ? 128 : 64;
     if constexpr (KS <= 2) {
       if (k.njw == 4) {
-        if (vec) MS_LAUNCH((cn_classes_kernel<HT, HP, WP, KS, 4, TP, true>), gw, block, 0, st, c);
-        else MS_LAUNCH((cn_classes_kernel<HT, HP, WP, KS, 4, TP, false>), gw, block, 0, st, c);
+        if (vec) MS_LAUNCH((cn_classes_kernel<HT, WT, KS, 4, TP, true>), gw, block, 0, st, c);
+        else MS_LAUNCH((cn_classes_kernel<HT, WT, KS, 4, TP, false>), gw, block, 0, st, c);
       } else {
-        if (vec) MS_LAUNCH((cn_classes_kernel<HT, HP, WP, KS, 2, TP, true>), gw, block, 0, st, c);
-        else MS_LAUNCH((cn_classes_kernel<HT, HP, WP, KS, 2, TP, false>), gw, block, 0, st, c);
+        if (vec) MS_LAUNCH((cn_classes_kernel<HT, WT, KS, 2, TP, true>), gw, block, 0, st, c);
+        else MS_LAUNCH((cn_classes_kernel<HT, WT, KS, 2, TP, false>), gw, block, 0, st, c);
       }
     } else {
-      if (vec) MS_LAUNCH((cn_classes_kernel<HT, HP, WP, KS, 2, TP, true>), gw, block, 0, st, c);
-      else MS_LAUNCH((cn_classes_kernel<HT, HP, WP, KS, 2, TP, false>), gw, block, 0, st, c);
+      if (vec) MS_LAUNCH((cn_classes_kernel<HT, WT, KS, 2, TP, true>), gw, block, 0, st, c);
+      else MS_LAUNCH((cn_classes_kernel<HT, WT, KS, 2, TP, false>), gw, block, 0, st, c);
     }
     if (int e = check_launch("class_ce_classes")) return e;
   }
