@@ -17,7 +17,10 @@
 namespace ms {
 
 constexpr int kCnClasses = 64;        // classes of one image chunk
-constexpr int kCnPrep = 256;          // most workgroups of the prep pass
+constexpr int kCnPrep = 256;          // most workgroups that count
+// 16-column groups a wave keeps.  Pixels: 2 - 4 halve the LDS reads a product, but leave two waves a SIMD for 3 to 4 (400k pixels x 64 channels, 151 classes: 144 -> 113 us).
+// Classes: 4 where the registers hold them and there are that many (one pixel tile then serves 256 classes: 1M pixels x 64, 256 classes: 301 -> 227 us), else 2.
+constexpr int kCnNJ = 2;
 
 // 16-byte chunk j of row r of a tile of KS * 32 columns lies at chunk j ^ cn_swz(r): both the row reads and the transposing reads below are then free of bank conflicts
 template <int KS> __device__ __forceinline__ int cn_swz(int r) { return KS == 1 ? (r >> 1) & 3 : (KS == 3 ? (r >> 2) & 3 : r & 7); }
@@ -38,16 +41,15 @@ __device__ __forceinline__ ms_h8 cn_tr2(const _Float16* tile, int k0, int k1, in
   return u.h;
 }
 
-// One workgroup a chunk of classes (the first nch), and all of them count: slots[block] = rows that take part.  scal[1] is made ready for the pixel pass.
+// One workgroup a chunk of classes (the first nch), and all of them count: slots[block] = rows that take part.
 // One scale for 64 classes: a weight is held to 2^-22, or 2^-39 of the chunk's largest - an absolute error that no logit notices.
 template <typename WT, int WP, int KS>
 __global__ __launch_bounds__(256) void cn_prep_kernel(const void* __restrict__ w, const float* __restrict__ b, const int64_t* __restrict__ labels, long P, int count,
-                                                      char* __restrict__ img, int* __restrict__ slots, int nslots, int* __restrict__ scal, int V, int nch, int C) {
+                                                      char* __restrict__ img, int* __restrict__ slots, int nslots, int V, int nch, int C) {
   using IO = ActIO<WT>;
   using IM = CnImage<KS, WP>;
   __shared__ int red[4];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  if (blockIdx.x == 0 && threadIdx.x == 0) scal[1] = -100000;
   if ((int)blockIdx.x < nch) {
     const int v0 = blockIdx.x * 64;
     constexpr int kPer = 64 * KS * 32 / 256;
@@ -111,15 +113,17 @@ __device__ __forceinline__ void cn_stage(const char* img, int chunk, unsigned ld
 }
 
 struct CnArgs {
-  const void *h, *w; const int64_t* labels; const char* img; const int* slots; int nslots; int* scal;
+  const void *h, *w; const int64_t* labels; const char* img; const int* slots; int nslots;
   float *nll, *lse_out; const float *lse_in, *grad, *scale_dev; float sign; int mean_valid, drop;
   void* dh; double* lsum;
   float *fx, *lse2, *gp; int* lab;          // what the class pass needs of every row (NULL: it does not run)
-  long P; int C, HW, V, nch;
+  long P; int C, HW, V, nch, w_vec;
 };
 
-// The running maximum m is moved only when a logit exceeds it by more than 1 (in log2), for a whole wave at once: e = 2^(14 + z - m) then stays below 2^15 in fp16, and
-// most classes after the first cost no rescaling.  With the log-sum given (lse_in) m is that, and never moves.
+// The running maximum m is moved only when a logit exceeds it by more than kCnSlack (in log2), for a whole wave at once: e = 2^(kCnTop + z - m) then stays below 2^15 in
+// fp16 (and is held to 2^-34 of e at m: the lowest step of its low plane), and classes after the first few cost no rescaling - with a slack of 1 some pixel of 64 still
+// had it done for most of 256 classes.  With the log-sum given (lse_in) m is that, and never moves.
+constexpr float kCnSlack = 6.f, kCnTop = 9.f;
 template <typename HT, typename WT, int KS, int NJ, bool DH>
 __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
   using IO = ActIO<HT>;
@@ -248,19 +252,24 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
           for (int r = 0; r < 4; ++r) s[tt][j][r] = __builtin_fmaf(s[tt][j][r], fs[j], bb[r]);
       }
       if (online) {
-        bool grow = false;
+        bool grow = false, here = false;
         float mx[NJ];
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          if (__any((lab[j] >> 5) == t * 2 + h2)) {          // some pixel's label is among these 32 classes
+        for (int j = 0; j < NJ; ++j) here |= (lab[j] >> 5) == t * 2 + h2;
+        if (__any(here)) {             // some pixel's label is among these 32 classes (seldom so in a label map)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) {
             const int y = lab[j] - (t * kCnClasses + h2 * 32 + q * 4);
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
               for (int r = 0; r < 4; ++r) zl[j] = y == tt * 16 + r ? s[tt][j][r] : zl[j];
           }
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
           mx[j] = fmaxf(fmaxf(fmaxf(s[0][j][0], s[0][j][1]), fmaxf(s[0][j][2], s[0][j][3])), fmaxf(fmaxf(s[1][j][0], s[1][j][1]), fmaxf(s[1][j][2], s[1][j][3])));
-          grow |= mx[j] > m[j] + 1.f;
+          grow |= mx[j] > m[j] + kCnSlack;
         }
         if (__any(grow)) {
 #pragma unroll
@@ -281,19 +290,15 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
       ms_h8 gh[NJ], gl[NJ];
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        const float mm = (m[j] == -__builtin_inff() ? 0.f : m[j]) - 14.f;
+        const float mm = (m[j] == -__builtin_inff() ? 0.f : m[j]) - kCnTop;
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float e = __builtin_amdgcn_exp2f(s[tt][j][r] - mm);
-            l[j] += e;
-            if (DH) {
-              _Float16 hi, lo;
-              ce_split(e, hi, lo);
-              gh[j][tt * 4 + r] = hi; gl[j][tt * 4 + r] = lo;
-            }
+            s[tt][j][r] = __builtin_amdgcn_exp2f(s[tt][j][r] - mm);
+            l[j] += s[tt][j][r];
           }
+        if (DH) ce_split8(s[0][j], s[1][j], gh[j], gl[j]);
       }
       if (DH) {
         // Two planes of e also for a bf16 dh: o / l - w[label] nearly cancels where the network is sure, and has to be right to more than e's 11 bits there.
@@ -304,7 +309,7 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
           for (int j = 0; j < NJ; ++j) o[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh, gh[j], o[c][j], 0, 0, 0);
 #pragma unroll
           for (int j = 0; j < NJ; ++j) o[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh, gl[j], o[c][j], 0, 0, 0);
-          if (WP == 2) {
+          if (WP == 2 && HP == 2) {         // (a bf16 dh is the gradient of w held to 11 bits)
             const ms_h8 wl = cn_tr2<KS>(wp + IM::kPlane, h2 * 32, h2 * 32 + 16, c * 16, lane);
 #pragma unroll
             for (int j = 0; j < NJ; ++j) o[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wl, gh[j], o[c][j], 0, 0, 0);
@@ -316,18 +321,17 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
   // ---- rows: loss, what the class pass needs, dh
   const float cnt = (float)(a.mean_valid ? max(cn_count(a.slots, a.nslots, redi), 1) : P);
   double acc_l = 0.0;
-  int emax = -100000;
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
     const int p = pw + j * 16;
-    float lse2 = m[j], fac = 1.f / 16384.f;
+    float lse2 = m[j], fac = 1.f / 512.f;
     if (online) {
       l[j] += __shfl_xor(l[j], 16, 64);
       l[j] += __shfl_xor(l[j], 32, 64);
       zl[j] += __shfl_xor(zl[j], 16, 64);             // (one lane of the four holds it, the others 0)
       zl[j] += __shfl_xor(zl[j], 32, 64);
       fac = 1.f / l[j];
-      const float lg = __builtin_amdgcn_logf(l[j]) - 14.f;      // log2
+      const float lg = __builtin_amdgcn_logf(l[j]) - kCnTop;      // log2
       lse2 = m[j] + lg;
       const float ln2 = 0.693147180559945309f, nll = lab[j] >= 0 ? ((m[j] - zl[j]) + lg) * ln2 : 0.f;
       if (q == 0 && p < P) {
@@ -338,8 +342,6 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
     float gp = 0.f;
     if (lab[j] >= 0) gp = a.grad != nullptr ? a.grad[p] : a.sign / cnt * (a.scale_dev != nullptr ? *a.scale_dev : 1.f);
     if (a.fx != nullptr) {
-      const unsigned gb = __float_as_uint(gp) & 0x7FFFFFFFu;
-      if (gb != 0u && gb < 0x7F800000u) emax = max(emax, (int)(gb >> 23) - 126 + (int)(__float_as_uint(fx[j]) >> 23) - 127);
       if (q == 0) {                                   // (arrays padded to whole workgroups)
         a.fx[p] = fx[j]; a.gp[p] = gp; a.lab[p] = lab[j];
         a.lse2[p] = gp == 0.f ? __builtin_inff() : lse2;        // a row that takes no part: exp2(z - inf) = 0 whatever z is
@@ -349,11 +351,28 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
       const int pc = min(p, P - 1), n = pc / a.HW;
       const size_t base = (size_t)n * a.C * a.HW + (size_t)(pc - n * a.HW), wrow = (size_t)max(lab[j], 0) * a.C;
       const float f = scale * fac;
-      float wl[CT][4];
+      float wl[CT][4];                    // the label's weights, rounded as the products' were (16 bytes a lane: 4-byte loads from 64 rows at once cost 100 us a million pixels)
+      if (a.w_vec) {
 #pragma unroll
-      for (int c = 0; c < CT; ++c)
+        for (int c = 0; c < CT; ++c) {
+          const float4 t = ActIO<WT>::ld4(a.w, wrow + min(c * 16 + q * 4, a.C - 4));
+          wl[c][0] = t.x; wl[c][1] = t.y; wl[c][2] = t.z; wl[c][3] = t.w;
+        }
+      } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) wl[c][r] = ActIO<WT>::ld1(a.w, wrow + min(c * 16 + q * 4 + r, a.C - 1));
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) wl[c][r] = ActIO<WT>::ld1(a.w, wrow + min(c * 16 + q * 4 + r, a.C - 1));
+      }
+      if (HP == 1 && WP == 2) {
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const unsigned u = __float_as_uint(wl[c][r]);
+            wl[c][r] = __uint_as_float((u + 0xFFFu + ((u >> 13) & 1u)) & ~0x1FFFu);
+          }
+      }
 #pragma unroll
       for (int c = 0; c < CT; ++c)
 #pragma unroll
@@ -368,17 +387,11 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
     acc_l = block_sum_d(acc_l, redd);
     if (threadIdx.x == 0) a.lsum[blockIdx.x] = acc_l;
   }
-  if (a.fx != nullptr) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) emax = max(emax, __shfl_xor(emax, off, 64));
-    // (looked at first: the atomics of 16384 waves on one word took 180 us)
-    if (lane == 0 && emax > __hip_atomic_load(&a.scal[1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(&a.scal[1], emax);
-  }
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------ dw, db
 struct CnwArgs {
-  const void* h; const char* img; const float *fx, *lse2, *gp; const int* lab; const int* scal;
+  const void* h; const char* img; const float *fx, *lse2, *gp; const int* lab;
   float *dwp, *dbp; size_t dw_split; int db_split;
   long P; int C, HW, V, units, wpx, splits, tiles;
 };
@@ -391,16 +404,13 @@ __global__ __launch_bounds__(256, 2) void cn_classes_kernel(CnwArgs a) {
   using IM = CnImage<KS, WP>;
   constexpr int CT = KS * 2, kC = KS * 32, kTasks = kC * (TP / 8) / 256;
   __shared__ __attribute__((aligned(1024))) _Float16 xs[HP * kC * TP];
-  __shared__ __attribute__((aligned(16))) float rows[4][TP];       // 2^ex, lse, g_p 2^ex 2^k, g_p
+  __shared__ __attribute__((aligned(16))) float rows[4][TP];       // 2^ex, lse, g_p 2^ex, g_p
   __shared__ __attribute__((aligned(16))) int labs[TP];
+  __shared__ int tmax[2];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q = lane >> 4, li = lane & 15;
   const int wv = 4 / a.wpx, unit = blockIdx.y * wv + wave % wv, wp_ = wave / wv;
   const bool busy = unit < a.units;
   const int v0 = unit * (NJ * 16);
-  const int ge = a.scal[1];
-  const int gexp = ge < -50000 ? 0 : min(max(kCeTopExp - ge, -120), 120);
-  const float gn = ce_pow2(gexp);
-
   // this wave's classes
   ms_h8 w[WP][KS][NJ];
   float bw[NJ], db[NJ];
@@ -420,6 +430,11 @@ __global__ __launch_bounds__(256, 2) void cn_classes_kernel(CnwArgs a) {
     for (int c = 0; c < CT; ++c) o[c][j] = ms_f4{0.f, 0.f, 0.f, 0.f};
   }
   const int t0 = (int)((long)a.tiles * blockIdx.x / a.splits), t1 = (int)((long)a.tiles * (blockIdx.x + 1) / a.splits);
+
+  // G 2^ex is scaled so that the largest |g_p| 2^ex met so far lies below 2^kCeTopExp: the partial sums are moved along when a tile brings a larger one.
+  int kmax = -100000;
+  float gn = 0.f;
+  if (threadIdx.x < 2) tmax[threadIdx.x] = -100000;
 
   float pre[kTasks][8];
   float prow[3];
@@ -454,8 +469,13 @@ __global__ __launch_bounds__(256, 2) void cn_classes_kernel(CnwArgs a) {
   for (int t = t0; t < t1; ++t) {
     __syncthreads();                           // nobody reads the tile before this one
     if (threadIdx.x < TP) {
-      rows[0][threadIdx.x] = prow[0]; rows[1][threadIdx.x] = prow[1]; rows[2][threadIdx.x] = prow[2] * prow[0] * gn; rows[3][threadIdx.x] = prow[2];
+      rows[0][threadIdx.x] = prow[0]; rows[1][threadIdx.x] = prow[1]; rows[2][threadIdx.x] = prow[2] * prow[0]; rows[3][threadIdx.x] = prow[2];
       labs[threadIdx.x] = plab;
+      const unsigned gb = __float_as_uint(prow[2]) & 0x7FFFFFFFu;
+      int e = (gb != 0u && gb < 0x7F800000u) ? (int)(gb >> 23) - 126 + (int)(__float_as_uint(prow[0]) >> 23) - 127 : -100000;
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) e = max(e, __shfl_xor(e, off, 64));
+      if (lane == 0) atomicMax(&tmax[t & 1], e);
     }
     __syncthreads();
 #pragma unroll
@@ -476,7 +496,18 @@ __global__ __launch_bounds__(256, 2) void cn_classes_kernel(CnwArgs a) {
       if (HP == 2) *reinterpret_cast<ms_h8*>(xs + kC * TP + at) = lo;
     }
     if (t + 1 < t1) load(t + 1);
+    const int tm = tmax[t & 1];
     __syncthreads();
+    if (threadIdx.x == 0) tmax[t & 1] = -100000;          // (next used by tile t + 2)
+    if (tm > kmax) {
+      const float f = kmax < -50000 ? 0.f : ce_pow2(kmax - tm);
+      kmax = tm;
+      gn = ce_pow2(min(max(kCeTopExp - kmax, -120), 120));
+#pragma unroll
+      for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) o[c][j] *= f;
+    }
     if (busy) {
 #pragma unroll 1
       for (int sub = wp_; sub < TP / 32; sub += a.wpx) {
@@ -507,32 +538,45 @@ __global__ __launch_bounds__(256, 2) void cn_classes_kernel(CnwArgs a) {
         }
         ms_h8 gh[NJ], gl[NJ];
         constexpr bool kG2 = WP == 2;          // planes of G: two for an fp32 dw
+        bool here = false;
+        int y4[2][4];
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
           const int pr = p0 + tt * 16 + q * 4;
-          const float4 f = *reinterpret_cast<const float4*>(&rows[0][pr]), ls = *reinterpret_cast<const float4*>(&rows[1][pr]), rr = *reinterpret_cast<const float4*>(&rows[2][pr]),
-                       gg = *reinterpret_cast<const float4*>(&rows[3][pr]);
+          const float4 f = *reinterpret_cast<const float4*>(&rows[0][pr]), ls = *reinterpret_cast<const float4*>(&rows[1][pr]);
           const int4 yy = *reinterpret_cast<const int4*>(&labs[pr]);
-          const float ff[4] = {f.x * wl2, f.y * wl2, f.z * wl2, f.w * wl2}, l4[4] = {ls.x, ls.y, ls.z, ls.w}, r4[4] = {rr.x, rr.y, rr.z, rr.w}, g4[4] = {gg.x, gg.y, gg.z, gg.w};
-          const int y4[4] = {yy.x - v0 - li, yy.y - v0 - li, yy.z - v0 - li, yy.w - v0 - li};
+          const float ff[4] = {f.x * wl2, f.y * wl2, f.z * wl2, f.w * wl2}, l4[4] = {ls.x, ls.y, ls.z, ls.w};
+          y4[tt][0] = yy.x - v0; y4[tt][1] = yy.y - v0; y4[tt][2] = yy.z - v0; y4[tt][3] = yy.w - v0;
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) {
-            float e[4];
+          for (int r = 0; r < 4; ++r) here |= (unsigned)y4[tt][r] < (unsigned)(NJ * 16);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) e[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][j][r], ff[r], bw[j]) - l4[r]);
-            if (__any(y4[0] == j * 16 || y4[1] == j * 16 || y4[2] == j * 16 || y4[3] == j * 16)) {
+          for (int j = 0; j < NJ; ++j)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) e[r] -= y4[r] == j * 16 ? 1.f : 0.f;
-            }
+            for (int r = 0; r < 4; ++r) s[tt][j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][j][r], ff[r], bw[j]) - l4[r]);
+        }
+        if (__any(here)) {             // some pixel's label is among this wave's classes
+#pragma unroll
+          for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) s[tt][j][r] -= y4[tt][r] - li == j * 16 ? 1.f : 0.f;
+        }
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+          const int pr = p0 + tt * 16 + q * 4;
+          const float4 rr = *reinterpret_cast<const float4*>(&rows[2][pr]), gg = *reinterpret_cast<const float4*>(&rows[3][pr]);
+          const float r4[4] = {rr.x * gn, rr.y * gn, rr.z * gn, rr.w * gn}, g4[4] = {gg.x, gg.y, gg.z, gg.w};
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              db[j] = __builtin_fmaf(e[r], g4[r], db[j]);
-              _Float16 x, y;
-              ce_split(e[r] * r4[r], x, y);
-              gh[j][tt * 4 + r] = x; gl[j][tt * 4 + r] = y;
+              db[j] = __builtin_fmaf(s[tt][j][r], g4[r], db[j]);
+              s[tt][j][r] *= r4[r];
             }
-          }
         }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) ce_split8(s[0][j], s[1][j], gh[j], gl[j]);
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
           const int row = c * 16 + li;
@@ -558,7 +602,7 @@ __global__ __launch_bounds__(256, 2) void cn_classes_kernel(CnwArgs a) {
     }
   }
   if (!busy) return;
-  const float back = ce_pow2(-gexp);
+  const float back = kmax < -50000 ? 0.f : ce_pow2(-min(max(kCeTopExp - kmax, -120), 120));
   const int split = blockIdx.x * a.wpx + wp_;
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
@@ -614,16 +658,13 @@ __global__ __launch_bounds__(1024) void cn_join_kernel(const float* __restrict__
 
 // ------------------------------------------------------------------------------------------------------------------------------ host
 struct CnPlan {
-  int KS, nch, Vp, nslots; long P, Pp, wgs; int nj; int njw, units, wpx, vblocks, tp, tiles, splits;
-  size_t o_img, o_slots, o_scal, o_lsum, o_fx, o_lse, o_gp, o_lab, o_dw, o_db, total;
+  int KS, nch, Vp, nslots; long P, Pp, wgs; int njw, units, wpx, vblocks, tp, tiles, splits;
+  size_t o_img, o_slots, o_lsum, o_fx, o_lse, o_gp, o_lab, o_dw, o_db, total;
 };
 static CnPlan cn_plan(int N, int C, int V, int HW, int types, bool grad) {
   CnPlan k{};
   k.KS = cdiv(C, 32); k.nch = cdiv(V, 64); k.Vp = k.nch * 64; k.P = (long)N * HW;
-  // Pixels of a wave: as many as its registers hold, fewer where the launch would leave compute units idle.
-  k.nj = k.KS <= 2 ? 4 : 2;
-  if (k.nj == 4 && k.P < 256L * 256) k.nj = 2;
-  k.wgs = (k.P + k.nj * 64 - 1) / (k.nj * 64);
+  k.wgs = (k.P + kCnNJ * 64 - 1) / (kCnNJ * 64);
   k.Pp = (k.P + 255) / 256 * 256;
   k.nslots = (int)std::min<long>(kCnPrep, k.P / 1024 + 1);
   k.njw = k.KS <= 2 && V > 32 ? 4 : 2;
@@ -637,7 +678,7 @@ static CnPlan cn_plan(int N, int C, int V, int HW, int types, bool grad) {
   size_t o = 0;
   auto take = [&](size_t n) { const size_t at = o; o += (n + 255) & ~(size_t)255; return at; };
   k.o_img = take((size_t)k.nch * ((size_t)((types & 2) ? 1 : 2) * 64 * k.KS * 64 + 1024));
-  k.o_slots = take(kCnPrep * 4); k.o_scal = take(64); k.o_lsum = take((size_t)k.wgs * 8);
+  k.o_slots = take(kCnPrep * 4); k.o_lsum = take((size_t)k.wgs * 8);
   if (grad) {
     k.o_fx = take(k.Pp * 4); k.o_lse = take(k.Pp * 4); k.o_gp = take(k.Pp * 4); k.o_lab = take(k.Pp * 4);
     k.o_dw = take((size_t)k.splits * k.wpx * k.Vp * k.KS * 32 * 4);
@@ -661,44 +702,33 @@ static int cn_run(const CeArgs& a, const CnPlan& k) {
   char* ws = (char*)a.ws;
   hipStream_t st = a.st;
   int* slots = (int*)(ws + k.o_slots);
-  int* scal = (int*)(ws + k.o_scal);
-  MS_LAUNCH((cn_prep_kernel<WT, WP, KS>), dim3(std::max(k.nch, a.mean_valid ? k.nslots : 1)), dim3(256), 0, st, a.w, a.b, a.labels, k.P, a.mean_valid, ws + k.o_img, slots, k.nslots, scal, a.V,
-            k.nch, a.C);
+  MS_LAUNCH((cn_prep_kernel<WT, WP, KS>), dim3(std::max(k.nch, a.mean_valid ? k.nslots : 1)), dim3(256), 0, st, a.w, a.b, a.labels, k.P, a.mean_valid, ws + k.o_img, slots, k.nslots, a.V, k.nch, a.C);
   if (int e = check_launch("class_ce_prep")) return e;
   CnArgs p{};
-  p.h = a.h; p.w = a.w; p.labels = a.labels; p.img = ws + k.o_img; p.slots = slots; p.nslots = k.nslots; p.scal = scal;
+  p.h = a.h; p.w = a.w; p.labels = a.labels; p.img = ws + k.o_img; p.slots = slots; p.nslots = k.nslots;
   p.nll = a.nll; p.lse_out = a.lse; p.lse_in = a.lse_in; p.grad = a.grad; p.scale_dev = a.scale_dev; p.sign = a.sign; p.mean_valid = a.mean_valid; p.drop = need_grad ? 1 : 0;
   p.dh = a.dh; p.lsum = a.loss != nullptr ? (double*)(ws + k.o_lsum) : nullptr;
   if (need_dw) { p.fx = (float*)(ws + k.o_fx); p.lse2 = (float*)(ws + k.o_lse); p.gp = (float*)(ws + k.o_gp); p.lab = (int*)(ws + k.o_lab); }
+  p.w_vec = a.C % 4 == 0 && (reinterpret_cast<uintptr_t>(a.w) & (4 * sizeof(WT) - 1)) == 0;
   p.P = k.P; p.C = a.C; p.HW = a.HW; p.V = a.V; p.nch = k.nch;
   const dim3 grid((unsigned)k.wgs), block(256);
-  if constexpr (KS <= 2) {
-    if (k.nj == 4 && a.dh != nullptr) MS_LAUNCH((cn_pixels_kernel<HT, WT, KS, 4, true>), grid, block, 0, st, p);
-    else if (k.nj == 4) MS_LAUNCH((cn_pixels_kernel<HT, WT, KS, 4, false>), grid, block, 0, st, p);
-  }
-  if (k.nj == 2 && a.dh != nullptr) MS_LAUNCH((cn_pixels_kernel<HT, WT, KS, 2, true>), grid, block, 0, st, p);
-  else if (k.nj == 2) MS_LAUNCH((cn_pixels_kernel<HT, WT, KS, 2, false>), grid, block, 0, st, p);
+  if (a.dh != nullptr) MS_LAUNCH((cn_pixels_kernel<HT, WT, KS, kCnNJ, true>), grid, block, 0, st, p);
+  else MS_LAUNCH((cn_pixels_kernel<HT, WT, KS, kCnNJ, false>), grid, block, 0, st, p);
   if (int e = check_launch("class_ce_pixels")) return e;
   if (need_dw) {
     CnwArgs c{};
-    c.h = a.h; c.img = p.img; c.fx = p.fx; c.lse2 = p.lse2; c.gp = p.gp; c.lab = p.lab; c.scal = scal;
+    c.h = a.h; c.img = p.img; c.fx = p.fx; c.lse2 = p.lse2; c.gp = p.gp; c.lab = p.lab;
     c.dwp = (float*)(ws + k.o_dw); c.dbp = (float*)(ws + k.o_db); c.dw_split = (size_t)k.Vp * KS * 32; c.db_split = k.Vp;
     c.P = k.P; c.C = a.C; c.HW = a.HW; c.V = a.V; c.units = k.units; c.wpx = k.wpx; c.splits = k.splits; c.tiles = k.tiles;
     const dim3 gw((unsigned)k.splits, (unsigned)k.vblocks);
     const bool vec = a.HW % 8 == 0 && aligned16(a.h);          // 8-pixel groups that never cross an image, in whole vectors
     constexpr int TP = KS <= 2 ? 128 : 64;
     if constexpr (KS <= 2) {
-      if (k.njw == 4) {
-        if (vec) MS_LAUNCH((cn_classes_kernel<HT, WT, KS, 4, TP, true>), gw, block, 0, st, c);
-        else MS_LAUNCH((cn_classes_kernel<HT, WT, KS, 4, TP, false>), gw, block, 0, st, c);
-      } else {
-        if (vec) MS_LAUNCH((cn_classes_kernel<HT, WT, KS, 2, TP, true>), gw, block, 0, st, c);
-        else MS_LAUNCH((cn_classes_kernel<HT, WT, KS, 2, TP, false>), gw, block, 0, st, c);
-      }
-    } else {
-      if (vec) MS_LAUNCH((cn_classes_kernel<HT, WT, KS, 2, TP, true>), gw, block, 0, st, c);
-      else MS_LAUNCH((cn_classes_kernel<HT, WT, KS, 2, TP, false>), gw, block, 0, st, c);
+      if (k.njw == 4 && vec) MS_LAUNCH((cn_classes_kernel<HT, WT, KS, 4, TP, true>), gw, block, 0, st, c);
+      else if (k.njw == 4) MS_LAUNCH((cn_classes_kernel<HT, WT, KS, 4, TP, false>), gw, block, 0, st, c);
     }
+    if (k.njw == 2 && vec) MS_LAUNCH((cn_classes_kernel<HT, WT, KS, 2, TP, true>), gw, block, 0, st, c);
+    else if (k.njw == 2) MS_LAUNCH((cn_classes_kernel<HT, WT, KS, 2, TP, false>), gw, block, 0, st, c);
     if (int e = check_launch("class_ce_classes")) return e;
   }
   if (need_dw || a.loss != nullptr) {
