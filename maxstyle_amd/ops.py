@@ -406,6 +406,9 @@ def mse_loss(x, target):
 # ---------------------------------------------------------------------------------------------------------
 # head + cross entropy over many classes (the logits are never kept)
 # ---------------------------------------------------------------------------------------------------------
+HEAD_MAX_CLASSES = 4         # ms_head_ce's (head_ce): beyond it class_ce
+
+
 def _class_ce_args(h, w, b, labels):
     """Checks of the ms_class_ce family: (N, C, V, HW, types) of h [N,C,*spatial] (rows of features: [T,C]), w [V,C] or [V,C,1,1], b [V] | None, labels [N,*spatial]."""
     for name, t in (("h", h), ("w", w)):

@@ -49,6 +49,8 @@ class EngineOptions:
     xfin: bool = True                 # cross-workgroup BatchNorm finalize inside the consuming launch (`_xfin` entry points; needs an exclusive device)
     xfin_pro: bool = True             # ... also for consumers that need the coefficients in their prologue
     train_xfin: bool = False          # `_xfin` in the training engine's forward passes (-0.1 ms of 23: off)
+    train_act8: bool = False          # training passes keep the blocks' activations in 8 bits between forward and backward (ops.act8_*): 1/4 of their memory; the weight gradients
+                                      # then carry the checkpoints' rounding (the forward pass and the losses do not).  NOT bit-identical.  Not with MixStyle inside the encoder
     train_graph: bool = False         # training passes replayed from captured HIP graphs (same wall as eager: off)
 
     def replace(self, **kw):

@@ -22,6 +22,7 @@ import ctypes
 from typing import Dict, Optional
 
 import os
+import re
 
 import torch
 
@@ -103,9 +104,18 @@ class ParamBank:
               "ms_adamw_step")
 
 
+_ACT8_NAME = re.compile(r"(?:e\.d|s\.u|d\.u)([1-4])\.(xu|xd|u1|u2|out)$|e\.inc\.(ua|ub|out)$")
+
+
 class TrainEngine(InnerLoopEngine):
     """One forward/backward of the segmentation + reconstruction training pass.  Activations stay in this engine's buffers until
-    `backward_pass`; use one TrainEngine per pass that is alive at the same time (standard pass, hard-example pass)."""
+    `backward_pass`; use one TrainEngine per pass that is alive at the same time (standard pass, hard-example pass).
+
+    EngineOptions.train_act8: what the blocks save for the backward (raw conv outputs, block outputs, resampled inputs) is kept as 8-bit checkpoints
+    (ms_act8_pack: 8.125 bits an element, signs exact) and the fp32 tensors pass through a handful of buffers that all blocks share.  The backward reads a block's
+    checkpoints where it needs no more than signs and sums (ms_act8_bwd_reduce) and writes the fp32 tensors the convolutions read back into the shared buffers."""
+
+    act8 = False
 
     def __init__(self, spec: NetSpec, B: int, H: int, W: int, device, options=None):
         super().__init__(spec, B, H, W, device, options=options)
@@ -121,8 +131,69 @@ class TrainEngine(InnerLoopEngine):
         # per trainer iteration - the ~230 launches of a pass are not host-bound (4.5 ms of kernels in 6 ms of wall, the rest is launch boundaries
         # that a graph has too), so it is off by default (EngineOptions.train_graph turns it on).
         self.graph_passes = bool(self.options.train_graph)
+        self.act8 = bool(self.options.train_act8)
+        self._act8_pool = {}             # role -> flat fp32 buffer
         self._pgraphs = {}
         self.configure_styles([], {})
+
+    # ------------------------------------------------------------------ 8-bit checkpoints (EngineOptions.train_act8)
+    @staticmethod
+    def _act8_role(name):
+        """The shared buffer an activation passes through, None if it is kept in fp32 (the heads' inputs and the encoder's last block: read once more outside a block)."""
+        m = _ACT8_NAME.match(name)
+        if m is None or name in ("s.u4.out", "d.u4.out", "e.d4.out"):
+            return None
+        if m.group(3):
+            return {"ua": "u1", "ub": "u2", "out": "out0"}[m.group(3)]
+        role = m.group(2)
+        if role == "out":
+            return "out" + str(int(m.group(1)) & 1)          # a block's input and output are neighbours: two buffers in turn
+        return "src" if role in ("xu", "xd") else role
+
+    def t(self, name, *shape, dtype=F32, zero=True):
+        role = self._act8_role(name) if self.act8 else None
+        if role is None:
+            return super().t(name, *shape, dtype=dtype, zero=zero)
+        b = self.buf.get(name)
+        if b is None or tuple(b.shape) != tuple(shape):
+            if b is not None and self._any_graph():
+                raise RuntimeError(f"buffer {name} would be re-allocated while a captured graph holds its address")
+            n = 1
+            for k in shape:
+                n *= int(k)
+            pool = self._act8_pool.get(role)
+            if pool is None:
+                pool = self._act8_pool[role] = torch.empty(max(n, self.B * self.spec.widths[0] * self.H * self.W), dtype=F32, device=self.dev)
+            b = self.buf[name] = pool[:n].view(shape) if n <= pool.numel() else torch.empty(*shape, dtype=F32, device=self.dev)
+        return b
+
+    def _act8_keep(self, name, coef=None):
+        """Checkpoint of the activation `name` (coef: name of the BatchNorm record of a raw conv output)."""
+        x = self.buf[name]
+        N, C, H, W = x.shape
+        q = self.t(name + ".q8", N, C, H, W, dtype=torch.int8, zero=False)
+        s = self.t(name + ".s8", N, C, (H * W + ops.ACT8_BLOCK - 1) // ops.ACT8_BLOCK, zero=False)
+        check(lib.ms_act8_pack(x.data_ptr(), 0 if coef is None else self.buf[coef].data_ptr(), q.data_ptr(), s.data_ptr(), N, C, H * W, self._st()), "ms_act8_pack:" + name)
+
+    def _act8_restore(self, name, coef=None):
+        x, q, s = self.buf[name], self.buf[name + ".q8"], self.buf[name + ".s8"]
+        N, C, H, W = x.shape
+        check(lib.ms_act8_unpack(q.data_ptr(), s.data_ptr(), 0 if coef is None else self.buf[coef].data_ptr(), x.data_ptr(), N, C, H * W, self._st()), "ms_act8_unpack:" + name)
+
+    def res_fwd(self, pfx, net, key, x, kind, **kw):
+        if not self.act8:
+            return super().res_fwd(pfx, net, key, x, kind, **kw)
+        if pfx == "e.d1":                # the double conv in front of the encoder's blocks is complete: its buffers are the blocks' from here on
+            self._act8_keep("e.inc.ua", "e.inc.bn1.coef")
+            self._act8_keep("e.inc.ub", "e.inc.bn4.coef")
+            self._act8_keep("e.inc.out")
+        out = super().res_fwd(pfx, net, key, x, kind, **kw)
+        self._act8_keep(pfx + ".u1", pfx + ".bn1.coef")
+        self._act8_keep(pfx + ".u2", pfx + ".bn4.coef")
+        if kind != "nn":
+            self._act8_keep(pfx + (".xu" if kind == "convT" else ".xd"))
+        self._act8_keep(pfx + ".out")
+        return out
 
     # ------------------------------------------------------------------ helpers
     def _names(self, net):
@@ -184,14 +255,22 @@ class TrainEngine(InnerLoopEngine):
         ws = self.t("cs.ws", max(lib.ms_channel_sum_ws_bytes(N, self.spec.code_ch), 64), dtype=torch.uint8)
         check(lib.ms_channel_sum(x.data_ptr(), N, C, H * W, out.data_ptr(), 1, ws.data_ptr(), ws.numel(), self._st()), "ms_channel_sum")
 
-    def act_bwd_t(self, name, gin, ref, u, coef, slope, net, bn_key, dsum=None):
-        """Mask gin in place, BatchNorm-backward coefficients, BatchNorm parameter gradients (+ dsum: bias.grad of the residual 1x1 conv)."""
+    def act_bwd_t(self, name, gin, ref, u, coef, slope, net, bn_key, dsum=None, kept=None):
+        """Mask gin in place, BatchNorm-backward coefficients, BatchNorm parameter gradients (+ dsum: bias.grad of the residual 1x1 conv).
+        kept = (name of ref, name of u): both are 8-bit checkpoints; the mask comes from ref's signs, and `u` receives its fp32 values for the convolutions behind."""
         N, C, H, W = u.shape
-        nparts = lib.ms_act_bwd_parts(N, C, H * W)
-        part = self.t(name + ".part", C, nparts, 2)
         bc = self.t(name + ".bcoef", C, 4)
-        check(lib.ms_act_bwd_reduce(gin.data_ptr(), 0 if ref is None else ref.data_ptr(), u.data_ptr(), coef.data_ptr(), gin.data_ptr(), part.data_ptr(),
-                                    N, C, H * W, slope, self._st()), "ms_act_bwd_reduce:" + name)
+        if kept is not None:
+            b = self.buf
+            nparts = lib.ms_act8_bwd_parts(N, C, H * W)
+            part = self.t(name + ".part", C, nparts, 2)
+            check(lib.ms_act8_bwd_reduce(gin.data_ptr(), b[kept[0] + ".q8"].data_ptr(), b[kept[1] + ".q8"].data_ptr(), b[kept[1] + ".s8"].data_ptr(), coef.data_ptr(),
+                                         gin.data_ptr(), u.data_ptr(), part.data_ptr(), N, C, H * W, slope, self._st()), "ms_act8_bwd_reduce:" + name)
+        else:
+            nparts = lib.ms_act_bwd_parts(N, C, H * W)
+            part = self.t(name + ".part", C, nparts, 2)
+            check(lib.ms_act_bwd_reduce(gin.data_ptr(), 0 if ref is None else ref.data_ptr(), u.data_ptr(), coef.data_ptr(), gin.data_ptr(), part.data_ptr(),
+                                        N, C, H * W, slope, self._st()), "ms_act_bwd_reduce:" + name)
         dg = db = None
         if self.bn_affine_grad:
             dg, db = self._gw(net, bn_key), self._gb(net, bn_key)
@@ -263,6 +342,8 @@ class TrainEngine(InnerLoopEngine):
 
     def run_forward(self, image, labels, clean, track: bool, net_bns=None):
         """forward_pass on engine-owned copies of the inputs (a captured graph holds addresses); see `graph_passes`."""
+        if self.act8 and self.enc_mix is not None:
+            raise NotImplementedError("train_act8 with MixStyle layers inside the encoder (they keep their own activations in fp32)")
         xi, li, ci = self._static_inputs(image, labels, clean)
         if not self.graph_passes or self.enc_mix is not None:        # (the MixStyle layers allocate their outputs: not capturable)
             return self.forward_pass(xi, li, ci, track, net_bns)
@@ -363,7 +444,15 @@ class TrainEngine(InnerLoopEngine):
         c0, c3, ci = tbl[key + ".c0"], tbl[key + ".c3"], tbl[key + ".ci"]
         u1, u2 = b[pfx + ".u1"], b[pfx + ".u2"]
         cf1 = b[pfx + ".bn1.coef"]
-        g2, bc2 = self.act_bwd_t(pfx + ".bw2", dout, b[pfx + ".out"], u2, b[pfx + ".bn4.coef"], LEAKY, net, key + ".bn4", dsum=self._gb(net, key + ".ci"))
+        if self.act8:
+            i = int(pfx[-1])
+            if pfx == "e.d1" or i > 1:                         # (the first decoder blocks read the codes, which stay in fp32)
+                self._act8_restore("e.inc.out" if pfx == "e.d1" else pfx[:-1] + str(i - 1) + ".out")
+            self._act8_restore(pfx + ".u1", pfx + ".bn1.coef")
+            if kind != "nn":
+                self._act8_restore(pfx + (".xu" if kind == "convT" else ".xd"))
+        g2, bc2 = self.act_bwd_t(pfx + ".bw2", dout, b[pfx + ".out"], u2, b[pfx + ".bn4.coef"], LEAKY, net, key + ".bn4", dsum=self._gb(net, key + ".ci"),
+                                 kept=(pfx + ".out", pfx + ".u2") if self.act8 else None)
         self.wgrad(g2, u1, self._gw(net, key + ".c3"), 3, p_bnbwd=(bc2, u2), q_act=(cf1, LEAKY))
         g1, bc1 = self.dgrad_act_bwd_t(pfx + ".da1", pfx + ".bw1", g2, c3, (bc2, u2), u1, cf1, LEAKY, net, key + ".bn1")
         src = x if kind == "nn" else (b[pfx + ".xu"] if kind == "convT" else b[pfx + ".xd"])
@@ -472,7 +561,9 @@ class TrainEngine(InnerLoopEngine):
             prev = "e.inc.out" if i == 1 else f"e.d{i - 1}.out"
             dh = self.res_bwd_t(f"e.d{i}", net_e, f"d{i}", self._mixed(i, prev), dh, "down")
             dh = self._mix_bwd(i, dh, b[prev])
-        g, bc = self.act_bwd_t("e.inc.bw2", dh, b["e.inc.out"], b["e.inc.ub"], b["e.inc.bn4.coef"], LEAKY, net_e, "inc4")
+        if self.act8:
+            self._act8_restore("e.inc.ua", "e.inc.bn1.coef")
+        g, bc = self.act_bwd_t("e.inc.bw2", dh, b["e.inc.out"], b["e.inc.ub"], b["e.inc.bn4.coef"], LEAKY, net_e, "inc4", kept=("e.inc.out", "e.inc.ub") if self.act8 else None)
         self.wgrad(g, b["e.inc.ua"], self._gw(net_e, "inc3"), 3, p_bnbwd=(bc, b["e.inc.ub"]), q_act=(b["e.inc.bn1.coef"], LEAKY))
         g, bc = self.dgrad_act_bwd_t("e.inc.da", "e.inc.bw1", g, e["inc3"], (bc, b["e.inc.ub"]), b["e.inc.ua"], b["e.inc.bn1.coef"], LEAKY, net_e, "inc1")
         self.wgrad(g, image, self._gw(net_e, "inc0"), 3, p_bnbwd=(bc, b["e.inc.ua"]))      # the input image needs no gradient

@@ -178,6 +178,18 @@ def test_agrees_with_the_small_head():
     assert (dh - dh2).abs().max() < 1e-6 * dh.abs().max()
 
 
+@pytest.mark.parametrize("c", [4, 5, 21, 150])
+def test_cross_entropy_2D_of_any_number_of_classes(c):
+    g = torch.Generator().manual_seed(c)
+    z = torch.randn(2, c, 17, 19, generator=g).cuda() * 3
+    lab = torch.randint(0, c, (2, 17, 19), generator=g).cuda()
+    zd = z.double()
+    want = (torch.logsumexp(zd, 1) - zd.gather(1, lab.unsqueeze(1)).squeeze(1)).mean()
+    # each pixel within 2 |z| 3 2^-22 (the planes) + 16 u32 of its log-sum and loss
+    tol = (6 * 2.0 ** -22 + 32 * U32) * float(zd.abs().max() + want + 6)
+    assert abs(float(maxstyle_amd.cross_entropy_2D(z, lab)) - float(want)) <= tol
+
+
 def test_no_row_takes_part():
     h, w, b, lab = make((2, 16, 9, 9), 11)
     lab.fill_(11)
