@@ -171,17 +171,17 @@ template <typename AT> struct A8Vec<AT, false> {
   static __device__ __forceinline__ int get(int w, int) { return w; }
 };
 
-// First pass: partial sums of g' and g' (x' - mean) of each (plane, segment) -> part[c][n S + s], the layout ms_bn_bwd_full reads; optionally g' and x' themselves
-// (the training engine's convolutions read both).  Planes of channels [c0, c0 + nc).
-template <typename AT, bool VEC>
+// First pass: partial sums of g' and g' (x' - mean) of each (plane, segment) -> part[c][n S + s], the layout ms_bn_bwd_full reads; with OUT optionally g' and x'
+// themselves (the training engine's convolutions read both).
+template <typename AT, bool VEC, bool OUT>
 __global__ __launch_bounds__(kA8Threads) void act8_bwd_reduce_kernel(const void* __restrict__ gin, const int8_t* __restrict__ ref, const int8_t* __restrict__ q,
                                                                      const float* __restrict__ s, const float4* __restrict__ coef, void* __restrict__ gout, void* __restrict__ uout,
-                                                                     float2* __restrict__ part, int c0, int nc, int C, int HW, int nb, int seg, int S, int N, float slope) {
+                                                                     float2* __restrict__ part, int C, int HW, int nb, int seg, int S, int N, float slope) {
   using V = A8Vec<AT, VEC>;
   __shared__ float red[16];
   const int si = blockIdx.x % S, pl = blockIdx.x / S;
-  const int n = pl / nc, c = c0 + (pl - n * nc);
-  const size_t plane = (size_t)n * C + c, base = plane * HW;
+  const int n = pl / C, c = pl - n * C;
+  const size_t plane = (size_t)pl, base = plane * HW;
   const A8Chan a = a8_chan(coef, c, ref != nullptr);
   const int beg = si * seg, end = min(HW, beg + seg);
   float s1 = 0.f, s2 = 0.f;
@@ -198,10 +198,10 @@ __global__ __launch_bounds__(kA8Threads) void act8_bwd_reduce_kernel(const void*
       o[j] = a8_on(a, k, V::get(rw, j), sc) ? g[j] : g[j] * slope;
       s1 += o[j];
       s2 += o[j] * (a.off + (float)k * sc);
-      if (uout != nullptr) u[j] = (float)(a.ctr + (double)k * (double)sc);
+      if (OUT && uout != nullptr) u[j] = (float)(a.ctr + (double)k * (double)sc);
     }
-    if (gout != nullptr) V::stg(gout, base + i, o);
-    if (uout != nullptr) V::stg(uout, base + i, u);
+    if (OUT && gout != nullptr) V::stg(gout, base + i, o);
+    if (OUT && uout != nullptr) V::stg(uout, base + i, u);
   }
   s1 = block_sum(s1, red);
   s2 = block_sum(s2, red);
@@ -214,17 +214,19 @@ __device__ __forceinline__ A8Coef a8_coef(const float4 f, double s1, double s2, 
   return A8Coef{f.x, (float)(s1 / count), (float)(s2 * (double)f.w * (double)f.w / count)};
 }
 
-// Second pass: every workgroup sums its channel's partials again (N S of them, fixed order, 64 bits), then writes its segment of du.
+// Second pass: every workgroup sums its channel's partials again (N S of them, fixed order, 64 bits), then writes its segment of du.  Channels in groups whose data stays
+// in the last-level cache between the passes were slower at every group size (24 .. 160 MB: 567 .. 224 us against 194 in one group).
 template <typename AT, bool VEC>
 __global__ __launch_bounds__(kA8Threads) void act8_bwd_apply_kernel(const void* __restrict__ gin, const int8_t* __restrict__ ref, const int8_t* __restrict__ q,
                                                                     const float* __restrict__ s, const float4* __restrict__ coef, const float2* __restrict__ part,
                                                                     void* __restrict__ du, float* __restrict__ dgamma, float* __restrict__ dbeta,
-                                                                    int c0, int nc, int C, int HW, int nb, int seg, int S, int N, float slope) {
+                                                                    int C, int HW, int nb, int seg, int S, int N, float slope) {
   using V = A8Vec<AT, VEC>;
   __shared__ double redd[16];
-  const int si = blockIdx.x % S, pl = blockIdx.x / S;
-  const int n = pl / nc, c = c0 + (pl - n * nc);
-  const size_t plane = (size_t)n * C + c, base = plane * HW;
+  const int id = gridDim.x - 1 - blockIdx.x;        // from the end: what the first pass read last is still in the last-level cache (193 -> 188 us at 16x64x256x256)
+  const int si = id % S, pl = id / S;
+  const int n = pl / C, c = pl - n * C;
+  const size_t plane = (size_t)pl, base = plane * HW;
   const A8Chan a = a8_chan(coef, c, ref != nullptr);
   const float4 f = coef[c];
   double d1 = 0.0, d2 = 0.0;
@@ -305,9 +307,9 @@ static int act8_bwd_reduce_impl(const void* gin, const int8_t* ref, const int8_t
   const int nb = cdiv(HW, kA8Block);
   hipStream_t st = (hipStream_t)stream;
   if (a8_bwd_vec<AT>(gin, ref, q, gout, uout, HW))
-    MS_LAUNCH((act8_bwd_reduce_kernel<AT, true>), grid, block, 0, st, gin, ref, q, s, (const float4*)coef4, gout, uout, (float2*)part2, 0, C, C, HW, nb, sp.seg, sp.S, N, slope);
+    MS_LAUNCH((act8_bwd_reduce_kernel<AT, true, true>), grid, block, 0, st, gin, ref, q, s, (const float4*)coef4, gout, uout, (float2*)part2, C, HW, nb, sp.seg, sp.S, N, slope);
   else
-    MS_LAUNCH((act8_bwd_reduce_kernel<AT, false>), grid, block, 0, st, gin, ref, q, s, (const float4*)coef4, gout, uout, (float2*)part2, 0, C, C, HW, nb, sp.seg, sp.S, N, slope);
+    MS_LAUNCH((act8_bwd_reduce_kernel<AT, false, true>), grid, block, 0, st, gin, ref, q, s, (const float4*)coef4, gout, uout, (float2*)part2, C, HW, nb, sp.seg, sp.S, N, slope);
   return check_launch("act8_bwd_reduce");
 }
 
@@ -323,13 +325,14 @@ static int act8_bn_act_bwd_impl(const void* g, const int8_t* ref, const int8_t* 
   const int nb = cdiv(HW, kA8Block);
   hipStream_t st = (hipStream_t)stream;
   const bool vec = a8_bwd_vec<AT>(g, ref, q, du, nullptr, HW);
-  dim3 block(kA8Threads), grid(N * C * sp.S);
+  dim3 block(kA8Threads);
+  const dim3 grid(N * C * sp.S);
 #define A8_ARGS(PART) st, g, ref, q, s, (const float4*)coef4, PART
-  if (vec) MS_LAUNCH((act8_bwd_reduce_kernel<AT, true>), grid, block, 0, A8_ARGS(nullptr), nullptr, (float2*)ws, 0, C, C, HW, nb, sp.seg, sp.S, N, slope);
-  else MS_LAUNCH((act8_bwd_reduce_kernel<AT, false>), grid, block, 0, A8_ARGS(nullptr), nullptr, (float2*)ws, 0, C, C, HW, nb, sp.seg, sp.S, N, slope);
+  if (vec) MS_LAUNCH((act8_bwd_reduce_kernel<AT, true, false>), grid, block, 0, A8_ARGS(nullptr), nullptr, (float2*)ws, C, HW, nb, sp.seg, sp.S, N, slope);
+  else MS_LAUNCH((act8_bwd_reduce_kernel<AT, false, false>), grid, block, 0, A8_ARGS(nullptr), nullptr, (float2*)ws, C, HW, nb, sp.seg, sp.S, N, slope);
   if (int e = check_launch("act8_bwd_reduce")) return e;
-  if (vec) MS_LAUNCH((act8_bwd_apply_kernel<AT, true>), grid, block, 0, A8_ARGS((const float2*)ws), du, dgamma, dbeta, 0, C, C, HW, nb, sp.seg, sp.S, N, slope);
-  else MS_LAUNCH((act8_bwd_apply_kernel<AT, false>), grid, block, 0, A8_ARGS((const float2*)ws), du, dgamma, dbeta, 0, C, C, HW, nb, sp.seg, sp.S, N, slope);
+  if (vec) MS_LAUNCH((act8_bwd_apply_kernel<AT, true>), grid, block, 0, A8_ARGS((const float2*)ws), du, dgamma, dbeta, C, HW, nb, sp.seg, sp.S, N, slope);
+  else MS_LAUNCH((act8_bwd_apply_kernel<AT, false>), grid, block, 0, A8_ARGS((const float2*)ws), du, dgamma, dbeta, C, HW, nb, sp.seg, sp.S, N, slope);
 #undef A8_ARGS
   return check_launch("act8_bwd_apply");
 }

@@ -16,17 +16,12 @@ namespace ms {
 constexpr size_t kCePieceBytes = (size_t)128 << 20;
 
 // ------------------------------------------------------------------------------------------------------------------------------ small passes
-// scal[0]: rows that take part; scal[1]: max over rows of exponent(g_p) + ex[p]; scal[2]: max over classes of ew[v]   (integers: their order does not matter)
-__global__ void ce_init_kernel(int* scal) {
-  if (threadIdx.x == 0) { scal[0] = 0; scal[1] = -100000; scal[2] = -100000; }
-}
-
 // Rows [rows][C] -> planes [rows_pad][Cp] and each row's 2^e.  One wave a row; 8 channels a lane where the rows are made of whole vectors.
-//   weights: bpad[v] = b or -inf behind the last class; features (labels != nullptr): a row that takes no part is packed as zeros when `drop` is set (it may hold anything)
+//   weights: bpad[v] = b log2(e), or -inf behind the last class; features (labels != nullptr): a row that takes no part is packed as zeros when `drop` is set (it may hold anything)
 template <typename WT, int PL, bool VEC>
 __global__ __launch_bounds__(256) void ce_pack_rows_kernel(const void* __restrict__ w, const float* __restrict__ b, const int64_t* __restrict__ labels, int classes, int drop,
                                                            _Float16* __restrict__ out, size_t plane, float* __restrict__ fw, float* __restrict__ bpad,
-                                                           int* __restrict__ lab32, int* __restrict__ scal, int rows, int rows_pad, int C, int Cp) {
+                                                           int* __restrict__ lab32, int rows, int rows_pad, int C, int Cp) {
   using IO = ActIO<WT>;
   const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (r >= rows_pad) return;
@@ -56,9 +51,7 @@ __global__ __launch_bounds__(256) void ce_pack_rows_kernel(const void* __restric
   const float inv = ce_pow2(-e);
   if (lane == 0) {
     fw[r] = ce_pow2(e);
-    if (bpad != nullptr) bpad[r] = r < rows ? (b != nullptr ? b[r] : 0.f) : -__builtin_inff();
-    // (looked at first: 32768 rows' atomics on one word took 370 us, this 10)
-    if (bpad != nullptr && r < rows && e > __hip_atomic_load(&scal[2], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(&scal[2], e);
+    if (bpad != nullptr) bpad[r] = r < rows ? (b != nullptr ? b[r] * kLog2e : 0.f) : -__builtin_inff();
   }
   for (int c = lane * 8; c < Cp; c += 512) {
     float v[8];
@@ -117,49 +110,87 @@ __global__ __launch_bounds__(1024) void ce_pack_planes_kernel(const void* __rest
   }
 }
 
-// rows that take part (for the mean over them)
-__global__ __launch_bounds__(256) void ce_count_kernel(const int64_t* __restrict__ labels, long P, int classes, int* __restrict__ scal) {
+// rows that take part (for the mean over them): slots[workgroup]
+constexpr int kCeSlots = 256, kCeRowBlocks = 1024;
+__global__ __launch_bounds__(256) void ce_count_kernel(const int64_t* __restrict__ labels, long P, int classes, int* __restrict__ slots) {
+  __shared__ int red[4];
   int k = 0;
   for (long p = (long)blockIdx.x * 256 + threadIdx.x; p < P; p += (long)gridDim.x * 256) { const int64_t l = labels[p]; k += (l >= 0 && l < classes) ? 1 : 0; }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) k += __shfl_xor(k, off, 64);
-  if ((threadIdx.x & 63) == 0 && k) atomicAdd(&scal[0], k);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = k;
+  __syncthreads();
+  if (threadIdx.x == 0) slots[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+}
+__device__ __forceinline__ int ce_count(const int* __restrict__ slots, int n, int* red /* 4 */) {       // by the first 256 threads of a workgroup; all get the sum
+  int s = threadIdx.x < (unsigned)n ? slots[threadIdx.x] : 0;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+  if (threadIdx.x < 256 && (threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  return red[0] + red[1] + red[2] + red[3];
 }
 
-// The upstream gradient of every row: grad[p], or sign / rows (rows that take part) times *scale_dev; 0 where the label is not a class.
+// The upstream gradient of every row: grad[p], or sign / rows (rows that take part) times *scale_dev; 0 where the label is not a class.  A row without one gets a log-sum
+// of infinity: exp(z - inf) = 0 whatever its logits are.  rowmax[workgroup]: the largest exponent of g_p 2^ex[p].
 __global__ __launch_bounds__(256) void ce_rowgrad_kernel(const float* __restrict__ grad, float sign, int mean_valid, const float* __restrict__ scale_dev, const int* __restrict__ lab32,
-                                                         const float* __restrict__ fx, float* __restrict__ gp, const float* __restrict__ lse_in, float* __restrict__ lse,
-                                                         int* __restrict__ scal, long P, long Pp) {
+                                                         const float* __restrict__ fx, float* __restrict__ gp, const float* __restrict__ lse_in, float* __restrict__ lse2,
+                                                         const int* __restrict__ slots, int nslots, int* __restrict__ rowmax, long P, long Pp) {
+  __shared__ int red[4];
+  const int cnt = mean_valid ? ce_count(slots, nslots, red) : 0;
+  const float g0 = grad != nullptr ? 0.f : sign / (float)(mean_valid ? max(cnt, 1) : P) * (scale_dev != nullptr ? *scale_dev : 1.f);
   int e = -100000;
   for (long p = (long)blockIdx.x * 256 + threadIdx.x; p < Pp; p += (long)gridDim.x * 256) {
     float g = 0.f;
-    if (p < P && lab32[p] >= 0) {
-      if (grad != nullptr) g = grad[p];
-      else g = sign / (float)(mean_valid ? max(scal[0], 1) : P) * (scale_dev != nullptr ? *scale_dev : 1.f);
-      const unsigned b = __float_as_uint(g) & 0x7FFFFFFFu;
-      if (b != 0u && b < 0x7F800000u) e = max(e, (int)(b >> 23) - 126 + (int)(__float_as_uint(fx[p]) >> 23) - 127);
-    }
+    if (p < P && lab32[p] >= 0) g = grad != nullptr ? grad[p] : g0;
+    const unsigned b = __float_as_uint(g) & 0x7FFFFFFFu;
+    if (b != 0u && b < 0x7F800000u) e = max(e, (int)(b >> 23) - 126 + (int)(__float_as_uint(fx[p]) >> 23) - 127);
     gp[p] = g;
-    if (lse_in != nullptr) lse[p] = p < P ? lse_in[p] : 0.f;        // (the caller's has no padding)
+    if (g == 0.f) lse2[p] = __builtin_inff();
+    else if (lse_in != nullptr) lse2[p] = lse_in[p] * kLog2e;
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) e = max(e, __shfl_xor(e, off, 64));
-  if ((threadIdx.x & 63) == 0 && e > __hip_atomic_load(&scal[1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(&scal[1], e);
-}
-// 2^k that brings the largest |G| 2^(ex + ew) below 2^14; and its reciprocal
-__device__ __forceinline__ int ce_gexp(const int* __restrict__ scal) {
-  const int a = scal[1], b = scal[2];
-  return (a < -50000 || b < -50000) ? 0 : min(max(kCeTopExp - (a + b), -120), 120);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = e;
+  __syncthreads();
+  if (threadIdx.x == 0) rowmax[blockIdx.x] = max(max(red[0], red[1]), max(red[2], red[3]));
 }
 
-// part[t][p] = {max, sum exp} over one class range -> lse, nll; loss partials in 64 bits.  64 rows a workgroup, 16 threads each over the class ranges.
+// One workgroup: the loss, and the power of two (scal[0]) that brings the largest |G| 2^(ex + ew) below 2^14.
+__global__ __launch_bounds__(1024) void ce_scalars_kernel(const double* __restrict__ lsum, int n, float sign, int mean_valid, const int* __restrict__ slots, int nslots, long P,
+                                                          float* __restrict__ loss, const int* __restrict__ rowmax, int nrow, const float* __restrict__ fw, int V, int* __restrict__ scal) {
+  __shared__ double redd[16];
+  __shared__ int redi[32];
+  if (loss != nullptr) {
+    const int cnt = mean_valid ? ce_count(slots, nslots, redi) : 0;
+    double a = 0.0;
+    for (int i = threadIdx.x; i < n; i += 1024) a += lsum[i];
+    a = block_sum_d(a, redd);
+    if (threadIdx.x == 0) loss[0] = (float)((double)sign * a / (double)(mean_valid ? max(cnt, 1) : P));
+  }
+  if (rowmax == nullptr) return;
+  int er = -100000, ew = -100000;
+  if ((int)threadIdx.x < nrow) er = rowmax[threadIdx.x];
+  for (int v = threadIdx.x; v < V; v += 1024) ew = max(ew, (int)(__float_as_uint(fw[v]) >> 23) - 127);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) { er = max(er, __shfl_xor(er, off, 64)); ew = max(ew, __shfl_xor(ew, off, 64)); }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) { redi[threadIdx.x >> 6] = er; redi[16 + (threadIdx.x >> 6)] = ew; }
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int k = 0; k < 16; ++k) { er = max(er, redi[k]); ew = max(ew, redi[16 + k]); }
+  scal[0] = er < -50000 ? 0 : min(max(kCeTopExp - (er + ew), -120), 120);
+}
+
+// part[t][p] = {max, sum exp} over one class range -> lse, nll; loss partials in 64 bits.  64 rows a workgroup, 16 threads each over the class ranges.  All in units of log2.
 __device__ __forceinline__ void ce_merge(float& m, float& l, float mo, float lo) {
   const float mn = fmaxf(m, mo), mm = mn == -__builtin_inff() ? 0.f : mn;
-  l = l * __builtin_amdgcn_exp2f((m - mm) * kLog2e) + lo * __builtin_amdgcn_exp2f((mo - mm) * kLog2e);
+  l = l * __builtin_amdgcn_exp2f(m - mm) + lo * __builtin_amdgcn_exp2f(mo - mm);
   m = mn;
 }
 __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict__ part, int nparts, size_t stride, const float* __restrict__ zlab, const int* __restrict__ lab32,
-                                                       float* __restrict__ lse, float* __restrict__ lse_out, float* __restrict__ nll_out, double* __restrict__ lsum, long P) {
+                                                       float* __restrict__ lse2, float* __restrict__ lse_out, float* __restrict__ nll_out, double* __restrict__ lsum, long P) {
   __shared__ float2 sh[16][64];
   const int el = threadIdx.x & 63, grp = threadIdx.x >> 6;
   const long p = (long)blockIdx.x * 64 + el;          // (padded)
@@ -170,24 +201,17 @@ __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict_
   __syncthreads();
   if (grp != 0) return;
   for (int k = 1; k < 16; ++k) ce_merge(m, l, sh[k][el].x, sh[k][el].y);
-  const float lg = logf(l), s = m + lg;
-  lse[p] = s;
+  const float lg = __builtin_amdgcn_logf(l), ln2 = 0.693147180559945309f;      // (log2)
+  lse2[p] = m + lg;
   double acc = 0.0;
   if (p < P) {
-    if (lse_out != nullptr) lse_out[p] = s;
-    const float v = lab32[p] >= 0 ? (m - zlab[p]) + lg : 0.f;        // (max - z) + log sum: nothing cancels where the label has the maximum
+    if (lse_out != nullptr) lse_out[p] = (m + lg) * ln2;
+    const float v = lab32[p] >= 0 ? ((m - zlab[p]) + lg) * ln2 : 0.f;        // (max - z) + log sum: nothing cancels where the label has the maximum
     if (nll_out != nullptr) nll_out[p] = v;
     acc = (double)v;
   }
   acc = wave_sum_d(acc);
   if (el == 0) lsum[blockIdx.x] = acc;
-}
-__global__ __launch_bounds__(256) void ce_loss_kernel(const double* __restrict__ lsum, int n, float sign, int mean_valid, const int* __restrict__ scal, long P, float* __restrict__ loss) {
-  __shared__ double redd[16];
-  double a = 0.0;
-  for (int i = threadIdx.x; i < n; i += 256) a += lsum[i];
-  a = block_sum_d(a, redd);
-  if (threadIdx.x == 0) loss[0] = (float)((double)sign * a / (double)(mean_valid ? max(scal[0], 1) : P));
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------ matrix products
@@ -322,43 +346,47 @@ __global__ __launch_bounds__(WM * WN * 64) void ce_gemm_kernel(CeGemm g) {
   }
 
   const int vbase = m0 + wm * TM + q * 4;           // class inside the piece
-  float fxp[NJ];
+  float fs[NJ];                                     // 2^ex log2(e)
   int lab[NJ];
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
     const size_t p = (size_t)g.p0 + n0 + wn * TN + j * 16 + li;
-    fxp[j] = g.fx[p]; lab[j] = g.lab[p] - g.v0;
-    if (g.lab[p] < 0) lab[j] = -1;
-  }
-#pragma unroll
-  for (int i = 0; i < MI; ++i) {
-    const float4 f = *reinterpret_cast<const float4*>(g.fw + g.v0 + vbase + i * 16), b = *reinterpret_cast<const float4*>(g.bpad + g.v0 + vbase + i * 16);
-    const float ff[4] = {f.x, f.y, f.z, f.w}, bb[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) acc[i][j][r] = acc[i][j][r] * ff[r] * fxp[j] + bb[r];
+    fs[j] = g.fx[p] * kLog2e;
+    const int y = g.lab[p];
+    lab[j] = y < 0 ? -1000000000 : y - g.v0 - vbase;             // label relative to this lane's first class
   }
   if (EPI == CE_STATS) {
 #pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const float4 f = *reinterpret_cast<const float4*>(g.fw + g.v0 + vbase + i * 16), b = *reinterpret_cast<const float4*>(g.bpad + g.v0 + vbase + i * 16);
+      const float ff[4] = {f.x, f.y, f.z, f.w}, bb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(acc[i][j][r] * ff[r], fs[j], bb[r]);
+    }
+#pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const size_t p = (size_t)g.p0 + n0 + wn * TN + j * 16 + li;
+      if (__any((unsigned)lab[j] < (unsigned)(MI * 16))) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) if (lab[j] == i * 16 + r) g.zlab[p] = acc[i][j][r];
+      }
       float mx = -__builtin_inff();
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          mx = fmaxf(mx, acc[i][j][r]);
-          if (vbase + i * 16 + r == lab[j]) g.zlab[p] = acc[i][j][r];
-        }
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[i][j][r]);
       mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
       mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      const float ms_ = mx == -__builtin_inff() ? 0.f : mx;
+      const float mm = mx == -__builtin_inff() ? 0.f : mx;
       float l = 0.f;
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) l += __builtin_amdgcn_exp2f((acc[i][j][r] - ms_) * kLog2e);
+        for (int r = 0; r < 4; ++r) l += __builtin_amdgcn_exp2f(acc[i][j][r] - mm);
       l += __shfl_xor(l, 16, 64);
       l += __shfl_xor(l, 32, 64);
       if (q == 0) g.part[(size_t)(mt * WM + wm) * g.part_stride + p] = make_float2(mx, l);
@@ -366,33 +394,35 @@ __global__ __launch_bounds__(WM * WN * 64) void ce_gemm_kernel(CeGemm g) {
     return;
   }
   if (EPI == CE_GRAD || EPI == CE_GRAD2) {
-    const float gn = ce_pow2(ce_gexp(g.scal));
-    float gp[NJ], ls[NJ];
+    const float gn = ce_pow2(g.scal[0]);
+    float gp[NJ], ls[NJ], rj[NJ];
+    bool here = false;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const size_t p = (size_t)g.p0 + n0 + wn * TN + j * 16 + li;
       gp[j] = g.gp[p]; ls[j] = g.lse[p];
+      rj[j] = gp[j] * g.fx[p] * gn;
+      here |= (unsigned)lab[j] < (unsigned)(MI * 16);
     }
+    here = __any(here);
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
-      const float4 f = *reinterpret_cast<const float4*>(g.fw + g.v0 + vbase + i * 16);
-      const float ff[4] = {f.x, f.y, f.z, f.w};
+      const float4 f = *reinterpret_cast<const float4*>(g.fw + g.v0 + vbase + i * 16), b = *reinterpret_cast<const float4*>(g.bpad + g.v0 + vbase + i * 16);
+      const float ff[4] = {f.x, f.y, f.z, f.w}, bb[4] = {b.x, b.y, b.z, b.w};
       float db[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        ms_h4 hi, lo;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r] * ff[r], fs[j], bb[r]) - ls[j]);
+        if (here) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[i][j][r] -= lab[j] == i * 16 + r ? 1.f : 0.f;
+        }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          float s = __builtin_amdgcn_exp2f((acc[i][j][r] - ls[j]) * kLog2e) - (vbase + i * 16 + r == lab[j] ? 1.f : 0.f);
-          s = gp[j] == 0.f ? 0.f : s * gp[j];          // a row that takes no part gives zeros, whatever its logits are
-          db[r] += s;
-          _Float16 a, b;
-          ce_split(s * fxp[j] * gn * ff[r], a, b);
-          hi[r] = a; lo[r] = b;
+          db[r] = __builtin_fmaf(acc[i][j][r], gp[j], db[r]);
+          acc[i][j][r] *= rj[j] * ff[r];
         }
-        const size_t at = (size_t)(n0 + wn * TN + j * 16 + li) * g.g_ld + vbase + i * 16;
-        *reinterpret_cast<ms_h4*>(g.g + at) = hi;
-        if (EPI == CE_GRAD2) *reinterpret_cast<ms_h4*>(g.g + g.g_plane + at) = lo;
       }
       if (g.dbpart != nullptr) {
 #pragma unroll
@@ -401,6 +431,33 @@ __global__ __launch_bounds__(WM * WN * 64) void ce_gemm_kernel(CeGemm g) {
           for (int off = 1; off < 16; off <<= 1) db[r] += __shfl_xor(db[r], off, 64);
         }
         if (li == 0) *reinterpret_cast<float4*>(g.dbpart + (size_t)(nt * WN + wn) * g.db_stride + vbase + i * 16) = make_float4(db[0], db[1], db[2], db[3]);
+      }
+    }
+    // G goes out through LDS as [row][class], 16 bytes a lane in whole rows
+    _Float16* tile = &sm[0][0];
+    constexpr int kCh = BM / 8;
+#pragma unroll
+    for (int pl = 0; pl < (EPI == CE_GRAD2 ? 2 : 1); ++pl) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          ms_h4 v;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const _Float16 hi = (_Float16)acc[i][j][r];
+            v[r] = pl == 0 ? hi : (_Float16)(acc[i][j][r] - (float)hi);
+          }
+          const int row = wn * TN + j * 16 + li, col = wm * TM + i * 16 + q * 4;
+          *reinterpret_cast<ms_h4*>(tile + row * BM + (((col >> 3) ^ (row & 15)) * 8) + (col & 7)) = v;
+        }
+      __syncthreads();
+      _Float16* out = g.g + pl * g.g_plane + (size_t)n0 * g.g_ld + m0;
+#pragma unroll
+      for (int k = 0; k < BN * kCh / (NW * 64); ++k) {
+        const int i = k * (NW * 64) + threadIdx.x, row = i / kCh, ch = i % kCh;
+        *reinterpret_cast<ms_h8*>(out + (size_t)row * g.g_ld + ch * 8) = *reinterpret_cast<const ms_h8*>(tile + row * BM + ((ch ^ (row & 15)) * 8));
       }
     }
   }
@@ -413,7 +470,7 @@ __global__ __launch_bounds__(WM * WN * 64) void ce_gemm_kernel(CeGemm g) {
 template <typename OT, bool PLANES>
 __global__ __launch_bounds__(256) void ce_reduce_kernel(const float* __restrict__ part, size_t out_split, int ld, int split, const float* __restrict__ f, const int* __restrict__ scal,
                                                         float* __restrict__ acc, void* __restrict__ out, int first, int last, int rows, int cols, long r0, int HW, int C) {
-  const float gi = ce_pow2(-ce_gexp(scal));
+  const float gi = ce_pow2(-scal[0]);
   const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (row >= rows) return;
   for (int c = blockIdx.y * 64 + lane; c < cols; c += gridDim.y * 64) {
@@ -453,7 +510,7 @@ struct CePlan {
   int pb, vb;                    // rows / classes of a piece
   int nparts;
   int split_x, split_w;
-  size_t o_x, o_w, o_fx, o_fw, o_b, o_lab, o_lse, o_zl, o_gp, o_part, o_scal, o_lsum, o_g, o_db, o_px, o_pw, o_ax, o_aw, total;
+  size_t o_x, o_w, o_fx, o_fw, o_b, o_lab, o_lse, o_zl, o_gp, o_part, o_scal, o_slots, o_rowmax, o_lsum, o_g, o_db, o_px, o_pw, o_ax, o_aw, total;
 };
 static size_t ce_al(size_t n) { return (n + 255) & ~(size_t)255; }
 static long ce_up(long a, long b) { return (a + b - 1) / b * b; }
@@ -475,7 +532,7 @@ static CePlan ce_plan(int N, int C, int V, int HW, int types, bool grad) {
   k.o_w = take((size_t)k.wp * k.Vp * k.Cp * 2);
   k.o_fx = take(k.Pp * 4); k.o_fw = take((size_t)k.Vp * 4); k.o_b = take((size_t)k.Vp * 4);
   k.o_lab = take(k.Pp * 4); k.o_lse = take(k.Pp * 4); k.o_zl = take(k.Pp * 4); k.o_gp = take(k.Pp * 4);
-  k.o_scal = take(64);
+  k.o_scal = take(64); k.o_slots = take(kCeSlots * 4); k.o_rowmax = take(kCeRowBlocks * 4);
   k.o_lsum = take((size_t)(k.Pp / 64) * 8);
   const size_t stats = (size_t)k.nparts * k.Pp * 8;
   if (!grad) { k.o_part = take(stats); k.total = o; return k; }
@@ -502,8 +559,19 @@ static int ce_check(int N, int C, int V, int HW, int types, const char* who) {
   return MS_OK;
 }
 
+// M, N: sizes in elements, multiples of the tile.  256 x 256 tiles (one workgroup a CU) where there are enough of them for the chip: half the LDS traffic a product.
+// G's kernel keeps 128 x 128: its epilogue is as long as its product at 512 channels, and only a second workgroup on the CU overlaps the two (381 against 428 us).
+static bool ce_big(int M, int N, int split) { return M % 256 == 0 && N % 256 == 0 && (long)(M / 256) * (N / 256) * split >= 200; }
 template <int EPI, bool ACOL, bool BCOL>
-static int ce_gemm(const CeGemm& g, hipStream_t st, const char* what) {
+static int ce_gemm(CeGemm g, int M, int N, hipStream_t st, const char* what) {
+  if constexpr (EPI == CE_STATS || EPI == CE_OUT) {
+    if (ce_big(M, N, g.split)) {
+      g.mt = M / 256; g.nt = N / 256;
+      MS_LAUNCH((ce_gemm_kernel<256, 256, 2, 4, ACOL, BCOL, EPI>), dim3(g.mt * g.nt * g.split), dim3(512), 0, st, g);
+      return check_launch(what);
+    }
+  }
+  g.mt = M / 128; g.nt = N / 128;
   MS_LAUNCH((ce_gemm_kernel<128, 128, 2, 2, ACOL, BCOL, EPI>), dim3(g.mt * g.nt * g.split), dim3(256), 0, st, g);
   return check_launch(what);
 }
@@ -525,19 +593,17 @@ static int ce_run(const CeArgs& a, const char* who) {
   auto f32 = [&](size_t o) { return (float*)(ws + o); };
   _Float16 *x = (_Float16*)(ws + k.o_x), *w = (_Float16*)(ws + k.o_w);
   const size_t xpl = (size_t)k.Pp * k.Cp, wpl = (size_t)k.Vp * k.Cp;
-  int *lab = (int*)(ws + k.o_lab), *scal = (int*)(ws + k.o_scal);
+  int *lab = (int*)(ws + k.o_lab), *scal = (int*)(ws + k.o_scal), *slots = (int*)(ws + k.o_slots), *rowmax = (int*)(ws + k.o_rowmax);
   float *fx = f32(k.o_fx), *fw = f32(k.o_fw), *bp = f32(k.o_b), *lse = f32(k.o_lse), *zl = f32(k.o_zl), *gp = f32(k.o_gp);
   hipStream_t st = a.st;
-  MS_LAUNCH(ce_init_kernel, dim3(1), dim3(64), 0, st, scal);
-  if (int e = check_launch("class_ce_init")) return e;
   auto pack_rows = [&](const void* src, bool bf, const float* b, const int64_t* labels, _Float16* out, size_t pl, float* f, float* bpad, int rows, int rows_pad) {
     const bool vec = a.C % 8 == 0 && aligned16(src);
     const dim3 grid(rows_pad / 4), block(256);
     const int drop = need_grad ? 1 : 0;
-    if (bf && vec) MS_LAUNCH((ce_pack_rows_kernel<ms_bf16, 1, true>), grid, block, 0, st, src, b, labels, a.V, drop, out, pl, f, bpad, lab, scal, rows, rows_pad, a.C, k.Cp);
-    else if (bf) MS_LAUNCH((ce_pack_rows_kernel<ms_bf16, 1, false>), grid, block, 0, st, src, b, labels, a.V, drop, out, pl, f, bpad, lab, scal, rows, rows_pad, a.C, k.Cp);
-    else if (vec) MS_LAUNCH((ce_pack_rows_kernel<float, 2, true>), grid, block, 0, st, src, b, labels, a.V, drop, out, pl, f, bpad, lab, scal, rows, rows_pad, a.C, k.Cp);
-    else MS_LAUNCH((ce_pack_rows_kernel<float, 2, false>), grid, block, 0, st, src, b, labels, a.V, drop, out, pl, f, bpad, lab, scal, rows, rows_pad, a.C, k.Cp);
+    if (bf && vec) MS_LAUNCH((ce_pack_rows_kernel<ms_bf16, 1, true>), grid, block, 0, st, src, b, labels, a.V, drop, out, pl, f, bpad, lab, rows, rows_pad, a.C, k.Cp);
+    else if (bf) MS_LAUNCH((ce_pack_rows_kernel<ms_bf16, 1, false>), grid, block, 0, st, src, b, labels, a.V, drop, out, pl, f, bpad, lab, rows, rows_pad, a.C, k.Cp);
+    else if (vec) MS_LAUNCH((ce_pack_rows_kernel<float, 2, true>), grid, block, 0, st, src, b, labels, a.V, drop, out, pl, f, bpad, lab, rows, rows_pad, a.C, k.Cp);
+    else MS_LAUNCH((ce_pack_rows_kernel<float, 2, false>), grid, block, 0, st, src, b, labels, a.V, drop, out, pl, f, bpad, lab, rows, rows_pad, a.C, k.Cp);
     return check_launch("class_ce_pack");
   };
   if (int e = pack_rows(a.w, (a.types & 2) != 0, a.b, nullptr, w, wpl, fw, bp, a.V, k.Vp)) return e;
@@ -549,8 +615,9 @@ static int ce_run(const CeArgs& a, const char* who) {
     else MS_LAUNCH((ce_pack_planes_kernel<float, 2>), gx, dim3(1024), 0, st, a.h, a.labels, a.V, need_grad ? 1 : 0, x, xpl, fx, lab, k.P, k.Pp, a.C, k.Cp, a.HW);
     if (int e = check_launch("class_ce_pack")) return e;
   }
+  const int nslots = (int)std::min<long>(kCeSlots, k.P / 1024 + 1);
   if (a.mean_valid) {
-    MS_LAUNCH(ce_count_kernel, dim3((unsigned)std::min<long>(cdiv((int)std::min<long>(k.P, 1 << 30), 1024), 1024)), dim3(256), 0, st, a.labels, k.P, a.V, scal);
+    MS_LAUNCH(ce_count_kernel, dim3(nslots), dim3(256), 0, st, a.labels, k.P, a.V, slots);
     if (int e = check_launch("class_ce_count")) return e;
   }
   CeGemm g{};
@@ -559,19 +626,23 @@ static int ce_run(const CeArgs& a, const char* who) {
     // logits -> statistics: M = classes, N = rows
     g.a = CeOperand{w, wpl, k.Cp, 0}; g.b = CeOperand{x, xpl, k.Cp, 0};
     ce_pairs(g, k.wp, k.xp);
-    g.ksteps = k.Cp / kCeBK; g.mt = k.Vp / 128; g.nt = (int)(k.Pp / 128); g.split = 1;
+    g.ksteps = k.Cp / kCeBK; g.split = 1;
     g.part = (float2*)(ws + k.o_part); g.part_stride = (size_t)k.Pp;
-    if (int e = ce_gemm<CE_STATS, false, false>(g, st, "class_ce_stats")) return e;
-    MS_LAUNCH(ce_join_kernel, dim3((unsigned)(k.Pp / 64)), dim3(1024), 0, st, (const float2*)g.part, k.nparts, g.part_stride, zl, lab, lse, a.lse, a.nll, (double*)(ws + k.o_lsum), k.P);
+    if (int e = ce_gemm<CE_STATS, false, false>(g, k.Vp, (int)k.Pp, st, "class_ce_stats")) return e;
+    MS_LAUNCH(ce_join_kernel, dim3((unsigned)(k.Pp / 64)), dim3(1024), 0, st, (const float2*)g.part, ce_big(k.Vp, (int)k.Pp, 1) ? k.nparts / 2 : k.nparts, g.part_stride, zl, lab, lse, a.lse, a.nll, (double*)(ws + k.o_lsum), k.P);
     if (int e = check_launch("class_ce_join")) return e;
-    if (a.loss != nullptr) {
-      MS_LAUNCH(ce_loss_kernel, dim3(1), dim3(256), 0, st, (const double*)(ws + k.o_lsum), (int)(k.Pp / 64), a.sign, a.mean_valid, scal, k.P, a.loss);
-      if (int e = check_launch("class_ce_loss")) return e;
-    }
+  }
+  const int nrow = (int)std::min<long>(k.Pp / 256, kCeRowBlocks);
+  if (need_grad) {
+    MS_LAUNCH(ce_rowgrad_kernel, dim3(nrow), dim3(256), 0, st, a.grad, a.sign, a.mean_valid, a.scale_dev, lab, fx, gp, a.lse_in, lse, slots, nslots, rowmax, k.P, k.Pp);
+    if (int e = check_launch("class_ce_rowgrad")) return e;
+  }
+  if (need_grad || a.loss != nullptr) {
+    MS_LAUNCH(ce_scalars_kernel, dim3(1), dim3(1024), 0, st, (const double*)(ws + k.o_lsum), (int)(k.Pp / 64), a.sign, a.mean_valid, slots, nslots, k.P, a.loss,
+              need_grad ? rowmax : (const int*)nullptr, nrow, fw, a.V, scal);
+    if (int e = check_launch("class_ce_scalars")) return e;
   }
   if (!need_grad) return MS_OK;
-  MS_LAUNCH(ce_rowgrad_kernel, dim3((unsigned)std::min<long>(k.Pp / 256, 1024)), dim3(256), 0, st, a.grad, a.sign, a.mean_valid, a.scale_dev, lab, fx, gp, a.lse_in, lse, scal, k.P, k.Pp);
-  if (int e = check_launch("class_ce_rowgrad")) return e;
   const long cp = ce_up(k.Cp, 128);
   for (long p0 = 0; p0 < k.Pp; p0 += k.pb) {
     const int pn = (int)std::min<long>(k.pb, k.Pp - p0);
@@ -580,13 +651,13 @@ static int ce_run(const CeArgs& a, const char* who) {
       CeGemm d = g;
       d.a = CeOperand{w + (size_t)v0 * k.Cp, wpl, k.Cp, 0}; d.b = CeOperand{x + (size_t)p0 * k.Cp, xpl, k.Cp, 0};
       ce_pairs(d, k.wp, k.xp);
-      d.ksteps = k.Cp / kCeBK; d.mt = vn / 128; d.nt = pn / 128; d.split = 1; d.v0 = v0; d.p0 = p0;
+      d.ksteps = k.Cp / kCeBK; d.split = 1; d.v0 = v0; d.p0 = p0;
       _Float16* G = (_Float16*)(ws + k.o_g);
       const size_t gpl = (size_t)k.pb * k.vb;
       d.g = G; d.g_plane = gpl; d.g_ld = k.vb;
       d.dbpart = a.db != nullptr ? f32(k.o_db) : nullptr; d.db_stride = k.vb;
-      if (k.gpl == 2) { if (int e = ce_gemm<CE_GRAD2, false, false>(d, st, "class_ce_grad")) return e; }
-      else { if (int e = ce_gemm<CE_GRAD, false, false>(d, st, "class_ce_grad")) return e; }
+      if (k.gpl == 2) { if (int e = ce_gemm<CE_GRAD2, false, false>(d, vn, pn, st, "class_ce_grad")) return e; }
+      else { if (int e = ce_gemm<CE_GRAD, false, false>(d, vn, pn, st, "class_ce_grad")) return e; }
       if (a.db != nullptr) {
         const int vr = std::min(vn, a.V - v0);
         if (vr > 0) {
@@ -604,14 +675,14 @@ static int ce_run(const CeArgs& a, const char* who) {
         const int rows = (int)std::min<long>(pn, k.P - p0), first = v0 == 0, last = v0 + vn >= k.Vp;
         float* ac = (a.types & 1) ? f32(k.o_ax) : (float*)a.dh;
         if (rows_form) {
-          o.a = og; o.b = ow; ce_pairs(o, pg, pw); o.mt = pn / 128; o.nt = (int)(cp / 128); o.out_ld = (int)cp;
-          if (int e = ce_gemm<CE_OUT, false, true>(o, st, "class_ce_dh")) return e;
+          o.a = og; o.b = ow; ce_pairs(o, pg, pw); o.out_ld = (int)cp;
+          if (int e = ce_gemm<CE_OUT, false, true>(o, pn, (int)cp, st, "class_ce_dh")) return e;
           const dim3 grid((unsigned)cdiv(rows, 4), (unsigned)std::min(cdiv(a.C, 64), 4));
           if (a.types & 1) MS_LAUNCH((ce_reduce_kernel<ms_bf16, false>), grid, dim3(256), 0, st, o.out, o.out_split, o.out_ld, o.split, fx, scal, ac, a.dh, first, last, rows, a.C, p0, 1, a.C);
           else MS_LAUNCH((ce_reduce_kernel<float, false>), grid, dim3(256), 0, st, o.out, o.out_split, o.out_ld, o.split, fx, scal, ac, a.dh, first, last, rows, a.C, p0, 1, a.C);
         } else {
-          o.a = ow; o.b = og; ce_pairs(o, pw, pg); o.mt = (int)(cp / 128); o.nt = pn / 128; o.out_ld = k.pb;
-          if (int e = ce_gemm<CE_OUT, true, false>(o, st, "class_ce_dh")) return e;
+          o.a = ow; o.b = og; ce_pairs(o, pw, pg); o.out_ld = k.pb;
+          if (int e = ce_gemm<CE_OUT, true, false>(o, (int)cp, pn, st, "class_ce_dh")) return e;
           const dim3 grid((unsigned)cdiv(a.C, 4), (unsigned)std::min(cdiv(rows, 64), 64));
           if (a.types & 1) MS_LAUNCH((ce_reduce_kernel<ms_bf16, true>), grid, dim3(256), 0, st, o.out, o.out_split, o.out_ld, o.split, fx, scal, ac, a.dh, first, last, a.C, rows, p0, a.HW, a.C);
           else MS_LAUNCH((ce_reduce_kernel<float, true>), grid, dim3(256), 0, st, o.out, o.out_split, o.out_ld, o.split, fx, scal, ac, a.dh, first, last, a.C, rows, p0, a.HW, a.C);
@@ -623,9 +694,9 @@ static int ce_run(const CeArgs& a, const char* who) {
         CeGemm o{};
         o.a = CeOperand{G, gpl, k.vb, k.vb}; o.b = CeOperand{x + (size_t)p0 * k.Cp, xpl, k.Cp, k.Cp};
         ce_pairs(o, (a.types & 2) ? 1 : 2, (a.types & 2) ? 1 : k.xp);
-        o.ksteps = pn / kCeBK; o.mt = vn / 128; o.nt = (int)(cp / 128); o.split = std::min(k.split_w, std::max(1, o.ksteps / 8));
+        o.ksteps = pn / kCeBK; o.split = std::min(k.split_w, std::max(1, o.ksteps / 8));
         o.out = f32(k.o_pw); o.out_ld = (int)cp; o.out_split = (size_t)k.vb * cp;
-        if (int e = ce_gemm<CE_OUT, true, true>(o, st, "class_ce_dw")) return e;
+        if (int e = ce_gemm<CE_OUT, true, true>(o, vn, (int)cp, st, "class_ce_dw")) return e;
         const int first = p0 == 0, last = p0 + pn >= k.Pp;
         const dim3 grid((unsigned)cdiv(vr, 4), (unsigned)std::min(cdiv(a.C, 64), 4));
         float* ac = (a.types & 2) ? f32(k.o_aw) : (float*)a.dw;

@@ -10,6 +10,7 @@
 // 8 P V C products, and nothing of size P V is stored.  The vector unit, not the matrix cores, sets the time: about 8 operations a logit in the pixel pass and 10 in
 // the class pass, and an exp2, which counts 4.
 #include <algorithm>
+#include <type_traits>
 #include "ms_class_ce.h"
 #include "ms_class_ce_narrow.h"
 #include "maxstyle_hip.h"
@@ -22,22 +23,33 @@ constexpr int kCnPrep = 256;          // most workgroups that count
 // Classes: 4 where the registers hold them and there are that many (one pixel tile then serves 256 classes: 1M pixels x 64, 256 classes: 301 -> 227 us), else 2.
 constexpr int kCnNJ = 2;
 
-// 16-byte chunk j of row r of a tile of KS * 32 columns lies at chunk j ^ cn_swz(r): both the row reads and the transposing reads below are then free of bank conflicts
-template <int KS> __device__ __forceinline__ int cn_swz(int r) { return KS == 1 ? (r >> 1) & 3 : (KS == 3 ? (r >> 2) & 3 : r & 7); }
+// Widths: KS steps of 32 channels; KS = 0 is 16 channels (the narrow networks' head) on the 16-deep matrix instruction, half the registers and loads of a padded step.
+template <int KS> struct CnW {
+  static constexpr int kW = KS == 0 ? 16 : KS * 32;              // channels of a packed row
+  static constexpr int kN = KS == 0 ? 1 : KS;                    // k-steps
+  static constexpr int kF = KS == 0 ? 4 : 8;                     // channels of a lane's fragment: ks * 32 + q * kF + k
+  static constexpr int kCT = kW / 16;
+  typedef typename std::conditional<KS == 0, ms_h4, ms_h8>::type Frag;
+};
+__device__ __forceinline__ ms_f4 cn_mfma(ms_h8 a, ms_h8 b, ms_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ ms_f4 cn_mfma(ms_h4 a, ms_h4 b, ms_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
+
+// 16-byte chunk j of row r of a tile of kW columns lies at chunk j ^ cn_swz(r): both the row reads and the transposing reads below are then free of bank conflicts
+template <int KS> __device__ __forceinline__ int cn_swz(int r) { return KS == 0 ? 0 : KS == 1 ? (r >> 1) & 3 : (KS == 3 ? (r >> 2) & 3 : r & 7); }
 template <int KS, int WP> struct CnImage {
-  static constexpr int kPlane = kCnClasses * KS * 32;                    // halves of one plane
+  static constexpr int kPlane = kCnClasses * CnW<KS>::kW;                    // halves of one plane
   static constexpr int kBytes = WP * kPlane * 2 + 1024;                  // + 64 x {b log2(e)}, 2^e log2(e), 2^e of the chunk
 };
 
-// transposing read: lane (q, i) gets column mn + i of rows k .. k + 3, k = k0 + 4 q (swizzled tile of KS * 32 columns)
+// transposing read: lane (q, i) gets column mn + i of rows k .. k + 3, k = k0 + 4 q (swizzled tile of kW columns)
 template <int KS>
 __device__ __forceinline__ ms_h8 cn_tr2(const _Float16* tile, int k0, int k1, int mn, int lane) {
   const int q = lane >> 4, i = lane & 15;
   typedef __attribute__((address_space(3))) ms_s4* lp;
   union { ms_s4 s[2]; ms_h8 h; } u;
   const int ra = k0 + q * 4 + (i >> 2), rb = k1 + q * 4 + (i >> 2), ch = (mn >> 3) + ((i & 3) >> 1), off = (i & 1) * 4;
-  u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(ms_s4*)(tile + ra * (KS * 32) + ((ch ^ cn_swz<KS>(ra)) * 8) + off));
-  u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(ms_s4*)(tile + rb * (KS * 32) + ((ch ^ cn_swz<KS>(rb)) * 8) + off));
+  u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(ms_s4*)(tile + ra * CnW<KS>::kW + ((ch ^ cn_swz<KS>(ra)) * 8) + off));
+  u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(ms_s4*)(tile + rb * CnW<KS>::kW + ((ch ^ cn_swz<KS>(rb)) * 8) + off));
   return u.h;
 }
 
@@ -52,12 +64,12 @@ __global__ __launch_bounds__(256) void cn_prep_kernel(const void* __restrict__ w
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   if ((int)blockIdx.x < nch) {
     const int v0 = blockIdx.x * 64;
-    constexpr int kPer = 64 * KS * 32 / 256;
+    constexpr int kW = CnW<KS>::kW, kPer = 64 * kW / 256;
     float x[kPer];
     unsigned am = 0;
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
-      const int i = k * 256 + threadIdx.x, r = i / (KS * 32), c = i % (KS * 32);
+      const int i = k * 256 + threadIdx.x, r = i / kW, c = i % kW;
       x[k] = (v0 + r < V && c < C) ? IO::ld1(w, (size_t)(v0 + r) * C + c) : 0.f;
       const unsigned bits = __float_as_uint(x[k]) & 0x7FFFFFFFu;
       am = max(am, bits < 0x7F800000u ? bits : 0u);          // (an infinity or NaN spoils its own class only)
@@ -74,10 +86,10 @@ __global__ __launch_bounds__(256) void cn_prep_kernel(const void* __restrict__ w
     _Float16* pl = (_Float16*)im;
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
-      const int i = k * 256 + threadIdx.x, r = i / (KS * 32), c = i % (KS * 32);
+      const int i = k * 256 + threadIdx.x, r = i / kW, c = i % kW;
       _Float16 hi, lo;
       ce_split(x[k] * inv, hi, lo);
-      const int at = r * (KS * 32) + (((c >> 3) ^ cn_swz<KS>(r)) * 8) + (c & 7);
+      const int at = r * kW + (((c >> 3) ^ cn_swz<KS>(r)) * 8) + (c & 7);
       pl[at] = hi;
       if (WP == 2) pl[IM::kPlane + at] = lo;
     }
@@ -127,7 +139,8 @@ constexpr float kCnSlack = 6.f, kCnTop = 9.f;
 template <typename HT, typename WT, int KS, int NJ, bool DH>
 __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
   using IO = ActIO<HT>;
-  constexpr int HP = sizeof(HT) == 4 ? 2 : 1, WP = sizeof(WT) == 4 ? 2 : 1, CT = KS * 2;
+  constexpr int HP = sizeof(HT) == 4 ? 2 : 1, WP = sizeof(WT) == 4 ? 2 : 1, CT = CnW<KS>::kCT, KN = CnW<KS>::kN, KF = CnW<KS>::kF, kW = CnW<KS>::kW;
+  typedef typename CnW<KS>::Frag Frag;
   using IM = CnImage<KS, WP>;
   __shared__ __attribute__((aligned(1024))) char sm[2][IM::kBytes];
   __shared__ int redi[4];
@@ -139,13 +152,13 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
   if (nch > 0) cn_stage<WP, KS>(a.img, 0, lds0, wave, lane);
 
   // ---- this wave's pixels: scaled fp16 planes in the layout of a matrix operand (column = pixel li, 8 channels 32 ks + 8 q + k)
-  ms_h8 x[HP][KS][NJ];
+  Frag x[HP][KN][NJ];
   float fx[NJ];
   int lab[NJ];
   const int pw = (int)blockIdx.x * (4 * NJ * 16) + wave * (NJ * 16) + li;      // (at most 2^30 rows)
   const int P = (int)a.P;
   // every load unconditional, at a clamped address, and all of them in flight together (loads behind branches wait for one another: 20 us more at 400k pixels x 64 channels)
-  float v[NJ][KS][8];
+  float v[NJ][KN][KF];
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
     const int p = min(pw + j * 16, P - 1), n = p / a.HW;
@@ -153,19 +166,19 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
     const int64_t lb = a.labels[p];
     lab[j] = (lb >= 0 && lb < a.V && pw + j * 16 < P) ? (int)lb : -1;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
+    for (int ks = 0; ks < KN; ++ks)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[j][ks][k] = IO::ld1(a.h, base + (size_t)min(ks * 32 + q * 8 + k, a.C - 1) * a.HW);
+      for (int k = 0; k < KF; ++k) v[j][ks][k] = IO::ld1(a.h, base + (size_t)min(ks * 32 + q * KF + k, a.C - 1) * a.HW);
   }
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
     const bool live = pw + j * 16 < P && (!a.drop || lab[j] >= 0);
     unsigned am = 0;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
+    for (int ks = 0; ks < KN; ++ks)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (!live || ks * 32 + q * 8 + k >= a.C) v[j][ks][k] = 0.f;
+      for (int k = 0; k < KF; ++k) {
+        if (!live || ks * 32 + q * KF + k >= a.C) v[j][ks][k] = 0.f;
         am = max(am, __float_as_uint(v[j][ks][k]) & 0x7FFFFFFFu);
       }
     am = max(am, (unsigned)__shfl_xor((int)am, 16, 64));
@@ -174,9 +187,9 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
     const float inv = ce_pow2(-e);
     fx[j] = ce_pow2(e);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
+    for (int ks = 0; ks < KN; ++ks)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < KF; ++k) {
         _Float16 hi, lo;
         ce_split(v[j][ks][k] * inv, hi, lo);
         x[0][ks][j][k] = hi;
@@ -226,19 +239,19 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
         for (int j = 0; j < NJ; ++j) s[tt][j] = ms_f4{0.f, 0.f, 0.f, 0.f};
         const int r = h2 * 32 + tt * 16 + li;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const int at = r * (KS * 32) + (((ks * 4 + q) ^ cn_swz<KS>(r)) * 8);
-          const ms_h8 hi = *reinterpret_cast<const ms_h8*>(wp + at);
+        for (int ks = 0; ks < KN; ++ks) {
+          const int at = r * kW + (KS == 0 ? q * 4 : ((ks * 4 + q) ^ cn_swz<KS>(r)) * 8);
+          const Frag hi = *reinterpret_cast<const Frag*>(wp + at);
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) s[tt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, x[0][ks][j], s[tt][j], 0, 0, 0);
+          for (int j = 0; j < NJ; ++j) s[tt][j] = cn_mfma(hi, x[0][ks][j], s[tt][j]);
           if (HP == 2) {
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) s[tt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, x[HP - 1][ks][j], s[tt][j], 0, 0, 0);
+            for (int j = 0; j < NJ; ++j) s[tt][j] = cn_mfma(hi, x[HP - 1][ks][j], s[tt][j]);
           }
           if (WP == 2) {
-            const ms_h8 lo = *reinterpret_cast<const ms_h8*>(wp + IM::kPlane + at);
+            const Frag lo = *reinterpret_cast<const Frag*>(wp + IM::kPlane + at);
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) s[tt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, x[0][ks][j], s[tt][j], 0, 0, 0);
+            for (int j = 0; j < NJ; ++j) s[tt][j] = cn_mfma(lo, x[0][ks][j], s[tt][j]);
           }
         }
       }
@@ -400,9 +413,10 @@ struct CnwArgs {
 template <typename HT, typename WT, int KS, int NJ, int TP, bool VEC>
 __global__ __launch_bounds__(256, 2) void cn_classes_kernel(CnwArgs a) {
   using IO = ActIO<HT>;
+  typedef typename CnW<KS>::Frag Frag;
   constexpr int HP = sizeof(HT) == 4 ? 2 : 1, WP = sizeof(WT) == 4 ? 2 : 1;
   using IM = CnImage<KS, WP>;
-  constexpr int CT = KS * 2, kC = KS * 32, kTasks = kC * (TP / 8) / 256;
+  constexpr int CT = CnW<KS>::kCT, KN = CnW<KS>::kN, KF = CnW<KS>::kF, kC = CnW<KS>::kW, kTasks = kC * (TP / 8) / 256;
   __shared__ __attribute__((aligned(1024))) _Float16 xs[HP * kC * TP];
   __shared__ __attribute__((aligned(16))) float rows[4][TP];       // 2^ex, lse, g_p 2^ex, g_p
   __shared__ __attribute__((aligned(16))) int labs[TP];
@@ -412,7 +426,7 @@ __global__ __launch_bounds__(256, 2) void cn_classes_kernel(CnwArgs a) {
   const bool busy = unit < a.units;
   const int v0 = unit * (NJ * 16);
   // this wave's classes
-  ms_h8 w[WP][KS][NJ];
+  Frag w[WP][KN][NJ];
   float bw[NJ], db[NJ];
   const float wl2 = busy ? ((const float*)(a.img + (size_t)(v0 >> 6) * IM::kBytes + WP * IM::kPlane * 2))[64] : 0.f;      // (the classes of a wave lie in one chunk)
   ms_f4 o[CT][NJ];
@@ -425,7 +439,7 @@ __global__ __launch_bounds__(256, 2) void cn_classes_kernel(CnwArgs a) {
 #pragma unroll
     for (int pl = 0; pl < WP; ++pl)
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) w[pl][ks][j] = *reinterpret_cast<const ms_h8*>((const _Float16*)im + pl * IM::kPlane + r * kC + (((ks * 4 + q) ^ cn_swz<KS>(r)) * 8));
+      for (int ks = 0; ks < KN; ++ks) w[pl][ks][j] = *reinterpret_cast<const Frag*>((const _Float16*)im + pl * IM::kPlane + r * kC + (KS == 0 ? q * 4 : ((ks * 4 + q) ^ cn_swz<KS>(r)) * 8));
 #pragma unroll
     for (int c = 0; c < CT; ++c) o[c][j] = ms_f4{0.f, 0.f, 0.f, 0.f};
   }
@@ -518,21 +532,21 @@ __global__ __launch_bounds__(256, 2) void cn_classes_kernel(CnwArgs a) {
 #pragma unroll
           for (int j = 0; j < NJ; ++j) s[tt][j] = ms_f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks)
+          for (int ks = 0; ks < KN; ++ks)
 #pragma unroll
             for (int pl = 0; pl < HP; ++pl) {
-              // rows of the operand = pixels, 8 channels 32 ks + 8 q + k: transposing reads of rows 4 at a time
+              // rows of the operand = pixels, channels 32 ks + KF q + k: transposing reads of 4 channel rows at a time
               typedef __attribute__((address_space(3))) ms_s4* lp;
-              union { ms_s4 s[2]; ms_h8 h; } u;
-              const int c = ks * 32 + q * 8 + (li >> 2), chn = ((p0 + tt * 16) >> 3) + ((li & 3) >> 1), off = (li & 1) * 4;
+              union { ms_s4 s[KF / 4]; Frag h; } u;
+              const int c = ks * 32 + q * KF + (li >> 2), chn = ((p0 + tt * 16) >> 3) + ((li & 3) >> 1), off = (li & 1) * 4;
               const _Float16* b = xs + pl * kC * TP;
               u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(ms_s4*)(b + c * TP + ((chn ^ (c & 7)) * 8) + off));
-              u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(ms_s4*)(b + (c + 4) * TP + ((chn ^ ((c + 4) & 7)) * 8) + off));
+              if constexpr (KS > 0) u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(ms_s4*)(b + (c + 4) * TP + ((chn ^ ((c + 4) & 7)) * 8) + off));
 #pragma unroll
-              for (int j = 0; j < NJ; ++j) s[tt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(u.h, w[0][ks][j], s[tt][j], 0, 0, 0);
+              for (int j = 0; j < NJ; ++j) s[tt][j] = cn_mfma(u.h, w[0][ks][j], s[tt][j]);
               if (WP == 2 && pl == 0) {
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) s[tt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(u.h, w[WP - 1][ks][j], s[tt][j], 0, 0, 0);
+                for (int j = 0; j < NJ; ++j) s[tt][j] = cn_mfma(u.h, w[WP - 1][ks][j], s[tt][j]);
               }
             }
         }
@@ -663,7 +677,8 @@ struct CnPlan {
 };
 static CnPlan cn_plan(int N, int C, int V, int HW, int types, bool grad) {
   CnPlan k{};
-  k.KS = cdiv(C, 32); k.nch = cdiv(V, 64); k.Vp = k.nch * 64; k.P = (long)N * HW;
+  k.KS = C <= 16 ? 0 : cdiv(C, 32);
+  const int kW = k.KS == 0 ? 16 : k.KS * 32; k.nch = cdiv(V, 64); k.Vp = k.nch * 64; k.P = (long)N * HW;
   k.wgs = (k.P + kCnNJ * 64 - 1) / (kCnNJ * 64);
   k.Pp = (k.P + 255) / 256 * 256;
   k.nslots = (int)std::min<long>(kCnPrep, k.P / 1024 + 1);
@@ -677,11 +692,11 @@ static CnPlan cn_plan(int N, int C, int V, int HW, int types, bool grad) {
   k.splits = (int)std::max<long>(1, std::min<long>(k.tiles, 512 / std::min(k.vblocks, 512)));
   size_t o = 0;
   auto take = [&](size_t n) { const size_t at = o; o += (n + 255) & ~(size_t)255; return at; };
-  k.o_img = take((size_t)k.nch * ((size_t)((types & 2) ? 1 : 2) * 64 * k.KS * 64 + 1024));
+  k.o_img = take((size_t)k.nch * ((size_t)((types & 2) ? 1 : 2) * 64 * kW * 2 + 1024));
   k.o_slots = take(kCnPrep * 4); k.o_lsum = take((size_t)k.wgs * 8);
   if (grad) {
     k.o_fx = take(k.Pp * 4); k.o_lse = take(k.Pp * 4); k.o_gp = take(k.Pp * 4); k.o_lab = take(k.Pp * 4);
-    k.o_dw = take((size_t)k.splits * k.wpx * k.Vp * k.KS * 32 * 4);
+    k.o_dw = take((size_t)k.splits * k.wpx * k.Vp * kW * 4);
     k.o_db = take((size_t)k.splits * k.wpx * k.Vp * 4);
   }
   k.total = o;
@@ -697,7 +712,7 @@ size_t ce_narrow_ws_bytes(int N, int C, int V, int HW, int types, bool grad) { r
 
 template <typename HT, typename WT, int KS>
 static int cn_run(const CeArgs& a, const CnPlan& k) {
-  constexpr int WP = sizeof(WT) == 4 ? 2 : 1;
+  constexpr int WP = sizeof(WT) == 4 ? 2 : 1, kW = CnW<KS>::kW;
   const bool need_dw = a.dw != nullptr || a.db != nullptr, need_grad = need_dw || a.dh != nullptr;
   char* ws = (char*)a.ws;
   hipStream_t st = a.st;
@@ -718,7 +733,7 @@ static int cn_run(const CeArgs& a, const CnPlan& k) {
   if (need_dw) {
     CnwArgs c{};
     c.h = a.h; c.img = p.img; c.fx = p.fx; c.lse2 = p.lse2; c.gp = p.gp; c.lab = p.lab;
-    c.dwp = (float*)(ws + k.o_dw); c.dbp = (float*)(ws + k.o_db); c.dw_split = (size_t)k.Vp * KS * 32; c.db_split = k.Vp;
+    c.dwp = (float*)(ws + k.o_dw); c.dbp = (float*)(ws + k.o_db); c.dw_split = (size_t)k.Vp * kW; c.db_split = k.Vp;
     c.P = k.P; c.C = a.C; c.HW = a.HW; c.V = a.V; c.units = k.units; c.wpx = k.wpx; c.splits = k.splits; c.tiles = k.tiles;
     const dim3 gw((unsigned)k.splits, (unsigned)k.vblocks);
     const bool vec = a.HW % 8 == 0 && aligned16(a.h);          // 8-pixel groups that never cross an image, in whole vectors
@@ -732,10 +747,10 @@ static int cn_run(const CeArgs& a, const CnPlan& k) {
     if (int e = check_launch("class_ce_classes")) return e;
   }
   if (need_dw || a.loss != nullptr) {
-    const int wb = a.dw != nullptr ? cdiv(a.V * KS * 32, 64) : 0;
+    const int wb = a.dw != nullptr ? cdiv(a.V * kW, 64) : 0;
     const unsigned blocks = (unsigned)(wb + (a.db != nullptr ? cdiv(a.V, 64) : 0) + (a.loss != nullptr ? 1 : 0));
-    MS_LAUNCH((cn_join_kernel<WT>), dim3(blocks), dim3(1024), 0, st, (const float*)(ws + k.o_dw), (const float*)(ws + k.o_db), (size_t)k.Vp * KS * 32, k.Vp, k.splits * k.wpx, a.dw, a.db,
-              a.V, a.C, KS * 32, wb, p.lsum, (int)k.wgs, slots, k.nslots, a.sign, a.mean_valid, k.P, a.loss);
+    MS_LAUNCH((cn_join_kernel<WT>), dim3(blocks), dim3(1024), 0, st, (const float*)(ws + k.o_dw), (const float*)(ws + k.o_db), (size_t)k.Vp * kW, k.Vp, k.splits * k.wpx, a.dw, a.db,
+              a.V, a.C, kW, wb, p.lsum, (int)k.wgs, slots, k.nslots, a.sign, a.mean_valid, k.P, a.loss);
     if (int e = check_launch("class_ce_join")) return e;
   }
   return MS_OK;
@@ -743,6 +758,7 @@ static int cn_run(const CeArgs& a, const CnPlan& k) {
 template <typename HT, typename WT>
 static int cn_dispatch(const CeArgs& a, const CnPlan& k) {
   switch (k.KS) {
+    case 0: return cn_run<HT, WT, 0>(a, k);
     case 1: return cn_run<HT, WT, 1>(a, k);
     case 2: return cn_run<HT, WT, 2>(a, k);
     case 3: return cn_run<HT, WT, 3>(a, k);

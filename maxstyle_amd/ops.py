@@ -17,6 +17,24 @@ def _stream():
     return torch.cuda.current_stream().cuda_stream
 
 
+class _Here:
+    """The no-op in place of torch.cuda.device(..) where that device is already current (3 us of host time a call)."""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def _on(device):
+    """Context that makes `device` current: launches go to torch's current stream on the device the tensors live on."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
 def _ptr(t):
     if t is None:
         return 0
@@ -462,7 +480,7 @@ def class_ce(h, w, b, labels, loss_sign=1.0, mean_over="all", need_dh=True, need
         _need_cuda_f32(grad_scale)
         if grad_scale.numel() != 1 or grad_scale.device != h.device:
             raise ValueError("class_ce: grad_scale is one fp32 value on the device of h")
-    with torch.cuda.device(h.device):
+    with _on(h.device):
         loss = torch.empty((), device=h.device, dtype=torch.float32)
         dh = torch.empty_like(h) if need_dh else None
         dw = torch.empty_like(w) if need_dw else None
@@ -477,7 +495,7 @@ def class_ce_fwd(h, w, b, labels):
     """Cross entropy of every row and the log-sum of its exponentials, (nll, lse) [N,*spatial] fp32 (ms_class_ce_fwd); arguments as class_ce.  nll is 0 where the label
     is not a class."""
     N, C, V, HW, types = _class_ce_args(h, w, b, labels)
-    with torch.cuda.device(h.device):
+    with _on(h.device):
         nll = torch.empty(labels.shape, device=h.device, dtype=torch.float32)
         lse = torch.empty_like(nll)
         ws = _class_ce_ws(N, C, V, HW, types, False, h.device)
@@ -495,7 +513,7 @@ def class_ce_bwd(h, w, b, labels, lse, grad, need_dh=True, need_dw=True):
             raise ValueError("class_ce_bwd: lse and grad have the shape and the device of labels")
     if not (need_dh or need_dw):
         return None, None, None
-    with torch.cuda.device(h.device):
+    with _on(h.device):
         dh = torch.empty_like(h) if need_dh else None
         dw = torch.empty_like(w) if need_dw else None
         db = torch.empty_like(b) if (need_dw and b is not None) else None
@@ -551,10 +569,11 @@ def act8_pack(x, coef4=None, q=None, s=None):
     bf = _need_cuda_act(x)
     N, C, HW = _act8_dims(x.shape, "act8_pack")
     _act8_coef(coef4, C, x.device, "act8_pack")
-    with torch.cuda.device(x.device):
+    with _on(x.device):
+        given = q is not None or s is not None
         q = torch.empty(x.shape, dtype=torch.int8, device=x.device) if q is None else q
         s = torch.empty(N, C, (HW + ACT8_BLOCK - 1) // ACT8_BLOCK, dtype=torch.float32, device=x.device) if s is None else s
-        if _act8_kept(q, s, "act8_pack") != (N, C, HW) or q.device != x.device:
+        if given and (_act8_kept(q, s, "act8_pack") != (N, C, HW) or q.shape != x.shape or q.device != x.device):
             raise ValueError("act8_pack: q must have the shape and the device of x")
         check(_fn("ms_act8_pack", bf)(x.data_ptr(), _ptr(coef4), q.data_ptr(), s.data_ptr(), N, C, HW, _stream()), "ms_act8_pack")
     return q, s
@@ -564,7 +583,7 @@ def act8_unpack(q, s, coef4=None, dtype=torch.float32, out=None):
     """The activation that a checkpoint of act8_pack stands for, in fp32 or bf16; coef4: the record it was made with (ms_act8_unpack)."""
     N, C, HW = _act8_kept(q, s, "act8_unpack")
     _act8_coef(coef4, C, q.device, "act8_unpack")
-    with torch.cuda.device(q.device):
+    with _on(q.device):
         out = torch.empty(q.shape, dtype=dtype, device=q.device) if out is None else out
         bf = _need_cuda_act(out)
         if out.shape != q.shape or out.device != q.device:
@@ -593,7 +612,7 @@ def act8_bwd_reduce(gin, q, s, coef4, slope, ref_q=None, gout=None, uout=None, p
     uout: a tensor that receives the kept activation on the way."""
     bf, N, C, HW = _act8_bwd_args(gin, q, s, coef4, slope, ref_q, "act8_bwd_reduce")
     _need_cuda_f32(part)
-    with torch.cuda.device(gin.device):
+    with _on(gin.device):
         nparts = lib.ms_act8_bwd_parts(N, C, HW)
         gout = torch.empty_like(gin) if gout is None else gout
         part = torch.empty(C, nparts, 2, device=gin.device, dtype=torch.float32) if part is None else part
@@ -612,7 +631,7 @@ def act8_bn_act_bwd(g, q, s, coef4, slope, ref_q=None, out=None):
     g: gradient of the activation's output, fp32 or bf16; coef4: the bn_finalize record the checkpoint was made with; ref_q: the int8 part of the checkpoint of the saved
     activation output where something was added in front of the activation (a residual block's tail) - without it the mask comes from the checkpoint itself."""
     bf, N, C, HW = _act8_bwd_args(g, q, s, coef4, slope, ref_q, "act8_bn_act_bwd")
-    with torch.cuda.device(g.device):
+    with _on(g.device):
         out = torch.empty_like(g) if out is None else out
         if out.shape != g.shape or out.dtype != g.dtype or not out.is_contiguous() or out.device != g.device:
             raise ValueError("act8_bn_act_bwd: out is contiguous and like g")
