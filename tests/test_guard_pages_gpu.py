@@ -36,6 +36,7 @@ def _env(mode):
     return env
 
 
+@pytest.mark.skip(reason="makes the GPU fault on purpose: a machine that counts such a fault as a failure of the card ends with it")
 def test_a_read_past_a_guarded_tensor_is_fatal():
     """Positive control: the guard works on this box.  ms_bn_finalize is handed a gamma vector of 16 values and told it holds 4112: the read of gamma[16] leaves the
     block, the process dies with a GPU memory fault (without the guard the same call reads whatever follows and returns)."""
