@@ -267,12 +267,17 @@ static int a8_check(int N, int C, int HW, const char* who) {
   if ((long long)N * C * cdiv(HW, 1024) >= (1LL << 31) - 8 || HW > 0x7FFFFFFF - 32768) { set_error("%s: more than 2^31 segments of 1024 elements", who); return MS_ERR_INVALID; }
   return MS_OK;
 }
+static int a8_aligned(const float* coef4, const void* part, const char* who) {
+  if (!aligned16(coef4) || (reinterpret_cast<uintptr_t>(part) & 7u)) { set_error("%s: coef4 must be 16-byte aligned, partial sums 8-byte", who); return MS_ERR_ALIGN; }
+  return MS_OK;
+}
 static bool a8_al(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 template <typename AT>
 static int act8_pack_impl(const void* x, const float* coef4, int8_t* q, float* s, int N, int C, int HW, void* stream) {
   if (int e = a8_check(N, C, HW, "ms_act8_pack")) return e;
   if (x == nullptr || q == nullptr || s == nullptr) { set_error("ms_act8_pack: null pointer"); return MS_ERR_INVALID; }
+  if (int e = a8_aligned(coef4, nullptr, "ms_act8_pack")) return e;
   const int nb = cdiv(HW, kA8Block), items = cdiv(nb, kPackBlocks), total = N * C * items;
   const bool vec = HW % 4 == 0 && a8_al(x, 4 * ActIO<AT>::kBytes) && a8_al(q, 4);      // rows of whole 4-element words; otherwise element by element
   dim3 grid(cdiv(total, kA8Threads / 64)), block(kA8Threads);
@@ -284,6 +289,7 @@ template <typename AT>
 static int act8_unpack_impl(const int8_t* q, const float* s, const float* coef4, void* x, int N, int C, int HW, void* stream) {
   if (int e = a8_check(N, C, HW, "ms_act8_unpack")) return e;
   if (x == nullptr || q == nullptr || s == nullptr) { set_error("ms_act8_unpack: null pointer"); return MS_ERR_INVALID; }
+  if (int e = a8_aligned(coef4, nullptr, "ms_act8_unpack")) return e;
   const int nb = cdiv(HW, kA8Block), items = cdiv(nb, kPackBlocks), total = N * C * items;
   const bool vec = HW % 4 == 0 && a8_al(x, 4 * ActIO<AT>::kBytes) && a8_al(q, 4);
   dim3 grid(cdiv(total, kA8Threads / 64)), block(kA8Threads);
@@ -302,6 +308,7 @@ static int act8_bwd_reduce_impl(const void* gin, const int8_t* ref, const int8_t
                                 int N, int C, int HW, float slope, void* stream) {
   if (int e = a8_check(N, C, HW, "ms_act8_bwd_reduce")) return e;
   if (gin == nullptr || q == nullptr || s == nullptr || coef4 == nullptr || part2 == nullptr) { set_error("ms_act8_bwd_reduce: null pointer"); return MS_ERR_INVALID; }
+  if (int e = a8_aligned(coef4, part2, "ms_act8_bwd_reduce")) return e;
   const A8Split sp = a8_split((long)N * C, HW);
   dim3 grid(N * C * sp.S), block(kA8Threads);
   const int nb = cdiv(HW, kA8Block);
@@ -321,6 +328,7 @@ static int act8_bn_act_bwd_impl(const void* g, const int8_t* ref, const int8_t* 
     set_error("ms_act8_bn_act_bwd: null pointer"); return MS_ERR_INVALID;
   }
   if (ws == nullptr || ws_bytes < ms_act8_bwd_ws_bytes(N, C, HW)) { set_error("ms_act8_bn_act_bwd: workspace too small"); return MS_ERR_WORKSPACE; }
+  if (int e = a8_aligned(coef4, ws, "ms_act8_bn_act_bwd")) return e;
   const A8Split sp = a8_split((long)N * C, HW);
   const int nb = cdiv(HW, kA8Block);
   hipStream_t st = (hipStream_t)stream;

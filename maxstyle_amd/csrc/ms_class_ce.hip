@@ -13,7 +13,7 @@
 
 namespace ms {
 
-constexpr size_t kCePieceBytes = (size_t)128 << 20;
+constexpr size_t kCePieceBytes = (size_t)128 << 20, kCeStatsBytes = (size_t)256 << 20;
 
 // ------------------------------------------------------------------------------------------------------------------------------ small passes
 // Rows [rows][C] -> planes [rows_pad][Cp] and each row's 2^e.  One wave a row; 8 channels a lane where the rows are made of whole vectors.
@@ -190,13 +190,13 @@ __device__ __forceinline__ void ce_merge(float& m, float& l, float mo, float lo)
   m = mn;
 }
 __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict__ part, int nparts, size_t stride, const float* __restrict__ zlab, const int* __restrict__ lab32,
-                                                       float* __restrict__ lse2, float* __restrict__ lse_out, float* __restrict__ nll_out, double* __restrict__ lsum, long P) {
+                                                       float* __restrict__ lse2, float* __restrict__ lse_out, float* __restrict__ nll_out, double* __restrict__ lsum, long p0, long P) {
   __shared__ float2 sh[16][64];
   const int el = threadIdx.x & 63, grp = threadIdx.x >> 6;
-  const long p = (long)blockIdx.x * 64 + el;          // (padded)
+  const long pr = (long)blockIdx.x * 64 + el, p = p0 + pr;          // (padded)
   float m = -__builtin_inff(), l = 0.f;
 #pragma unroll 4
-  for (int t = grp; t < nparts; t += 16) { const float2 o = part[(size_t)t * stride + p]; ce_merge(m, l, o.x, o.y); }
+  for (int t = grp; t < nparts; t += 16) { const float2 o = part[(size_t)t * stride + pr]; ce_merge(m, l, o.x, o.y); }
   sh[grp][el] = make_float2(m, l);
   __syncthreads();
   if (grp != 0) return;
@@ -211,7 +211,7 @@ __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict_
     acc = (double)v;
   }
   acc = wave_sum_d(acc);
-  if (el == 0) lsum[blockIdx.x] = acc;
+  if (el == 0) lsum[p0 / 64 + blockIdx.x] = acc;
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------ matrix products
@@ -389,7 +389,7 @@ __global__ __launch_bounds__(WM * WN * 64) void ce_gemm_kernel(CeGemm g) {
         for (int r = 0; r < 4; ++r) l += __builtin_amdgcn_exp2f(acc[i][j][r] - mm);
       l += __shfl_xor(l, 16, 64);
       l += __shfl_xor(l, 32, 64);
-      if (q == 0) g.part[(size_t)(mt * WM + wm) * g.part_stride + p] = make_float2(mx, l);
+      if (q == 0) g.part[(size_t)(mt * WM + wm) * g.part_stride + (p - (size_t)g.p0)] = make_float2(mx, l);
     }
     return;
   }
@@ -508,7 +508,7 @@ struct CePlan {
   long P, Pp; int Vp, Cp, HW;
   int xp, wp, gpl;               // planes of h, w, G
   int pb, vb;                    // rows / classes of a piece
-  int nparts;
+  int nparts, sb;                // partial statistics of a row, rows whose statistics are formed at a time
   int split_x, split_w;
   size_t o_x, o_w, o_fx, o_fw, o_b, o_lab, o_lse, o_zl, o_gp, o_part, o_scal, o_slots, o_rowmax, o_lsum, o_g, o_db, o_px, o_pw, o_ax, o_aw, total;
 };
@@ -526,6 +526,7 @@ static CePlan ce_plan(int N, int C, int V, int HW, int types, bool grad) {
   k.vb = (int)even(k.Vp, 8192);
   k.pb = (int)even(k.Pp, std::max<long>(kCePad, (long)(kCePieceBytes / ((size_t)k.vb * 2 * k.gpl)) / kCePad * kCePad));
   k.nparts = k.Vp / 128 * 2;
+  k.sb = (int)even(k.Pp, std::max<long>(kCePad, (long)(kCeStatsBytes / ((size_t)k.nparts * 8)) / kCePad * kCePad));
   size_t o = 0;
   auto take = [&](size_t n) { const size_t at = o; o += ce_al(n); return at; };
   k.o_x = take((size_t)k.xp * k.Pp * k.Cp * 2);
@@ -534,7 +535,7 @@ static CePlan ce_plan(int N, int C, int V, int HW, int types, bool grad) {
   k.o_lab = take(k.Pp * 4); k.o_lse = take(k.Pp * 4); k.o_zl = take(k.Pp * 4); k.o_gp = take(k.Pp * 4);
   k.o_scal = take(64); k.o_slots = take(kCeSlots * 4); k.o_rowmax = take(kCeRowBlocks * 4);
   k.o_lsum = take((size_t)(k.Pp / 64) * 8);
-  const size_t stats = (size_t)k.nparts * k.Pp * 8;
+  const size_t stats = (size_t)k.nparts * k.sb * 8;
   if (!grad) { k.o_part = take(stats); k.total = o; return k; }
   // The statistics are read before the first piece of G is written: they share its memory.
   k.o_part = o;
@@ -624,13 +625,18 @@ static int ce_run(const CeArgs& a, const char* who) {
   g.fw = fw; g.bpad = bp; g.fx = fx; g.lab = lab; g.lse = lse; g.gp = gp; g.scal = scal; g.zlab = zl;
   if (a.lse_in == nullptr) {
     // logits -> statistics: M = classes, N = rows
-    g.a = CeOperand{w, wpl, k.Cp, 0}; g.b = CeOperand{x, xpl, k.Cp, 0};
-    ce_pairs(g, k.wp, k.xp);
-    g.ksteps = k.Cp / kCeBK; g.split = 1;
-    g.part = (float2*)(ws + k.o_part); g.part_stride = (size_t)k.Pp;
-    if (int e = ce_gemm<CE_STATS, false, false>(g, k.Vp, (int)k.Pp, st, "class_ce_stats")) return e;
-    MS_LAUNCH(ce_join_kernel, dim3((unsigned)(k.Pp / 64)), dim3(1024), 0, st, (const float2*)g.part, ce_big(k.Vp, (int)k.Pp, 1) ? k.nparts / 2 : k.nparts, g.part_stride, zl, lab, lse, a.lse, a.nll, (double*)(ws + k.o_lsum), k.P);
-    if (int e = check_launch("class_ce_join")) return e;
+    for (long p0 = 0; p0 < k.Pp; p0 += k.sb) {
+      const int pn = (int)std::min<long>(k.sb, k.Pp - p0);
+      CeGemm d = g;
+      d.a = CeOperand{w, wpl, k.Cp, 0}; d.b = CeOperand{x + (size_t)p0 * k.Cp, xpl, k.Cp, 0};
+      ce_pairs(d, k.wp, k.xp);
+      d.ksteps = k.Cp / kCeBK; d.split = 1; d.v0 = 0; d.p0 = p0;
+      d.part = (float2*)(ws + k.o_part); d.part_stride = (size_t)k.sb;
+      if (int e = ce_gemm<CE_STATS, false, false>(d, k.Vp, pn, st, "class_ce_stats")) return e;
+      MS_LAUNCH(ce_join_kernel, dim3((unsigned)(pn / 64)), dim3(1024), 0, st, (const float2*)d.part, ce_big(k.Vp, pn, 1) ? k.nparts / 2 : k.nparts, d.part_stride, zl, lab, lse, a.lse, a.nll,
+                (double*)(ws + k.o_lsum), p0, k.P);
+      if (int e = check_launch("class_ce_join")) return e;
+    }
   }
   const int nrow = (int)std::min<long>(k.Pp / 256, kCeRowBlocks);
   if (need_grad) {

@@ -43,4 +43,6 @@ def test_c_entries_refuse_before_any_launch():
     assert lib.ms_act8_bwd_reduce(p, 0, p, p, 0, p, 0, p, 1, 1, 1, 0.2, 0) == -1
     assert lib.ms_act8_bn_act_bwd(p, 0, p, p, p, p, p, p, 1, 8, 4096, 0.2, p, 1, 0) == -3
     assert lib.ms_act8_bn_act_bwd(p, 0, p, p, p, 0, p, p, 1, 8, 64, 0.2, p, 4096, 0) == -1
+    off = p + 8 - p % 16 if p % 16 <= 8 else p + 4            # a record that is not 16-byte aligned
+    assert off % 16 and lib.ms_act8_pack(p, off, p, p, 1, 1, 1, 0) == -2 and lib.ms_act8_unpack(p, p, off, p, 1, 1, 1, 0) == -2
     assert lib.ms_act8_block() == ops.ACT8_BLOCK

@@ -296,6 +296,24 @@ def test_several_pieces():
         close(db, r["db"], tdb, "db")
 
 
+def test_the_most_classes():
+    """2^20 classes: the statistics of all rows no longer fit beside one another and are formed 2048 rows at a time.  Checked on rows around the cut and at the end."""
+    V, C, P = 1 << 20, 136, 2100
+    h, w, b, lab = make((P, C), 64, B, B, seed=3, void=0.0)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    w = (torch.randn(V, C, generator=g, device="cuda") / C ** 0.5).to(B)
+    b = torch.randn(V, generator=g, device="cuda") * 0.3
+    lab = torch.randint(0, V, (P,), generator=g, device="cuda")
+    nll, lse = ops.class_ce_fwd(h, w, b, lab)
+    for i in (0, 1, 1023, 1024, 2047, 2048, 2049, 2098, 2099):
+        z = (w.double() @ h[i].double()) + b.double()
+        A = float((w.double().abs() @ h[i].double().abs()).max() + b.abs().max())
+        want = torch.logsumexp(z, 0)
+        # classes are summed 64 fp32 terms a thread, then in a tree of 16384 / 16 + 16 parts: (64 + 1040) u32 of the sum
+        tol = 2 * A * (3 * 2.0 ** -22 + (3 * C + 8) * U32) + (16 + 1104) * U32 * (abs(float(want)) + 1)
+        assert abs(float(lse[i]) - float(want)) <= tol and abs(float(nll[i]) - float(want - z[lab[i]])) <= tol
+
+
 def test_unaligned_views():
     h, w, b, lab = make((2, 16, 9, 7), 21, seed=3)
     want = ops.class_ce(h, w, b, lab)
