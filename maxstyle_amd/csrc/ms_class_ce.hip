@@ -5,7 +5,8 @@
 //   logits -> stats     tile of z stays in registers: (max, sum exp) of each row and class tile, and the label's own z
 //   join                lse and nll of every row, loss in 64 bits
 //   per piece           G (logits again, written as fp16 planes), dh += G w, dw += G^T h; db from G's epilogue
-// The logits are never written; G exists for one piece at a time (kCePieceBytes: it stays in the 256 MB last-level cache between its writer and its two readers).
+// The logits are never written; G exists for one piece at a time (kCePieceBytes: it
+// stays in the 256 MB last-level cache between its writer and its two readers).
 #include <algorithm>
 #include "ms_class_ce.h"
 #include "ms_class_ce_narrow.h"
@@ -13,7 +14,7 @@
 
 namespace ms {
 
-constexpr size_t kCePieceBytes = (size_t)128 << 20, kCeStatsBytes = (size_t)256 << 20;
+constexpr size_t kCePieceBytes = (size_t)224 << 20, kCeStatsBytes = (size_t)256 << 20;
 
 // ------------------------------------------------------------------------------------------------------------------------------ small passes
 // Rows [rows][C] -> planes [rows_pad][Cp] and each row's 2^e.  One wave a row; 8 channels a lane where the rows are made of whole vectors.
@@ -317,18 +318,24 @@ __global__ __launch_bounds__(WM * WN * 64) void ce_gemm_kernel(CeGemm g) {
     if (t + 1 < k1) stage(t + 1);
     const _Float16* sa = &sm[t & 1][0];
     const _Float16* sb = sa + BM * kCeBK;
+    // All fragments of the slab first, then its products in one run at raised priority: the other workgroup's (wave's) reads and DMA fill the gaps (1163 -> 1115 us for
+    // 6400 rows x 512 channels x 32768 classes).  A ring of four slabs of 32 with counted waits was slower (1298: a barrier per 32).
+    ms_h8 fa[2][MI], fb[2][NJ];
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      ms_h8 fa[MI], fb[NJ];
 #pragma unroll
-      for (int i = 0; i < MI; ++i) fa[i] = ce_frag<BM, ACOL>(sa, wm * TM + i * 16, ks, lane);
+      for (int i = 0; i < MI; ++i) fa[ks][i] = ce_frag<BM, ACOL>(sa, wm * TM + i * 16, ks, lane);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) fb[j] = ce_frag<BN, BCOL>(sb, wn * TN + j * 16, ks, lane);
+      for (int j = 0; j < NJ; ++j) fb[ks][j] = ce_frag<BN, BCOL>(sb, wn * TN + j * 16, ks, lane);
+    }
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[i], fb[j], acc[i][j], 0, 0, 0);
-    }
+        for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[ks][i], fb[ks][j], acc[i][j], 0, 0, 0);
+    __builtin_amdgcn_s_setprio(0);
   }
 
   // Fragment layout of the result: column n = lane & 15, rows m = 4 (lane >> 4) + 0..3.
@@ -521,9 +528,10 @@ static CePlan ce_plan(int N, int C, int V, int HW, int types, bool grad) {
   k.Pp = ce_up(k.P, kCePad); k.Vp = (int)ce_up(V, kCePad); k.Cp = (int)ce_up(C, kCeBK);
   k.xp = (types & 1) ? 1 : 2; k.wp = (types & 2) ? 1 : 2;
   k.gpl = (k.xp == 2 || k.wp == 2) ? 2 : 1;
-  // Pieces of G: up to 8192 classes, and as many rows as kCePieceBytes holds, both cut evenly (6 pieces of 90 % fill the chip better than 5 whole ones and a scrap).
+  // Pieces of G: up to 16384 classes, and as many rows as kCePieceBytes holds, both cut evenly (6 pieces of 90 % fill the chip better than 5 whole ones and a scrap).
+  // Half of both was 4 % slower (shorter sums, more partial results).
   auto even = [](long n, long most) { return ce_up((n + (n + most - 1) / most - 1) / ((n + most - 1) / most), kCePad); };
-  k.vb = (int)even(k.Vp, 8192);
+  k.vb = (int)even(k.Vp, 16384);
   k.pb = (int)even(k.Pp, std::max<long>(kCePad, (long)(kCePieceBytes / ((size_t)k.vb * 2 * k.gpl)) / kCePad * kCePad));
   k.nparts = k.Vp / 128 * 2;
   k.sb = (int)even(k.Pp, std::max<long>(kCePad, (long)(kCeStatsBytes / ((size_t)k.nparts * 8)) / kCePad * kCePad));
