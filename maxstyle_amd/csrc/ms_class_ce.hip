@@ -19,31 +19,34 @@ constexpr size_t kCePieceBytes = (size_t)224 << 20, kCeStatsBytes = (size_t)256 
 // ------------------------------------------------------------------------------------------------------------------------------ small passes
 // Rows [rows][C] -> planes [rows_pad][Cp] and each row's 2^e.  One wave a row; 8 channels a lane where the rows are made of whole vectors.
 //   weights: bpad[v] = b log2(e), or -inf behind the last class; features (labels != nullptr): a row that takes no part is packed as zeros when `drop` is set (it may hold anything)
-template <typename WT, int PL, bool VEC>
-__global__ __launch_bounds__(256) void ce_pack_rows_kernel(const void* __restrict__ w, const float* __restrict__ b, const int64_t* __restrict__ labels, int classes, int drop,
-                                                           _Float16* __restrict__ out, size_t plane, float* __restrict__ fw, float* __restrict__ bpad,
-                                                           int* __restrict__ lab32, int rows, int rows_pad, int C, int Cp) {
-  using IO = ActIO<WT>;
-  const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (r >= rows_pad) return;
-  bool live = r < rows;
-  if (labels != nullptr) {
+struct CePack {
+  const void* src; const float* b; const int64_t* labels; int classes, drop;
+  _Float16* out; size_t plane; float *f, *bpad; int* lab32; int rows, rows_pad, C, Cp;
+};
+template <typename T, bool VEC>
+__device__ __forceinline__ void ce_pack_row(const CePack& a, int r) {
+  using IO = ActIO<T>;
+  constexpr int PL = sizeof(T) == 4 ? 2 : 1;
+  const int lane = threadIdx.x & 63;
+  if (r >= a.rows_pad) return;
+  bool live = r < a.rows;
+  if (a.labels != nullptr) {
     int y = -1;
-    if (live) { const int64_t l = labels[r]; y = (l >= 0 && l < classes) ? (int)l : -1; }
-    live = live && (!drop || y >= 0);
-    if (lane == 0) lab32[r] = y;
+    if (live) { const int64_t l = a.labels[r]; y = (l >= 0 && l < a.classes) ? (int)l : -1; }
+    live = live && (!a.drop || y >= 0);
+    if (lane == 0) a.lab32[r] = y;
   }
-  const size_t base = (size_t)r * C;
+  const size_t base = (size_t)r * a.C;
   unsigned am = 0;
   auto see = [&](float v) { am = max(am, __float_as_uint(v) & 0x7FFFFFFFu); };
   if (live) {
     if (VEC) {
-      for (int c = lane * 8; c < C; c += 512) {
-        const float4 u = IO::ld4(w, base + c), v = IO::ld4(w, base + c + 4);
+      for (int c = lane * 8; c < a.C; c += 512) {
+        const float4 u = IO::ld4(a.src, base + c), v = IO::ld4(a.src, base + c + 4);
         see(u.x); see(u.y); see(u.z); see(u.w); see(v.x); see(v.y); see(v.z); see(v.w);
       }
     } else {
-      for (int c = lane; c < C; c += 64) see(IO::ld1(w, base + c));
+      for (int c = lane; c < a.C; c += 64) see(IO::ld1(a.src, base + c));
     }
   }
 #pragma unroll
@@ -51,25 +54,32 @@ __global__ __launch_bounds__(256) void ce_pack_rows_kernel(const void* __restric
   const int e = ce_exponent(__uint_as_float(am));
   const float inv = ce_pow2(-e);
   if (lane == 0) {
-    fw[r] = ce_pow2(e);
-    if (bpad != nullptr) bpad[r] = r < rows ? (b != nullptr ? b[r] * kLog2e : 0.f) : -__builtin_inff();
+    a.f[r] = ce_pow2(e);
+    if (a.bpad != nullptr) a.bpad[r] = r < a.rows ? (a.b != nullptr ? a.b[r] * kLog2e : 0.f) : -__builtin_inff();
   }
-  for (int c = lane * 8; c < Cp; c += 512) {
+  for (int c = lane * 8; c < a.Cp; c += 512) {
     float v[8];
     if (VEC) {
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f), d = a;
-      if (live && c < C) { a = IO::ld4(w, base + c); d = IO::ld4(w, base + c + 4); }
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = d.x; v[5] = d.y; v[6] = d.z; v[7] = d.w;
+      float4 p = make_float4(0.f, 0.f, 0.f, 0.f), d = p;
+      if (live && c < a.C) { p = IO::ld4(a.src, base + c); d = IO::ld4(a.src, base + c + 4); }
+      v[0] = p.x; v[1] = p.y; v[2] = p.z; v[3] = p.w; v[4] = d.x; v[5] = d.y; v[6] = d.z; v[7] = d.w;
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = (live && c + k < C) ? IO::ld1(w, base + c + k) : 0.f;
+      for (int k = 0; k < 8; ++k) v[k] = (live && c + k < a.C) ? IO::ld1(a.src, base + c + k) : 0.f;
     }
     ms_h8 hi, lo;
 #pragma unroll
     for (int k = 0; k < 8; ++k) { _Float16 x, y; ce_split(v[k] * inv, x, y); hi[k] = x; lo[k] = y; }
-    *reinterpret_cast<ms_h8*>(out + (size_t)r * Cp + c) = hi;
-    if (PL == 2) *reinterpret_cast<ms_h8*>(out + plane + (size_t)r * Cp + c) = lo;
+    *reinterpret_cast<ms_h8*>(a.out + (size_t)r * a.Cp + c) = hi;
+    if (PL == 2) *reinterpret_cast<ms_h8*>(a.out + a.plane + (size_t)r * a.Cp + c) = lo;
   }
+}
+// the first wblocks workgroups: weights; the others: feature rows (there are none when the features come as planes)
+template <typename HT, typename WT, bool VEC>
+__global__ __launch_bounds__(256) void ce_pack_rows_kernel(CePack w, CePack h, int wblocks) {
+  const int wave = threadIdx.x >> 6;
+  if ((int)blockIdx.x < wblocks) ce_pack_row<WT, VEC>(w, (int)blockIdx.x * 4 + wave);
+  else ce_pack_row<HT, VEC>(h, ((int)blockIdx.x - wblocks) * 4 + wave);
 }
 
 // h [N][C][HW], HW > 1 -> the same packed rows.  A workgroup takes 64 pixels: a wave reads 64 neighbouring pixels of a channel at a time and writes 8 channels of each.
@@ -132,27 +142,24 @@ __device__ __forceinline__ int ce_count(const int* __restrict__ slots, int n, in
   return red[0] + red[1] + red[2] + red[3];
 }
 
-// The upstream gradient of every row: grad[p], or sign / rows (rows that take part) times *scale_dev; 0 where the label is not a class.  A row without one gets a log-sum
-// of infinity: exp(z - inf) = 0 whatever its logits are.  rowmax[workgroup]: the largest exponent of g_p 2^ex[p].
-__global__ __launch_bounds__(256) void ce_rowgrad_kernel(const float* __restrict__ grad, float sign, int mean_valid, const float* __restrict__ scale_dev, const int* __restrict__ lab32,
-                                                         const float* __restrict__ fx, float* __restrict__ gp, const float* __restrict__ lse_in, float* __restrict__ lse2,
-                                                         const int* __restrict__ slots, int nslots, int* __restrict__ rowmax, long P, long Pp) {
+__device__ __forceinline__ int ce_row_exponent(float g, float fx) {
+  const unsigned b = __float_as_uint(g) & 0x7FFFFFFFu;
+  return (b != 0u && b < 0x7F800000u) ? (int)(b >> 23) - 126 + (int)(__float_as_uint(fx) >> 23) - 127 : -100000;
+}
+// The upstream gradient of every row: grad[p], 0 where the label is not a class.  A row without one gets a log-sum of infinity: exp(z - inf) = 0 whatever its logits are.
+// rowmax[workgroup]: the largest exponent of g_p 2^ex[p].
+__global__ __launch_bounds__(256) void ce_rowgrad_kernel(const float* __restrict__ grad, const int* __restrict__ lab32, const float* __restrict__ fx, float* __restrict__ gp,
+                                                         const float* __restrict__ lse_in, float* __restrict__ lse2, int* __restrict__ rowmax, long P, long Pp) {
   __shared__ int red[4];
-  const int cnt = mean_valid ? ce_count(slots, nslots, red) : 0;
-  const float g0 = grad != nullptr ? 0.f : sign / (float)(mean_valid ? max(cnt, 1) : P) * (scale_dev != nullptr ? *scale_dev : 1.f);
   int e = -100000;
   for (long p = (long)blockIdx.x * 256 + threadIdx.x; p < Pp; p += (long)gridDim.x * 256) {
-    float g = 0.f;
-    if (p < P && lab32[p] >= 0) g = grad != nullptr ? grad[p] : g0;
-    const unsigned b = __float_as_uint(g) & 0x7FFFFFFFu;
-    if (b != 0u && b < 0x7F800000u) e = max(e, (int)(b >> 23) - 126 + (int)(__float_as_uint(fx[p]) >> 23) - 127);
+    const float g = (p < P && lab32[p] >= 0) ? grad[p] : 0.f;
+    e = max(e, ce_row_exponent(g, fx[p]));
     gp[p] = g;
-    if (g == 0.f) lse2[p] = __builtin_inff();
-    else if (lse_in != nullptr) lse2[p] = lse_in[p] * kLog2e;
+    lse2[p] = g == 0.f ? __builtin_inff() : lse_in[p] * kLog2e;
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) e = max(e, __shfl_xor(e, off, 64));
-  __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = e;
   __syncthreads();
   if (threadIdx.x == 0) rowmax[blockIdx.x] = max(max(red[0], red[1]), max(red[2], red[3]));
@@ -172,7 +179,7 @@ __global__ __launch_bounds__(1024) void ce_scalars_kernel(const double* __restri
   }
   if (rowmax == nullptr) return;
   int er = -100000, ew = -100000;
-  if ((int)threadIdx.x < nrow) er = rowmax[threadIdx.x];
+  for (int i = threadIdx.x; i < nrow; i += 1024) er = max(er, rowmax[i]);
   for (int v = threadIdx.x; v < V; v += 1024) ew = max(ew, (int)(__float_as_uint(fw[v]) >> 23) - 127);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) { er = max(er, __shfl_xor(er, off, 64)); ew = max(ew, __shfl_xor(ew, off, 64)); }
@@ -184,15 +191,19 @@ __global__ __launch_bounds__(1024) void ce_scalars_kernel(const double* __restri
   scal[0] = er < -50000 ? 0 : min(max(kCeTopExp - (er + ew), -120), 120);
 }
 
-// part[t][p] = {max, sum exp} over one class range -> lse, nll; loss partials in 64 bits.  64 rows a workgroup, 16 threads each over the class ranges.  All in units of log2.
+struct CeRowGrad { float* gp; const float* fx; float sign; int mean_valid; const float* scale_dev; const int* slots; int nslots; int* rowmax; };
+
+// part[t][p] = {max, sum exp} over one class range -> lse, nll; loss partials in 64 bits; with r.gp the rows' upstream gradients (ce_rowgrad_kernel's work).  64 rows a workgroup, 16 threads each over the class ranges.  All in units of log2.
 __device__ __forceinline__ void ce_merge(float& m, float& l, float mo, float lo) {
   const float mn = fmaxf(m, mo), mm = mn == -__builtin_inff() ? 0.f : mn;
   l = l * __builtin_amdgcn_exp2f(m - mm) + lo * __builtin_amdgcn_exp2f(mo - mm);
   m = mn;
 }
 __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict__ part, int nparts, size_t stride, const float* __restrict__ zlab, const int* __restrict__ lab32,
-                                                       float* __restrict__ lse2, float* __restrict__ lse_out, float* __restrict__ nll_out, double* __restrict__ lsum, long p0, long P) {
+                                                       float* __restrict__ lse2, float* __restrict__ lse_out, float* __restrict__ nll_out, double* __restrict__ lsum, long p0, long P, CeRowGrad rg) {
   __shared__ float2 sh[16][64];
+  __shared__ int redi[16];
+  const int cnt = (rg.gp != nullptr && rg.mean_valid) ? ce_count(rg.slots, rg.nslots, redi) : 0;
   const int el = threadIdx.x & 63, grp = threadIdx.x >> 6;
   const long pr = (long)blockIdx.x * 64 + el, p = p0 + pr;          // (padded)
   float m = -__builtin_inff(), l = 0.f;
@@ -203,8 +214,18 @@ __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict_
   if (grp != 0) return;
   for (int k = 1; k < 16; ++k) ce_merge(m, l, sh[k][el].x, sh[k][el].y);
   const float lg = __builtin_amdgcn_logf(l), ln2 = 0.693147180559945309f;      // (log2)
-  lse2[p] = m + lg;
+  float ls = m + lg;
   double acc = 0.0;
+  if (rg.gp != nullptr) {
+    const float g = (p < P && lab32[p] >= 0) ? rg.sign / (float)(rg.mean_valid ? max(cnt, 1) : P) * (rg.scale_dev != nullptr ? *rg.scale_dev : 1.f) : 0.f;
+    rg.gp[p] = g;
+    if (g == 0.f) ls = __builtin_inff();
+    int e = ce_row_exponent(g, rg.fx[p]);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) e = max(e, __shfl_xor(e, off, 64));
+    if (el == 0) rg.rowmax[p0 / 64 + blockIdx.x] = e;
+  }
+  lse2[p] = ls;
   if (p < P) {
     if (lse_out != nullptr) lse_out[p] = (m + lg) * ln2;
     const float v = lab32[p] >= 0 ? ((m - zlab[p]) + lg) * ln2 : 0.f;        // (max - z) + log sum: nothing cancels where the label has the maximum
@@ -470,44 +491,54 @@ __global__ __launch_bounds__(WM * WN * 64) void ce_gemm_kernel(CeGemm g) {
   }
 }
 
-// Sum of a product's K-splits -> dh or dw.  part [split][rows][ld]:
-//   PLANES  rows = channels, columns = pixels of this piece, written as [n][channel][hw];  f = 2^ex of the column
+// The sums behind a piece's products, one launch: db from G's epilogue, dh and dw from their K-splits (each a range of workgroups; any may be empty).
+// A product's partials [split][rows][ld] ->
+//   planes  rows = channels, columns = pixels of this piece, written as [n][channel][hw];  f = 2^ex of the column
 //   else    rows = classes (dw) or feature rows (dh with HW = 1) of this piece, columns = channels, written as [row][channel];  f = 2^ew / 2^ex of the row
 //   first: nothing is there yet, else the fp32 running sum `acc` is added;  last: written to `out` in its type, else back to `acc`.
-template <typename OT, bool PLANES>
-__global__ __launch_bounds__(256) void ce_reduce_kernel(const float* __restrict__ part, size_t out_split, int ld, int split, const float* __restrict__ f, const int* __restrict__ scal,
-                                                        float* __restrict__ acc, void* __restrict__ out, int first, int last, int rows, int cols, long r0, int HW, int C) {
+struct CeSum { const float* part; size_t out_split; int ld, split; const float* f; float* acc; void* out; int first, last, rows, cols; long r0; int HW, C, blocks, rblocks; };
+struct CeSums { CeSum h, w; const float* dbpart; int dbn; size_t dbstride; float* db; int dbfirst, dbV, dbv0, dbblocks; const int* scal; };
+template <typename OT>
+__device__ __forceinline__ void ce_sum(const CeSum& a, int id, const int* scal, bool planes) {
   const float gi = ce_pow2(-scal[0]);
-  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (row >= rows) return;
-  for (int c = blockIdx.y * 64 + lane; c < cols; c += gridDim.y * 64) {
-    const float* src = part + (size_t)row * ld + c;
+  const int row = (id % a.rblocks) * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, ny = a.blocks / a.rblocks;
+  if (row >= a.rows) return;
+  for (int c = (id / a.rblocks) * 64 + lane; c < a.cols; c += ny * 64) {
+    const float* src = a.part + (size_t)row * a.ld + c;
     float s = 0.f;
-    for (int k = 0; k < split; ++k) s += src[k * out_split];
+    for (int k = 0; k < a.split; ++k) s += src[k * a.out_split];
     size_t dst;
-    if (PLANES) {
-      const int p = (int)r0 + c, n = p / HW;
-      dst = ((size_t)n * C + row) * HW + (p - n * HW);
-      s *= gi / f[p];
+    if (planes) {
+      const int p = (int)a.r0 + c, n = p / a.HW;
+      dst = ((size_t)n * a.C + row) * a.HW + (p - n * a.HW);
+      s *= gi / a.f[p];
     } else {
-      dst = (size_t)(r0 + row) * C + c;
-      s *= gi / f[r0 + row];
+      dst = (size_t)(a.r0 + row) * a.C + c;
+      s *= gi / a.f[a.r0 + row];
     }
-    if (!first) s += acc[dst];
-    if (last) ActIO<OT>::st1(out, dst, s); else acc[dst] = s;
+    if (!a.first) s += a.acc[dst];
+    if (a.last) ActIO<OT>::st1(a.out, dst, s); else a.acc[dst] = s;
   }
 }
-__global__ __launch_bounds__(1024) void ce_db_kernel(const float* __restrict__ part, int n, size_t stride, float* __restrict__ db, int first, int V, int v0) {
-  __shared__ double sh[16][64];
-  const int el = threadIdx.x & 63, grp = threadIdx.x >> 6, v = blockIdx.x * 64 + el;
-  double s = 0.0;
-#pragma unroll 4
-  for (int i = grp; i < n; i += 16) s += (double)part[(size_t)i * stride + v];      // (columns padded to whole tiles)
-  sh[grp][el] = s;
-  __syncthreads();
-  if (grp != 0 || v >= V) return;
-  for (int k = 1; k < 16; ++k) s += sh[k][el];
-  db[v0 + v] = (float)(first ? s : s + (double)db[v0 + v]);
+template <typename HT, typename WT>
+__global__ __launch_bounds__(256) void ce_sums_kernel(CeSums a) {
+  __shared__ double sh[4][64];
+  int id = blockIdx.x;
+  if (id < a.dbblocks) {
+    const int el = threadIdx.x & 63, grp = threadIdx.x >> 6, v = id * 64 + el;
+    double s = 0.0;
+#pragma unroll 8
+    for (int i = grp; i < a.dbn; i += 4) s += (double)a.dbpart[(size_t)i * a.dbstride + v];      // (columns padded to whole tiles)
+    sh[grp][el] = s;
+    __syncthreads();
+    if (grp != 0 || v >= a.dbV) return;
+    s += sh[1][el] + sh[2][el] + sh[3][el];
+    a.db[a.dbv0 + v] = (float)(a.dbfirst ? s : s + (double)a.db[a.dbv0 + v]);
+    return;
+  }
+  id -= a.dbblocks;
+  if (id < a.h.blocks) { ce_sum<HT>(a.h, id, a.scal, a.h.HW > 1); return; }
+  ce_sum<WT>(a.w, id - a.h.blocks, a.scal, false);
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------ host
@@ -541,7 +572,7 @@ static CePlan ce_plan(int N, int C, int V, int HW, int types, bool grad) {
   k.o_w = take((size_t)k.wp * k.Vp * k.Cp * 2);
   k.o_fx = take(k.Pp * 4); k.o_fw = take((size_t)k.Vp * 4); k.o_b = take((size_t)k.Vp * 4);
   k.o_lab = take(k.Pp * 4); k.o_lse = take(k.Pp * 4); k.o_zl = take(k.Pp * 4); k.o_gp = take(k.Pp * 4);
-  k.o_scal = take(64); k.o_slots = take(kCeSlots * 4); k.o_rowmax = take(kCeRowBlocks * 4);
+  k.o_scal = take(64); k.o_slots = take(kCeSlots * 4); k.o_rowmax = take((size_t)(k.Pp / 64) * 4);
   k.o_lsum = take((size_t)(k.Pp / 64) * 8);
   const size_t stats = (size_t)k.nparts * k.sb * 8;
   if (!grad) { k.o_part = take(stats); k.total = o; return k; }
@@ -605,23 +636,28 @@ static int ce_run(const CeArgs& a, const char* who) {
   int *lab = (int*)(ws + k.o_lab), *scal = (int*)(ws + k.o_scal), *slots = (int*)(ws + k.o_slots), *rowmax = (int*)(ws + k.o_rowmax);
   float *fx = f32(k.o_fx), *fw = f32(k.o_fw), *bp = f32(k.o_b), *lse = f32(k.o_lse), *zl = f32(k.o_zl), *gp = f32(k.o_gp);
   hipStream_t st = a.st;
-  auto pack_rows = [&](const void* src, bool bf, const float* b, const int64_t* labels, _Float16* out, size_t pl, float* f, float* bpad, int rows, int rows_pad) {
-    const bool vec = a.C % 8 == 0 && aligned16(src);
-    const dim3 grid(rows_pad / 4), block(256);
-    const int drop = need_grad ? 1 : 0;
-    if (bf && vec) MS_LAUNCH((ce_pack_rows_kernel<ms_bf16, 1, true>), grid, block, 0, st, src, b, labels, a.V, drop, out, pl, f, bpad, lab, rows, rows_pad, a.C, k.Cp);
-    else if (bf) MS_LAUNCH((ce_pack_rows_kernel<ms_bf16, 1, false>), grid, block, 0, st, src, b, labels, a.V, drop, out, pl, f, bpad, lab, rows, rows_pad, a.C, k.Cp);
-    else if (vec) MS_LAUNCH((ce_pack_rows_kernel<float, 2, true>), grid, block, 0, st, src, b, labels, a.V, drop, out, pl, f, bpad, lab, rows, rows_pad, a.C, k.Cp);
-    else MS_LAUNCH((ce_pack_rows_kernel<float, 2, false>), grid, block, 0, st, src, b, labels, a.V, drop, out, pl, f, bpad, lab, rows, rows_pad, a.C, k.Cp);
-    return check_launch("class_ce_pack");
-  };
-  if (int e = pack_rows(a.w, (a.types & 2) != 0, a.b, nullptr, w, wpl, fw, bp, a.V, k.Vp)) return e;
-  if (a.HW == 1) {
-    if (int e = pack_rows(a.h, (a.types & 1) != 0, nullptr, a.labels, x, xpl, fx, nullptr, a.N, (int)k.Pp)) return e;
-  } else {
+  const bool rows_form = a.HW == 1, hb = (a.types & 1) != 0, wb = (a.types & 2) != 0;
+  const int drop = need_grad ? 1 : 0;
+  {
+    const CePack pw{a.w, a.b, nullptr, 0, 0, w, wpl, fw, bp, nullptr, a.V, k.Vp, a.C, k.Cp};
+    const CePack ph{a.h, nullptr, a.labels, a.V, drop, x, xpl, fx, nullptr, lab, a.N, (int)k.Pp, a.C, k.Cp};
+    const bool vec = a.C % 8 == 0 && aligned16(a.w) && (!rows_form || aligned16(a.h));
+    const int wblocks = k.Vp / 4;
+    const dim3 grid((unsigned)(wblocks + (rows_form ? k.Pp / 4 : 0))), block(256);
+    if (hb && wb && vec) MS_LAUNCH((ce_pack_rows_kernel<ms_bf16, ms_bf16, true>), grid, block, 0, st, pw, ph, wblocks);
+    else if (hb && wb) MS_LAUNCH((ce_pack_rows_kernel<ms_bf16, ms_bf16, false>), grid, block, 0, st, pw, ph, wblocks);
+    else if (hb && vec) MS_LAUNCH((ce_pack_rows_kernel<ms_bf16, float, true>), grid, block, 0, st, pw, ph, wblocks);
+    else if (hb) MS_LAUNCH((ce_pack_rows_kernel<ms_bf16, float, false>), grid, block, 0, st, pw, ph, wblocks);
+    else if (wb && vec) MS_LAUNCH((ce_pack_rows_kernel<float, ms_bf16, true>), grid, block, 0, st, pw, ph, wblocks);
+    else if (wb) MS_LAUNCH((ce_pack_rows_kernel<float, ms_bf16, false>), grid, block, 0, st, pw, ph, wblocks);
+    else if (vec) MS_LAUNCH((ce_pack_rows_kernel<float, float, true>), grid, block, 0, st, pw, ph, wblocks);
+    else MS_LAUNCH((ce_pack_rows_kernel<float, float, false>), grid, block, 0, st, pw, ph, wblocks);
+    if (int e = check_launch("class_ce_pack")) return e;
+  }
+  if (!rows_form) {
     const dim3 gx((unsigned)(k.Pp / 64));
-    if (a.types & 1) MS_LAUNCH((ce_pack_planes_kernel<ms_bf16, 1>), gx, dim3(1024), 0, st, a.h, a.labels, a.V, need_grad ? 1 : 0, x, xpl, fx, lab, k.P, k.Pp, a.C, k.Cp, a.HW);
-    else MS_LAUNCH((ce_pack_planes_kernel<float, 2>), gx, dim3(1024), 0, st, a.h, a.labels, a.V, need_grad ? 1 : 0, x, xpl, fx, lab, k.P, k.Pp, a.C, k.Cp, a.HW);
+    if (hb) MS_LAUNCH((ce_pack_planes_kernel<ms_bf16, 1>), gx, dim3(1024), 0, st, a.h, a.labels, a.V, drop, x, xpl, fx, lab, k.P, k.Pp, a.C, k.Cp, a.HW);
+    else MS_LAUNCH((ce_pack_planes_kernel<float, 2>), gx, dim3(1024), 0, st, a.h, a.labels, a.V, drop, x, xpl, fx, lab, k.P, k.Pp, a.C, k.Cp, a.HW);
     if (int e = check_launch("class_ce_pack")) return e;
   }
   const int nslots = (int)std::min<long>(kCeSlots, k.P / 1024 + 1);
@@ -629,6 +665,7 @@ static int ce_run(const CeArgs& a, const char* who) {
     MS_LAUNCH(ce_count_kernel, dim3(nslots), dim3(256), 0, st, a.labels, k.P, a.V, slots);
     if (int e = check_launch("class_ce_count")) return e;
   }
+  const CeRowGrad rg{gp, fx, a.sign, a.mean_valid, a.scale_dev, slots, nslots, rowmax};
   CeGemm g{};
   g.fw = fw; g.bpad = bp; g.fx = fx; g.lab = lab; g.lse = lse; g.gp = gp; g.scal = scal; g.zlab = zl;
   if (a.lse_in == nullptr) {
@@ -642,13 +679,13 @@ static int ce_run(const CeArgs& a, const char* who) {
       d.part = (float2*)(ws + k.o_part); d.part_stride = (size_t)k.sb;
       if (int e = ce_gemm<CE_STATS, false, false>(d, k.Vp, pn, st, "class_ce_stats")) return e;
       MS_LAUNCH(ce_join_kernel, dim3((unsigned)(pn / 64)), dim3(1024), 0, st, (const float2*)d.part, ce_big(k.Vp, pn, 1) ? k.nparts / 2 : k.nparts, d.part_stride, zl, lab, lse, a.lse, a.nll,
-                (double*)(ws + k.o_lsum), p0, k.P);
+                (double*)(ws + k.o_lsum), p0, k.P, need_grad ? rg : CeRowGrad{});
       if (int e = check_launch("class_ce_join")) return e;
     }
   }
-  const int nrow = (int)std::min<long>(k.Pp / 256, kCeRowBlocks);
-  if (need_grad) {
-    MS_LAUNCH(ce_rowgrad_kernel, dim3(nrow), dim3(256), 0, st, a.grad, a.sign, a.mean_valid, a.scale_dev, lab, fx, gp, a.lse_in, lse, slots, nslots, rowmax, k.P, k.Pp);
+  const int nrow = a.lse_in != nullptr ? (int)std::min<long>(k.Pp / 256, kCeRowBlocks) : (int)(k.Pp / 64);
+  if (a.lse_in != nullptr) {
+    MS_LAUNCH(ce_rowgrad_kernel, dim3(nrow), dim3(256), 0, st, a.grad, lab, fx, gp, a.lse_in, lse, rowmax, k.P, k.Pp);
     if (int e = check_launch("class_ce_rowgrad")) return e;
   }
   if (need_grad || a.loss != nullptr) {
@@ -672,51 +709,48 @@ static int ce_run(const CeArgs& a, const char* who) {
       d.dbpart = a.db != nullptr ? f32(k.o_db) : nullptr; d.db_stride = k.vb;
       if (k.gpl == 2) { if (int e = ce_gemm<CE_GRAD2, false, false>(d, vn, pn, st, "class_ce_grad")) return e; }
       else { if (int e = ce_gemm<CE_GRAD, false, false>(d, vn, pn, st, "class_ce_grad")) return e; }
-      if (a.db != nullptr) {
-        const int vr = std::min(vn, a.V - v0);
-        if (vr > 0) {
-          MS_LAUNCH(ce_db_kernel, dim3(cdiv(vr, 64)), dim3(1024), 0, st, f32(k.o_db), pn / 128 * 2, (size_t)k.vb, a.db, p0 == 0 ? 1 : 0, vr, v0);
-          if (int e = check_launch("class_ce_db")) return e;
-        }
+      const int rows = (int)std::min<long>(pn, k.P - p0), vr = std::max(0, std::min(vn, a.V - v0));
+      CeSums sums{};
+      sums.scal = scal;
+      if (a.db != nullptr && vr > 0) {
+        sums.dbpart = f32(k.o_db); sums.dbn = pn / 128 * 2; sums.dbstride = (size_t)k.vb; sums.db = a.db; sums.dbfirst = p0 == 0; sums.dbV = vr; sums.dbv0 = v0;
+        sums.dbblocks = cdiv(vr, 64);
       }
       if (a.dh != nullptr) {        // dh^T [channels][pixels] = w^T G^T, or dh [rows][channels] = G w where the channels are neighbours
-        const bool rows_form = a.HW == 1;
         CeGemm o{};
         const CeOperand ow{w + (size_t)v0 * k.Cp, wpl, k.Cp, k.Cp}, og{G, gpl, k.vb, 0};
-        const int pw = (a.types & 1) ? 1 : k.wp, pg = (a.types & 1) ? 1 : 2;
+        const int pw = hb ? 1 : k.wp, pg = hb ? 1 : 2;
         o.ksteps = vn / kCeBK; o.split = std::min(k.split_x, std::max(1, o.ksteps / 8));
         o.out = f32(k.o_px); o.out_split = (size_t)cp * k.pb;
-        const int rows = (int)std::min<long>(pn, k.P - p0), first = v0 == 0, last = v0 + vn >= k.Vp;
-        float* ac = (a.types & 1) ? f32(k.o_ax) : (float*)a.dh;
         if (rows_form) {
           o.a = og; o.b = ow; ce_pairs(o, pg, pw); o.out_ld = (int)cp;
           if (int e = ce_gemm<CE_OUT, false, true>(o, pn, (int)cp, st, "class_ce_dh")) return e;
-          const dim3 grid((unsigned)cdiv(rows, 4), (unsigned)std::min(cdiv(a.C, 64), 4));
-          if (a.types & 1) MS_LAUNCH((ce_reduce_kernel<ms_bf16, false>), grid, dim3(256), 0, st, o.out, o.out_split, o.out_ld, o.split, fx, scal, ac, a.dh, first, last, rows, a.C, p0, 1, a.C);
-          else MS_LAUNCH((ce_reduce_kernel<float, false>), grid, dim3(256), 0, st, o.out, o.out_split, o.out_ld, o.split, fx, scal, ac, a.dh, first, last, rows, a.C, p0, 1, a.C);
         } else {
           o.a = ow; o.b = og; ce_pairs(o, pw, pg); o.out_ld = k.pb;
           if (int e = ce_gemm<CE_OUT, true, false>(o, (int)cp, pn, st, "class_ce_dh")) return e;
-          const dim3 grid((unsigned)cdiv(a.C, 4), (unsigned)std::min(cdiv(rows, 64), 64));
-          if (a.types & 1) MS_LAUNCH((ce_reduce_kernel<ms_bf16, true>), grid, dim3(256), 0, st, o.out, o.out_split, o.out_ld, o.split, fx, scal, ac, a.dh, first, last, a.C, rows, p0, a.HW, a.C);
-          else MS_LAUNCH((ce_reduce_kernel<float, true>), grid, dim3(256), 0, st, o.out, o.out_split, o.out_ld, o.split, fx, scal, ac, a.dh, first, last, a.C, rows, p0, a.HW, a.C);
         }
-        if (int e = check_launch("class_ce_dh_sum")) return e;
+        CeSum& q = sums.h;
+        q = CeSum{o.out, o.out_split, o.out_ld, o.split, fx, hb ? f32(k.o_ax) : (float*)a.dh, a.dh, v0 == 0, v0 + vn >= k.Vp, rows_form ? rows : a.C, rows_form ? a.C : rows, p0, a.HW, a.C, 0, 0};
+        q.rblocks = cdiv(q.rows, 4); q.blocks = q.rblocks * std::min(cdiv(q.cols, 64), rows_form ? 4 : 64);
       }
-      const int vr = std::min(vn, a.V - v0);
       if (a.dw != nullptr && vr > 0) {        // dw [classes][channels] = G^T h
         CeGemm o{};
         o.a = CeOperand{G, gpl, k.vb, k.vb}; o.b = CeOperand{x + (size_t)p0 * k.Cp, xpl, k.Cp, k.Cp};
-        ce_pairs(o, (a.types & 2) ? 1 : 2, (a.types & 2) ? 1 : k.xp);
+        ce_pairs(o, wb ? 1 : 2, wb ? 1 : k.xp);
         o.ksteps = pn / kCeBK; o.split = std::min(k.split_w, std::max(1, o.ksteps / 8));
         o.out = f32(k.o_pw); o.out_ld = (int)cp; o.out_split = (size_t)k.vb * cp;
         if (int e = ce_gemm<CE_OUT, true, true>(o, vn, (int)cp, st, "class_ce_dw")) return e;
-        const int first = p0 == 0, last = p0 + pn >= k.Pp;
-        const dim3 grid((unsigned)cdiv(vr, 4), (unsigned)std::min(cdiv(a.C, 64), 4));
-        float* ac = (a.types & 2) ? f32(k.o_aw) : (float*)a.dw;
-        if (a.types & 2) MS_LAUNCH((ce_reduce_kernel<ms_bf16, false>), grid, dim3(256), 0, st, o.out, o.out_split, o.out_ld, o.split, fw, scal, ac, a.dw, first, last, vr, a.C, (long)v0, 1, a.C);
-        else MS_LAUNCH((ce_reduce_kernel<float, false>), grid, dim3(256), 0, st, o.out, o.out_split, o.out_ld, o.split, fw, scal, ac, a.dw, first, last, vr, a.C, (long)v0, 1, a.C);
-        if (int e = check_launch("class_ce_dw_sum")) return e;
+        CeSum& q = sums.w;
+        q = CeSum{o.out, o.out_split, o.out_ld, o.split, fw, wb ? f32(k.o_aw) : (float*)a.dw, a.dw, p0 == 0, p0 + pn >= k.Pp, vr, a.C, (long)v0, 1, a.C, 0, 0};
+        q.rblocks = cdiv(q.rows, 4); q.blocks = q.rblocks * std::min(cdiv(q.cols, 64), 4);
+      }
+      const int blocks = sums.dbblocks + sums.h.blocks + sums.w.blocks;
+      if (blocks > 0) {
+        if (hb && wb) MS_LAUNCH((ce_sums_kernel<ms_bf16, ms_bf16>), dim3(blocks), dim3(256), 0, st, sums);
+        else if (hb) MS_LAUNCH((ce_sums_kernel<ms_bf16, float>), dim3(blocks), dim3(256), 0, st, sums);
+        else if (wb) MS_LAUNCH((ce_sums_kernel<float, ms_bf16>), dim3(blocks), dim3(256), 0, st, sums);
+        else MS_LAUNCH((ce_sums_kernel<float, float>), dim3(blocks), dim3(256), 0, st, sums);
+        if (int e = check_launch("class_ce_sums")) return e;
       }
     }
   }
