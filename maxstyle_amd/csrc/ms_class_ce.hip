@@ -254,10 +254,12 @@ struct CeGemm {
 enum { CE_STATS = 0, CE_GRAD = 1, CE_GRAD2 = 2, CE_OUT = 3 };
 
 constexpr int kCeBK = 64;
+// Slabs of a K-split: shorter ones cost more in the sums behind than they save (16 rows x 512 channels x 5000 classes, fp32: 88, 79, 81 us at 6, 12, 24; bf16 73, 62, 60 at 2, 4, 8).
+constexpr int kCeDeep = 12;
 
 // Stage one 64-deep slab of an operand tile into LDS by DMA: 1 KB an instruction, the source address permuted so that the fragment reads below are free of bank conflicts.
 //   ROW: [T rows][64 k]: 16-byte chunk j of row r lies at chunk j ^ (r & 7)
-//   COL: [64 k][T columns]: 32-byte unit u of row k lies at unit u ^ f(k), f = (k & 3) | ((k >> 3) & 1) << 2
+//   COL: [64 k][T columns]: 32-byte unit u of row k lies at unit u ^ f(k), f = (k & 3) | ((k >> 3) & 1) << 2 (T = 64 has four units: f = k & 3)
 template <int T, bool COL, int NW>
 __device__ __forceinline__ void ce_stage(const CeOperand& o, const _Float16* base, int mn0, int wave, int lane, unsigned lds) {
   constexpr int kInstr = T * kCeBK * 2 / 1024;
@@ -272,7 +274,7 @@ __device__ __forceinline__ void ce_stage(const CeOperand& o, const _Float16* bas
     } else {
       constexpr int kRows = 1024 / (T * 2), kCh = T / 8;
       const int k = ins * kRows + lane / kCh, ch = lane % kCh;
-      const int unit = (ch >> 1) ^ ((k & 3) | (((k >> 3) & 1) << 2));
+      const int unit = (ch >> 1) ^ ((k & 3) | (T > 64 ? ((k >> 3) & 1) << 2 : 0));
       const int col = min(mn0 + unit * 16 + (ch & 1) * 8, o.cols - 8);        // columns behind the operand's last are read twice and never used
       voff = (int)(((unsigned)k * (unsigned)o.ld + (unsigned)col) * 2u);
     }
@@ -285,7 +287,7 @@ __device__ __forceinline__ ms_h8 ce_frag(const _Float16* tile, int mn, int ks, i
   if (!COL) {
     return *reinterpret_cast<const ms_h8*>(tile + (mn + i) * kCeBK + (((ks * 4 + q) ^ (i & 7)) * 8));
   } else {
-    const int f = (i >> 2) | ((q & 1) << 2);
+    const int f = (i >> 2) | (T > 64 ? (q & 1) << 2 : 0);
     const int k = ks * 32 + q * 8 + (i >> 2);
     const _Float16* a = tile + k * T + (((mn >> 4) ^ f) * 16) + (i & 3) * 4;
     typedef __attribute__((address_space(3))) ms_s4* lp;
@@ -463,7 +465,7 @@ __global__ __launch_bounds__(WM * WN * 64) void ce_gemm_kernel(CeGemm g) {
     }
     // G goes out through LDS as [row][class], 16 bytes a lane in whole rows
     _Float16* tile = &sm[0][0];
-    constexpr int kCh = BM / 8;
+    constexpr int kCh = BM / 8, kSwz = kCh < 16 ? kCh - 1 : 15;
 #pragma unroll
     for (int pl = 0; pl < (EPI == CE_GRAD2 ? 2 : 1); ++pl) {
       __syncthreads();
@@ -478,14 +480,14 @@ __global__ __launch_bounds__(WM * WN * 64) void ce_gemm_kernel(CeGemm g) {
             v[r] = pl == 0 ? hi : (_Float16)(acc[i][j][r] - (float)hi);
           }
           const int row = wn * TN + j * 16 + li, col = wm * TM + i * 16 + q * 4;
-          *reinterpret_cast<ms_h4*>(tile + row * BM + (((col >> 3) ^ (row & 15)) * 8) + (col & 7)) = v;
+          *reinterpret_cast<ms_h4*>(tile + row * BM + (((col >> 3) ^ (row & kSwz)) * 8) + (col & 7)) = v;
         }
       __syncthreads();
       _Float16* out = g.g + pl * g.g_plane + (size_t)n0 * g.g_ld + m0;
 #pragma unroll
       for (int k = 0; k < BN * kCh / (NW * 64); ++k) {
         const int i = k * (NW * 64) + threadIdx.x, row = i / kCh, ch = i % kCh;
-        *reinterpret_cast<ms_h8*>(out + (size_t)row * g.g_ld + ch * 8) = *reinterpret_cast<const ms_h8*>(tile + row * BM + ((ch ^ (row & 15)) * 8));
+        *reinterpret_cast<ms_h8*>(out + (size_t)row * g.g_ld + ch * 8) = *reinterpret_cast<const ms_h8*>(tile + row * BM + ((ch ^ (row & kSwz)) * 8));
       }
     }
   }
@@ -574,17 +576,18 @@ static CePlan ce_plan(int N, int C, int V, int HW, int types, bool grad) {
   k.o_lab = take(k.Pp * 4); k.o_lse = take(k.Pp * 4); k.o_zl = take(k.Pp * 4); k.o_gp = take(k.Pp * 4);
   k.o_scal = take(64); k.o_slots = take(kCeSlots * 4); k.o_rowmax = take((size_t)(k.Pp / 64) * 4);
   k.o_lsum = take((size_t)(k.Pp / 64) * 8);
-  const size_t stats = (size_t)k.nparts * k.sb * 8;
+  // (two of a tile; 64-wide tiles, twice as many, are taken for less than 128 tiles of 128 x 128: 512 x 254 pairs at most)
+  const size_t stats = std::max((size_t)k.nparts * k.sb * 8, (size_t)2 << 20);
   if (!grad) { k.o_part = take(stats); k.total = o; return k; }
   // The statistics are read before the first piece of G is written: they share its memory.
   k.o_part = o;
   k.o_g = take(std::max((size_t)k.gpl * k.pb * k.vb * 2, stats));
-  k.o_db = take((size_t)(k.pb / 256 * 4) * k.vb * 4);
-  // K-splits: enough tiles for the chip (256 CUs, two workgroups each at 128 x 128), at least 8 slabs of 64 each
-  const long cp = ce_up(k.Cp, 128);
-  auto split = [&](long tiles, long ksteps) { return (int)std::max<long>(1, std::min<long>(std::min<long>(512 / std::max<long>(tiles, 1), ksteps / 8), 64)); };
-  k.split_x = split(cp / 128 * (k.pb / 128), k.vb / 64);
-  k.split_w = split(cp / 128 * (k.vb / 128), k.pb / 64);
+  k.o_db = take((size_t)(k.pb / 64 * 2) * k.vb * 4);
+  // K-splits: enough tiles for the chip (256 CUs, two workgroups each at 128 x 128), each at least kCeDeep slabs (three pairs of planes at most)
+  const long cp = ce_up(k.Cp, 128), rt = std::min<long>(k.pb, ce_up(k.P, 128)), vt = std::min<long>(k.vb, ce_up(V, 128));
+  auto split = [&](long tiles, long ksteps) { return (int)std::max<long>(1, std::min<long>(std::min<long>(512 / std::max<long>(tiles, 1), ksteps * 3 / kCeDeep), 64)); };
+  k.split_x = split(cp / 128 * (rt / 128), vt / 64);
+  k.split_w = split(cp / 128 * (vt / 128), rt / 64);
   k.o_px = take((size_t)k.split_x * cp * k.pb * 4);
   k.o_pw = take((size_t)k.split_w * k.vb * cp * 4);
   k.o_ax = take((k.vb < k.Vp && (types & 1)) ? (size_t)k.P * C * 4 : 0);
@@ -599,20 +602,30 @@ static int ce_check(int N, int C, int V, int HW, int types, const char* who) {
   return MS_OK;
 }
 
-// M, N: sizes in elements, multiples of the tile.  256 x 256 tiles (one workgroup a CU) where there are enough of them for the chip: half the LDS traffic a product.
-// G's kernel keeps 128 x 128: its epilogue is as long as its product at 512 channels, and only a second workgroup on the CU overlaps the two (381 against 428 us).
-static bool ce_big(int M, int N, int split) { return M % 256 == 0 && N % 256 == 0 && (long)(M / 256) * (N / 256) * split >= 200; }
+// Tile of a product of M x N (real sizes; the operands and results hold capM x capN, multiples of 128).
+//   256: one workgroup a CU, half the LDS traffic a product: where there are enough of them for the chip.  G's kernel does without: its epilogue is as long as its product
+//        at 512 channels, and only a second workgroup on the CU overlaps the two (381 against 428 us)
+//   64:  few rows or classes: a quarter of the work a slab on four times the CUs (1 row x 512 channels x 1000 classes, fp32: 92 -> 59 us)
+struct CeTile { int t, mt, nt; };
+template <int EPI> static CeTile ce_tile(long M, long N, int split, long capM, long capN) {
+  auto n = [](long x, long t) { return (x + t - 1) / t; };
+  int t = 64;
+  if ((EPI == CE_STATS || EPI == CE_OUT) && n(M, 256) * 256 <= capM && n(N, 256) * 256 <= capN && n(M, 256) * n(N, 256) * split >= 200) t = 256;
+  else if (n(M, 128) * n(N, 128) * split >= 128) t = 128;
+  return CeTile{t, (int)n(M, t), (int)n(N, t)};
+}
 template <int EPI, bool ACOL, bool BCOL>
-static int ce_gemm(CeGemm g, int M, int N, hipStream_t st, const char* what) {
+static int ce_gemm(CeGemm g, const CeTile& c, hipStream_t st, const char* what) {
+  g.mt = c.mt; g.nt = c.nt;
+  const dim3 grid((unsigned)((long)g.mt * g.nt * g.split));
   if constexpr (EPI == CE_STATS || EPI == CE_OUT) {
-    if (ce_big(M, N, g.split)) {
-      g.mt = M / 256; g.nt = N / 256;
-      MS_LAUNCH((ce_gemm_kernel<256, 256, 2, 4, ACOL, BCOL, EPI>), dim3(g.mt * g.nt * g.split), dim3(512), 0, st, g);
+    if (c.t == 256) {
+      MS_LAUNCH((ce_gemm_kernel<256, 256, 2, 4, ACOL, BCOL, EPI>), grid, dim3(512), 0, st, g);
       return check_launch(what);
     }
   }
-  g.mt = M / 128; g.nt = N / 128;
-  MS_LAUNCH((ce_gemm_kernel<128, 128, 2, 2, ACOL, BCOL, EPI>), dim3(g.mt * g.nt * g.split), dim3(256), 0, st, g);
+  if (c.t == 128) MS_LAUNCH((ce_gemm_kernel<128, 128, 2, 2, ACOL, BCOL, EPI>), grid, dim3(256), 0, st, g);
+  else MS_LAUNCH((ce_gemm_kernel<64, 64, 2, 2, ACOL, BCOL, EPI>), grid, dim3(256), 0, st, g);
   return check_launch(what);
 }
 static void ce_pairs(CeGemm& g, int a, int b) {       // planes of the two operands -> products
@@ -676,9 +689,10 @@ static int ce_run(const CeArgs& a, const char* who) {
       d.a = CeOperand{w, wpl, k.Cp, 0}; d.b = CeOperand{x + (size_t)p0 * k.Cp, xpl, k.Cp, 0};
       ce_pairs(d, k.wp, k.xp);
       d.ksteps = k.Cp / kCeBK; d.split = 1; d.v0 = 0; d.p0 = p0;
-      d.part = (float2*)(ws + k.o_part); d.part_stride = (size_t)k.sb;
-      if (int e = ce_gemm<CE_STATS, false, false>(d, k.Vp, pn, st, "class_ce_stats")) return e;
-      MS_LAUNCH(ce_join_kernel, dim3((unsigned)(pn / 64)), dim3(1024), 0, st, (const float2*)d.part, ce_big(k.Vp, pn, 1) ? k.nparts / 2 : k.nparts, d.part_stride, zl, lab, lse, a.lse, a.nll,
+      d.part = (float2*)(ws + k.o_part); d.part_stride = (size_t)pn;
+      const CeTile tile = ce_tile<CE_STATS>(a.V, std::min<long>(pn, k.P - p0), 1, k.Vp, pn);
+      if (int e = ce_gemm<CE_STATS, false, false>(d, tile, st, "class_ce_stats")) return e;
+      MS_LAUNCH(ce_join_kernel, dim3((unsigned)(pn / 64)), dim3(1024), 0, st, (const float2*)d.part, tile.mt * 2, d.part_stride, zl, lab, lse, a.lse, a.nll,
                 (double*)(ws + k.o_lsum), p0, k.P, need_grad ? rg : CeRowGrad{});
       if (int e = check_launch("class_ce_join")) return e;
     }
@@ -707,39 +721,41 @@ static int ce_run(const CeArgs& a, const char* who) {
       const size_t gpl = (size_t)k.pb * k.vb;
       d.g = G; d.g_plane = gpl; d.g_ld = k.vb;
       d.dbpart = a.db != nullptr ? f32(k.o_db) : nullptr; d.db_stride = k.vb;
-      if (k.gpl == 2) { if (int e = ce_gemm<CE_GRAD2, false, false>(d, vn, pn, st, "class_ce_grad")) return e; }
-      else { if (int e = ce_gemm<CE_GRAD, false, false>(d, vn, pn, st, "class_ce_grad")) return e; }
-      const int rows = (int)std::min<long>(pn, k.P - p0), vr = std::max(0, std::min(vn, a.V - v0));
+      const int rows = (int)std::min<long>(pn, k.P - p0), vr = std::min(vn, a.V - v0);      // (never empty: the padding is less than a piece's granule)
+      const CeTile tile = ce_tile<CE_GRAD>(vr, rows, 1, vn, pn);
+      if (k.gpl == 2) { if (int e = ce_gemm<CE_GRAD2, false, false>(d, tile, st, "class_ce_grad")) return e; }
+      else { if (int e = ce_gemm<CE_GRAD, false, false>(d, tile, st, "class_ce_grad")) return e; }
       CeSums sums{};
       sums.scal = scal;
-      if (a.db != nullptr && vr > 0) {
-        sums.dbpart = f32(k.o_db); sums.dbn = pn / 128 * 2; sums.dbstride = (size_t)k.vb; sums.db = a.db; sums.dbfirst = p0 == 0; sums.dbV = vr; sums.dbv0 = v0;
+      if (a.db != nullptr) {
+        sums.dbpart = f32(k.o_db); sums.dbn = tile.nt * 2; sums.dbstride = (size_t)k.vb; sums.db = a.db; sums.dbfirst = p0 == 0; sums.dbV = vr; sums.dbv0 = v0;
         sums.dbblocks = cdiv(vr, 64);
       }
       if (a.dh != nullptr) {        // dh^T [channels][pixels] = w^T G^T, or dh [rows][channels] = G w where the channels are neighbours
         CeGemm o{};
         const CeOperand ow{w + (size_t)v0 * k.Cp, wpl, k.Cp, k.Cp}, og{G, gpl, k.vb, 0};
         const int pw = hb ? 1 : k.wp, pg = hb ? 1 : 2;
-        o.ksteps = vn / kCeBK; o.split = std::min(k.split_x, std::max(1, o.ksteps / 8));
+        if (rows_form) ce_pairs(o, pg, pw); else ce_pairs(o, pw, pg);
+        o.ksteps = cdiv(vr, kCeBK); o.split = std::min(k.split_x, std::max(1, o.ksteps * o.nseg / kCeDeep));
         o.out = f32(k.o_px); o.out_split = (size_t)cp * k.pb;
         if (rows_form) {
-          o.a = og; o.b = ow; ce_pairs(o, pg, pw); o.out_ld = (int)cp;
-          if (int e = ce_gemm<CE_OUT, false, true>(o, pn, (int)cp, st, "class_ce_dh")) return e;
+          o.a = og; o.b = ow; o.out_ld = (int)cp;
+          if (int e = ce_gemm<CE_OUT, false, true>(o, ce_tile<CE_OUT>(rows, a.C, o.split, pn, cp), st, "class_ce_dh")) return e;
         } else {
-          o.a = ow; o.b = og; ce_pairs(o, pw, pg); o.out_ld = k.pb;
-          if (int e = ce_gemm<CE_OUT, true, false>(o, (int)cp, pn, st, "class_ce_dh")) return e;
+          o.a = ow; o.b = og; o.out_ld = k.pb;
+          if (int e = ce_gemm<CE_OUT, true, false>(o, ce_tile<CE_OUT>(a.C, rows, o.split, cp, pn), st, "class_ce_dh")) return e;
         }
         CeSum& q = sums.h;
         q = CeSum{o.out, o.out_split, o.out_ld, o.split, fx, hb ? f32(k.o_ax) : (float*)a.dh, a.dh, v0 == 0, v0 + vn >= k.Vp, rows_form ? rows : a.C, rows_form ? a.C : rows, p0, a.HW, a.C, 0, 0};
         q.rblocks = cdiv(q.rows, 4); q.blocks = q.rblocks * std::min(cdiv(q.cols, 64), rows_form ? 4 : 64);
       }
-      if (a.dw != nullptr && vr > 0) {        // dw [classes][channels] = G^T h
+      if (a.dw != nullptr) {        // dw [classes][channels] = G^T h
         CeGemm o{};
         o.a = CeOperand{G, gpl, k.vb, k.vb}; o.b = CeOperand{x + (size_t)p0 * k.Cp, xpl, k.Cp, k.Cp};
         ce_pairs(o, wb ? 1 : 2, wb ? 1 : k.xp);
-        o.ksteps = pn / kCeBK; o.split = std::min(k.split_w, std::max(1, o.ksteps / 8));
+        o.ksteps = cdiv(rows, kCeBK); o.split = std::min(k.split_w, std::max(1, o.ksteps * o.nseg / kCeDeep));
         o.out = f32(k.o_pw); o.out_ld = (int)cp; o.out_split = (size_t)k.vb * cp;
-        if (int e = ce_gemm<CE_OUT, true, true>(o, vn, (int)cp, st, "class_ce_dw")) return e;
+        if (int e = ce_gemm<CE_OUT, true, true>(o, ce_tile<CE_OUT>(vr, a.C, o.split, vn, cp), st, "class_ce_dw")) return e;
         CeSum& q = sums.w;
         q = CeSum{o.out, o.out_split, o.out_ld, o.split, fw, wb ? f32(k.o_aw) : (float*)a.dw, a.dw, p0 == 0, p0 + pn >= k.Pp, vr, a.C, (long)v0, 1, a.C, 0, 0};
         q.rblocks = cdiv(q.rows, 4); q.blocks = q.rblocks * std::min(cdiv(q.cols, 64), 4);
