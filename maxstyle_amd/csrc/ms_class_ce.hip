@@ -180,7 +180,13 @@ __global__ __launch_bounds__(1024) void ce_scalars_kernel(const double* __restri
   if (rowmax == nullptr) return;
   int er = -100000, ew = -100000;
   for (int i = threadIdx.x; i < nrow; i += 1024) er = max(er, rowmax[i]);
-  for (int v = threadIdx.x; v < V; v += 1024) ew = max(ew, (int)(__float_as_uint(fw[v]) >> 23) - 127);
+#pragma unroll 4
+  for (int v = threadIdx.x * 4; v < V; v += 4096) {        // (padded to whole tiles)
+    const float4 f = *reinterpret_cast<const float4*>(fw + v);
+    const float ff[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) if (v + k < V) ew = max(ew, (int)(__float_as_uint(ff[k]) >> 23) - 127);
+  }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) { er = max(er, __shfl_xor(er, off, 64)); ew = max(ew, __shfl_xor(ew, off, 64)); }
   __syncthreads();
@@ -299,10 +305,11 @@ __device__ __forceinline__ ms_h8 ce_frag(const _Float16* tile, int mn, int ks, i
 }
 
 // One BM x BN tile, (BM / WM) x (BN / WN) per wave, LDS double-buffered: slab t + 1 is on its way while slab t is multiplied; one barrier a slab.
-template <int BM, int BN, int WM, int WN, bool ACOL, bool BCOL, int EPI>
+template <int BM, int BN, int WM, int WN, int ST, bool ACOL, bool BCOL, int EPI>
 __global__ __launch_bounds__(WM * WN * 64) void ce_gemm_kernel(CeGemm g) {
   constexpr int NW = WM * WN, TM = BM / WM, TN = BN / WN, MI = TM / 16, NJ = TN / 16;
-  __shared__ __attribute__((aligned(1024))) _Float16 sm[2][(BM + BN) * kCeBK];
+  static_assert((ST & (ST - 1)) == 0, "slab t lies in buffer t mod ST");
+  __shared__ __attribute__((aligned(1024))) _Float16 sm[ST][(BM + BN) * kCeBK];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q = lane >> 4, li = lane & 15;
   const int wm = wave / WN, wn = wave % WN;
   // Tiles of one XCD (workgroups are dealt to the 8 of them in turn) are neighbours: they share operand panels in that XCD's L2.
@@ -328,18 +335,21 @@ __global__ __launch_bounds__(WM * WN * 64) void ce_gemm_kernel(CeGemm g) {
   const unsigned lds0 = ms_lds_addr(&sm[0][0]);
   auto stage = [&](int t) {
     const int seg = t / g.ksteps, kk = t - seg * g.ksteps;
-    const unsigned buf = lds0 + (unsigned)(t & 1) * (unsigned)((BM + BN) * kCeBK * 2);
+    const unsigned buf = lds0 + (unsigned)(t & (ST - 1)) * (unsigned)((BM + BN) * kCeBK * 2);
     const _Float16* a = g.a.p + (size_t)g.pa[seg] * g.a.plane + (ACOL ? (size_t)kk * kCeBK * g.a.ld : (size_t)m0 * g.a.ld + (size_t)kk * kCeBK);
     const _Float16* b = g.b.p + (size_t)g.pb[seg] * g.b.plane + (BCOL ? (size_t)kk * kCeBK * g.b.ld : (size_t)n0 * g.b.ld + (size_t)kk * kCeBK);
     ce_stage<BM, ACOL, NW>(g.a, a, m0, wave, lane, buf);
     ce_stage<BN, BCOL, NW>(g.b, b, n0, wave, lane, buf + BM * kCeBK * 2);
   };
-  if (k0 < k1) stage(k0);
+  constexpr int kLoads = (BM + BN) * kCeBK * 2 / 1024 / NW;         // DMA instructions of a slab and wave
+#pragma unroll
+  for (int t = 0; t < ST - 1; ++t) if (k0 + t < k1) stage(k0 + t);
   for (int t = k0; t < k1; ++t) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();                    // slab t has landed for every wave, and nobody reads the buffer that slab t + 1 goes to
-    if (t + 1 < k1) stage(t + 1);
-    const _Float16* sa = &sm[t & 1][0];
+    if (ST > 2 && t + ST - 2 < k1) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kLoads * (ST - 2)) : "memory");      // the ST - 2 slabs behind t may be on their way
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();                    // slab t has landed for every wave, and nobody reads the buffer that slab t + ST - 1 goes to
+    if (t + ST - 1 < k1) stage(t + ST - 1);
+    const _Float16* sa = &sm[t & (ST - 1)][0];
     const _Float16* sb = sa + BM * kCeBK;
     // All fragments of the slab first, then its products in one run at raised priority: the other workgroup's (wave's) reads and DMA fill the gaps (1163 -> 1115 us for
     // 6400 rows x 512 channels x 32768 classes).  A ring of four slabs of 32 with counted waits was slower (1298: a barrier per 32).
@@ -508,6 +518,7 @@ __device__ __forceinline__ void ce_sum(const CeSum& a, int id, const int* scal, 
   for (int c = (id / a.rblocks) * 64 + lane; c < a.cols; c += ny * 64) {
     const float* src = a.part + (size_t)row * a.ld + c;
     float s = 0.f;
+#pragma unroll 8
     for (int k = 0; k < a.split; ++k) s += src[k * a.out_split];
     size_t dst;
     if (planes) {
@@ -620,12 +631,12 @@ static int ce_gemm(CeGemm g, const CeTile& c, hipStream_t st, const char* what) 
   const dim3 grid((unsigned)((long)g.mt * g.nt * g.split));
   if constexpr (EPI == CE_STATS || EPI == CE_OUT) {
     if (c.t == 256) {
-      MS_LAUNCH((ce_gemm_kernel<256, 256, 2, 4, ACOL, BCOL, EPI>), grid, dim3(512), 0, st, g);
+      MS_LAUNCH((ce_gemm_kernel<256, 256, 2, 4, 2, ACOL, BCOL, EPI>), grid, dim3(512), 0, st, g);
       return check_launch(what);
     }
   }
-  if (c.t == 128) MS_LAUNCH((ce_gemm_kernel<128, 128, 2, 2, ACOL, BCOL, EPI>), grid, dim3(256), 0, st, g);
-  else MS_LAUNCH((ce_gemm_kernel<64, 64, 2, 2, ACOL, BCOL, EPI>), grid, dim3(256), 0, st, g);
+  if (c.t == 128) MS_LAUNCH((ce_gemm_kernel<128, 128, 2, 2, 2, ACOL, BCOL, EPI>), grid, dim3(256), 0, st, g);
+  else MS_LAUNCH((ce_gemm_kernel<64, 64, 2, 2, 4, ACOL, BCOL, EPI>), grid, dim3(256), 0, st, g);
   return check_launch(what);
 }
 static void ce_pairs(CeGemm& g, int a, int b) {       // planes of the two operands -> products
