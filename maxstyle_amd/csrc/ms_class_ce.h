@@ -38,16 +38,19 @@ __device__ __forceinline__ void ce_split(float x, _Float16& hi, _Float16& lo) {
   lo = (_Float16)(x - (float)hi);
 }
 
-// ... of eight at once (conversions in pairs)
+// ... of eight at once: conversions in pairs, and x - hi as one multiply-add that reads the half-precision operand as it is (the factor -1 is hidden from the compiler, which
+// would make a conversion and a subtraction of it; 104 classes x 16 channels x 1 M pixels 168 -> 163 us)
 typedef _Float16 ms_h2 __attribute__((ext_vector_type(2)));
 typedef float ms_f2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void ce_split8(ms_f4 a, ms_f4 b, ms_h8& hi, ms_h8& lo) {
   union { ms_h2 p[4]; ms_h8 h; } H, L;
+  float neg1 = -1.f;
+  asm("" : "+s"(neg1));
   const ms_f2 v[4] = {{a[0], a[1]}, {a[2], a[3]}, {b[0], b[1]}, {b[2], b[3]}};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     H.p[i] = __builtin_convertvector(v[i], ms_h2);
-    const ms_f2 r = {v[i][0] - (float)H.p[i][0], v[i][1] - (float)H.p[i][1]};
+    const ms_f2 r = {__builtin_fmaf((float)H.p[i][0], neg1, v[i][0]), __builtin_fmaf((float)H.p[i][1], neg1, v[i][1])};
     L.p[i] = __builtin_convertvector(r, ms_h2);
   }
   hi = H.h; lo = L.h;

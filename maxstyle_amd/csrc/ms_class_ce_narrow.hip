@@ -130,6 +130,7 @@ struct CnArgs {
   void* dh; double* lsum;
   float *fx, *lse2, *gp; int* lab;          // what the class pass needs of every row (NULL: it does not run)
   long P; int C, HW, V, nch, w_vec;
+  int full;                                 // C is the kernel's full width and h spans less than 4 GB: addresses are a scalar base and a 32-bit offset
 };
 
 // The running maximum m is moved only when a logit exceeds it by more than kCnSlack (in log2), for a whole wave at once: e = 2^(kCnTop + z - m) then stays below 2^15 in
@@ -159,16 +160,26 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
   const int P = (int)a.P;
   // every load unconditional, at a clamped address, and all of them in flight together (loads behind branches wait for one another: 20 us more at 400k pixels x 64 channels)
   float v[NJ][KN][KF];
+  unsigned off[NJ];                    // of the pixel's first channel, in bytes (`full`)
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
     const int p = min(pw + j * 16, P - 1), n = p / a.HW;
-    const size_t base = (size_t)n * a.C * a.HW + (size_t)(p - n * a.HW);
     const int64_t lb = a.labels[p];
     lab[j] = (lb >= 0 && lb < a.V && pw + j * 16 < P) ? (int)lb : -1;
+    off[j] = ((unsigned)n * (unsigned)a.C * (unsigned)a.HW + (unsigned)(p - n * a.HW)) * (unsigned)sizeof(HT);
+    if (a.full) {
+      const unsigned at = off[j] + (unsigned)(q * KF) * (unsigned)a.HW * (unsigned)sizeof(HT);
 #pragma unroll
-    for (int ks = 0; ks < KN; ++ks)
+      for (int ks = 0; ks < KN; ++ks)
 #pragma unroll
-      for (int k = 0; k < KF; ++k) v[j][ks][k] = IO::ld1(a.h, base + (size_t)min(ks * 32 + q * KF + k, a.C - 1) * a.HW);
+        for (int k = 0; k < KF; ++k) v[j][ks][k] = IO::ld1((const char*)a.h + (size_t)(ks * 32 + k) * a.HW * sizeof(HT) + at, 0);
+    } else {
+      const size_t base = (size_t)n * a.C * a.HW + (size_t)(p - n * a.HW);
+#pragma unroll
+      for (int ks = 0; ks < KN; ++ks)
+#pragma unroll
+        for (int k = 0; k < KF; ++k) v[j][ks][k] = IO::ld1(a.h, base + (size_t)min(ks * 32 + q * KF + k, a.C - 1) * a.HW);
+    }
   }
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
@@ -197,11 +208,13 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
       }
   }
 
+  int key[NJ];                         // the 32 classes that the label lies in, for the lane of the four that has it
   float m[NJ], l[NJ], zl[NJ];          // in units of log2; m is the same in the four lanes of a pixel, l and zl are each lane's part
   ms_f4 o[CT][NJ];
   float scale = 1.f;                   // 2^e of the chunk that o is measured in
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
+    key[j] = lab[j] >= 0 && ((lab[j] >> 2) & 3) == q ? lab[j] >> 5 : -1;
     m[j] = -__builtin_inff(); l[j] = 0.f; zl[j] = 0.f;
     if (!online) m[j] = pw + j * 16 < P ? a.lse_in[pw + j * 16] * kLog2e : 0.f;
 #pragma unroll
@@ -268,21 +281,23 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
         bool grow = false, here = false;
         float mx[NJ];
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) here |= (lab[j] >> 5) == t * 2 + h2;
-        if (__any(here)) {             // some pixel's label is among these 32 classes (seldom so in a label map)
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) {
-            const int y = lab[j] - (t * kCnClasses + h2 * 32 + q * 4);
-#pragma unroll
-            for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-              for (int r = 0; r < 4; ++r) zl[j] = y == tt * 16 + r ? s[tt][j][r] : zl[j];
-          }
-        }
-#pragma unroll
         for (int j = 0; j < NJ; ++j) {
           mx[j] = fmaxf(fmaxf(fmaxf(s[0][j][0], s[0][j][1]), fmaxf(s[0][j][2], s[0][j][3])), fmaxf(fmaxf(s[1][j][0], s[1][j][1]), fmaxf(s[1][j][2], s[1][j][3])));
           grow |= mx[j] > m[j] + kCnSlack;
+          here |= key[j] == t * 2 + h2;
+        }
+        if (__any(here)) {             // some pixel's label is among these 32 classes (seldom so in a label map): chosen by its bits 0, 1 and 4
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) {
+            float z[2];
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt) {
+              const float z0 = (lab[j] & 1) != 0 ? s[tt][j][1] : s[tt][j][0], z1 = (lab[j] & 1) != 0 ? s[tt][j][3] : s[tt][j][2];
+              z[tt] = (lab[j] & 2) != 0 ? z1 : z0;
+            }
+            const float zz = (lab[j] & 16) != 0 ? z[1] : z[0];
+            zl[j] = key[j] == t * 2 + h2 ? zz : zl[j];
+          }
         }
         if (__any(grow)) {
 #pragma unroll
@@ -361,8 +376,7 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
       }
     }
     if (DH) {
-      const int pc = min(p, P - 1), n = pc / a.HW;
-      const size_t base = (size_t)n * a.C * a.HW + (size_t)(pc - n * a.HW), wrow = (size_t)max(lab[j], 0) * a.C;
+      const size_t wrow = (size_t)max(lab[j], 0) * a.C;
       const float f = scale * fac;
       float wl[CT][4];                    // the label's weights, rounded as the products' were (16 bytes a lane: 4-byte loads from 64 rows at once cost 100 us a million pixels)
       if (a.w_vec) {
@@ -389,11 +403,26 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
 #pragma unroll
       for (int c = 0; c < CT; ++c)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int cc = c * 16 + q * 4 + r;
-          const float d = gp == 0.f ? 0.f : gp * (o[c][j][r] * f - wl[c][r]);
-          if (cc < a.C && p < P) IO::st1(a.dh, base + (size_t)cc * a.HW, d);
+        for (int r = 0; r < 4; ++r) wl[c][r] = gp == 0.f ? 0.f : gp * (o[c][j][r] * f - wl[c][r]);
+      if (a.full) {
+        const unsigned at = off[j] + (unsigned)(q * 4) * (unsigned)a.HW * (unsigned)sizeof(HT);
+        if (p < P) {
+#pragma unroll
+          for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) IO::st1((char*)a.dh + (size_t)(c * 16 + r) * a.HW * sizeof(HT) + at, 0, wl[c][r]);
         }
+      } else {
+        const int pc = min(p, P - 1), n = pc / a.HW;
+        const size_t base = (size_t)n * a.C * a.HW + (size_t)(pc - n * a.HW);
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int cc = c * 16 + q * 4 + r;
+            if (cc < a.C && p < P) IO::st1(a.dh, base + (size_t)cc * a.HW, wl[c][r]);
+          }
+      }
     }
   }
   if (a.lsum != nullptr) {
@@ -724,6 +753,7 @@ static int cn_run(const CeArgs& a, const CnPlan& k) {
   p.nll = a.nll; p.lse_out = a.lse; p.lse_in = a.lse_in; p.grad = a.grad; p.scale_dev = a.scale_dev; p.sign = a.sign; p.mean_valid = a.mean_valid; p.drop = need_grad ? 1 : 0;
   p.dh = a.dh; p.lsum = a.loss != nullptr ? (double*)(ws + k.o_lsum) : nullptr;
   if (need_dw) { p.fx = (float*)(ws + k.o_fx); p.lse2 = (float*)(ws + k.o_lse); p.gp = (float*)(ws + k.o_gp); p.lab = (int*)(ws + k.o_lab); }
+  p.full = a.C == CnW<KS>::kW && (size_t)a.N * a.HW * a.C * sizeof(HT) <= 0xFFFFFFFFu;
   p.w_vec = a.C % 4 == 0 && (reinterpret_cast<uintptr_t>(a.w) & (4 * sizeof(WT) - 1)) == 0;
   p.P = k.P; p.C = a.C; p.HW = a.HW; p.V = a.V; p.nch = k.nch;
   const dim3 grid((unsigned)k.wgs), block(256);
