@@ -599,7 +599,7 @@ MS_STABLE int ms_class_ce_bwd(const void* h, const void* w, const float* b, cons
  *                        output: only its signs are read) or scale x' + shift when ref_q == NULL; part2 [C][ms_act8_bwd_parts()][2] = {sum g', sum g'(x' - mean)} for
  *                        ms_bn_bwd_full; gout (g', may alias gin) and uout (x') may be NULL.  coef4 must be the record the checkpoint was made with.
  *   ms_act8_bn_act_bwd   the whole backward of BatchNorm (batch statistics) + LeakyReLU: du, dgamma, dbeta (may not be NULL; du may alias g).
- * Deterministic; any alignment and any HW. */
+ * Deterministic; any alignment and any HW; up to 2^26 runs of 1024 elements inside the planes, the backward entries up to 2^24 of up to 16384. */
 MS_STABLE int ms_act8_block(void);
 MS_STABLE int ms_act8_pack(const float* x, const float* coef4, int8_t* q, float* s, int N, int C, int HW, void* stream);
 MS_STABLE int ms_act8_unpack(const int8_t* q, const float* s, const float* coef4, float* x, int N, int C, int HW, void* stream);

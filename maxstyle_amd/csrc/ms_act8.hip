@@ -321,6 +321,12 @@ static int a8_check(int N, int C, int HW, const char* who) {
   if ((long long)N * C * cdiv(HW, 1024) >= (1LL << 31) - 8 || HW > 0x7FFFFFFF - 32768) { set_error("%s: more than 2^31 segments of 1024 elements", who); return MS_ERR_INVALID; }
   return MS_OK;
 }
+// A launch holds less than 2^32 threads: 2^24 segments of 256 threads, 2^26 items of one wave.  (Planes of a few elements reach it first.)
+static int a8_launchable(long long groups, long long most, const char* who) {
+  if (groups < most) return MS_OK;
+  set_error("%s: more than 2^24 segments (or 2^26 runs of 1024 elements) of the planes", who);
+  return MS_ERR_INVALID;
+}
 static int a8_aligned(const float* coef4, const void* part, const char* who) {
   if (!aligned16(coef4) || (reinterpret_cast<uintptr_t>(part) & 7u)) { set_error("%s: coef4 must be 16-byte aligned, partial sums 8-byte", who); return MS_ERR_ALIGN; }
   return MS_OK;
@@ -330,6 +336,7 @@ static bool a8_al(const void* p, unsigned n) { return (reinterpret_cast<uintptr_
 template <typename AT>
 static int act8_pack_impl(const void* x, const float* coef4, int8_t* q, float* s, int N, int C, int HW, void* stream) {
   if (int e = a8_check(N, C, HW, "ms_act8_pack")) return e;
+  if (int e = a8_launchable((long long)N * C * cdiv(cdiv(HW, kA8Block), kPackBlocks), 1LL << 26, "ms_act8_pack")) return e;
   if (x == nullptr || q == nullptr || s == nullptr) { set_error("ms_act8_pack: null pointer"); return MS_ERR_INVALID; }
   if (int e = a8_aligned(coef4, nullptr, "ms_act8_pack")) return e;
   const int nb = cdiv(HW, kA8Block), items = cdiv(nb, kPackBlocks), total = N * C * items;
@@ -342,6 +349,7 @@ static int act8_pack_impl(const void* x, const float* coef4, int8_t* q, float* s
 template <typename AT>
 static int act8_unpack_impl(const int8_t* q, const float* s, const float* coef4, void* x, int N, int C, int HW, void* stream) {
   if (int e = a8_check(N, C, HW, "ms_act8_unpack")) return e;
+  if (int e = a8_launchable((long long)N * C * cdiv(cdiv(HW, kA8Block), kPackBlocks), 1LL << 26, "ms_act8_unpack")) return e;
   if (x == nullptr || q == nullptr || s == nullptr) { set_error("ms_act8_unpack: null pointer"); return MS_ERR_INVALID; }
   if (int e = a8_aligned(coef4, nullptr, "ms_act8_unpack")) return e;
   const int nb = cdiv(HW, kA8Block), items = cdiv(nb, kPackBlocks), total = N * C * items;
@@ -364,6 +372,7 @@ static int act8_bwd_reduce_impl(const void* gin, const int8_t* ref, const int8_t
   if (gin == nullptr || q == nullptr || s == nullptr || coef4 == nullptr || part2 == nullptr) { set_error("ms_act8_bwd_reduce: null pointer"); return MS_ERR_INVALID; }
   if (int e = a8_aligned(coef4, part2, "ms_act8_bwd_reduce")) return e;
   const A8Split sp = a8_split((long)N * C, HW);
+  if (int e = a8_launchable((long long)N * C * sp.S, 1LL << 24, "ms_act8_bwd_reduce")) return e;
   dim3 grid(N * C * sp.S), block(kA8Threads);
   const int nb = cdiv(HW, kA8Block);
   hipStream_t st = (hipStream_t)stream;
@@ -393,6 +402,7 @@ static int act8_bn_act_bwd_impl(const void* g, const int8_t* ref, const int8_t* 
     else MS_LAUNCH((act8_bwd_one_kernel<AT, false>), dim3(C), b1, 0, st, g, ref, q, s, (const float4*)coef4, du, dgamma, dbeta, C, HW, nb, N, slope);
     return check_launch("act8_bwd_one");
   }
+  if (int e = a8_launchable((long long)N * C * sp.S, 1LL << 24, "ms_act8_bn_act_bwd")) return e;
   const dim3 block(kA8Threads), grid(N * C * sp.S);
 #define A8_ARGS(PART) st, g, ref, q, s, (const float4*)coef4, PART
   if (vec) MS_LAUNCH((act8_bwd_reduce_kernel<AT, true, false>), grid, block, 0, A8_ARGS(nullptr), nullptr, (float2*)ws, C, HW, nb, sp.seg, sp.S, N, slope);

@@ -78,8 +78,9 @@ __device__ __forceinline__ void ce_pack_row(const CePack& a, int r) {
 template <typename HT, typename WT, bool VEC>
 __global__ __launch_bounds__(256) void ce_pack_rows_kernel(CePack w, CePack h, int wblocks) {
   const int wave = threadIdx.x >> 6;
-  if ((int)blockIdx.x < wblocks) ce_pack_row<WT, VEC>(w, (int)blockIdx.x * 4 + wave);
-  else ce_pack_row<HT, VEC>(h, ((int)blockIdx.x - wblocks) * 4 + wave);
+  const int id = (int)(blockIdx.y * gridDim.x + blockIdx.x);
+  if (id < wblocks) ce_pack_row<WT, VEC>(w, id * 4 + wave);
+  else ce_pack_row<HT, VEC>(h, (id - wblocks) * 4 + wave);
 }
 
 // h [N][C][HW], HW > 1 -> the same packed rows.  A workgroup takes 64 pixels: a wave reads 64 neighbouring pixels of a channel at a time and writes 8 channels of each.
@@ -89,7 +90,8 @@ __global__ __launch_bounds__(1024) void ce_pack_planes_kernel(const void* __rest
   using IO = ActIO<HT>;
   __shared__ unsigned smax[16][64];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const long p = (long)blockIdx.x * 64 + lane;
+  const long p = ((long)blockIdx.y * gridDim.x + blockIdx.x) * 64 + lane;
+  if (p >= Pp) return;                 // (whole workgroups: Pp is a multiple of 256)
   int y = -1;
   if (p < P) { const int64_t l = labels[p]; y = (l >= 0 && l < classes) ? (int)l : -1; }
   if (wave == 0) lab32[p] = y;
@@ -607,6 +609,9 @@ static CePlan ce_plan(int N, int C, int V, int HW, int types, bool grad) {
   return k;
 }
 
+// n workgroups over two axes: more than 2^32 threads of one axis cannot be launched (2^26 rows, one wave each)
+static dim3 ce_grid(long n) { return n <= (1 << 20) ? dim3((unsigned)n) : dim3(1 << 20, (unsigned)((n + (1 << 20) - 1) >> 20)); }
+
 static int ce_check(int N, int C, int V, int HW, int types, const char* who) {
   if (N < 1 || C < 1 || V < 1 || HW < 1 || types < 0 || types > 3) { set_error("%s: invalid shape", who); return MS_ERR_INVALID; }
   if (C > 8192 || V > (1 << 20) || (long long)N * HW > (1LL << 30)) { set_error("%s: supported up to 8192 channels, 2^20 classes, 2^30 rows", who); return MS_ERR_INVALID; }
@@ -667,7 +672,7 @@ static int ce_run(const CeArgs& a, const char* who) {
     const CePack ph{a.h, nullptr, a.labels, a.V, drop, x, xpl, fx, nullptr, lab, a.N, (int)k.Pp, a.C, k.Cp};
     const bool vec = a.C % 8 == 0 && aligned16(a.w) && (!rows_form || aligned16(a.h));
     const int wblocks = k.Vp / 4;
-    const dim3 grid((unsigned)(wblocks + (rows_form ? k.Pp / 4 : 0))), block(256);
+    const dim3 grid = ce_grid(wblocks + (rows_form ? k.Pp / 4 : 0)), block(256);
     if (hb && wb && vec) MS_LAUNCH((ce_pack_rows_kernel<ms_bf16, ms_bf16, true>), grid, block, 0, st, pw, ph, wblocks);
     else if (hb && wb) MS_LAUNCH((ce_pack_rows_kernel<ms_bf16, ms_bf16, false>), grid, block, 0, st, pw, ph, wblocks);
     else if (hb && vec) MS_LAUNCH((ce_pack_rows_kernel<ms_bf16, float, true>), grid, block, 0, st, pw, ph, wblocks);
@@ -679,7 +684,7 @@ static int ce_run(const CeArgs& a, const char* who) {
     if (int e = check_launch("class_ce_pack")) return e;
   }
   if (!rows_form) {
-    const dim3 gx((unsigned)(k.Pp / 64));
+    const dim3 gx = ce_grid(k.Pp / 64);
     if (hb) MS_LAUNCH((ce_pack_planes_kernel<ms_bf16, 1>), gx, dim3(1024), 0, st, a.h, a.labels, a.V, drop, x, xpl, fx, lab, k.P, k.Pp, a.C, k.Cp, a.HW);
     else MS_LAUNCH((ce_pack_planes_kernel<float, 2>), gx, dim3(1024), 0, st, a.h, a.labels, a.V, drop, x, xpl, fx, lab, k.P, k.Pp, a.C, k.Cp, a.HW);
     if (int e = check_launch("class_ce_pack")) return e;

@@ -450,6 +450,8 @@ def _class_ce_args(h, w, b, labels):
         raise ValueError(f"class_ce: labels must be {(h.shape[0],) + tuple(h.shape[2:])}; got {tuple(labels.shape)}")
     if h.numel() == 0 or w.numel() == 0:
         raise ValueError("class_ce: empty input")
+    if h.shape[1] > 8192 or w.shape[0] > 1 << 20 or labels.numel() > 1 << 30:
+        raise ValueError("class_ce: supported up to 8192 channels, 2^20 classes, 2^30 rows")
     for t in (w, b, labels):
         if t is not None and t.device != h.device:
             raise ValueError("class_ce: all tensors must be on one device")
@@ -538,6 +540,8 @@ def _act8_dims(shape, who):
         HW *= int(n)
     if N * C * HW == 0:
         raise ValueError(f"{who}: empty input")
+    if max(N, C, HW) >= 1 << 31:
+        raise ValueError(f"{who}: N, C and the plane hold less than 2^31 elements each")
     return N, C, HW
 
 

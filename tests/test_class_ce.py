@@ -46,3 +46,14 @@ def test_c_entries_refuse_before_any_launch():
     off = p + 8 - p % 16 if p % 16 <= 8 else p + 4            # a record that is not 16-byte aligned
     assert off % 16 and lib.ms_act8_pack(p, off, p, p, 1, 1, 1, 0) == -2 and lib.ms_act8_unpack(p, p, off, p, 1, 1, 1, 0) == -2
     assert lib.ms_act8_block() == ops.ACT8_BLOCK
+
+
+def test_sizes_that_no_launch_holds_are_refused():
+    buf = ctypes.create_string_buffer(4096)
+    p = ctypes.addressof(buf) + 15 & ~15
+    assert lib.ms_act8_pack(p, 0, p, p, 1 << 13, 1 << 13, 4, 0) == -1 and lib.ms_act8_unpack(p, p, 0, p, 1 << 13, 1 << 13, 4, 0) == -1
+    assert lib.ms_act8_bwd_reduce(p, 0, p, p, p, p, 0, p, 1 << 13, 1 << 11, 4, 0.2, 0) == -1
+    assert lib.ms_act8_bn_act_bwd(p, 0, p, p, p, p, p, p, 1 << 13, 1 << 11, 4, 0.2, p, 1 << 40, 0) == -1
+    with pytest.raises(ValueError, match="2\\^31"):
+        ops._act8_dims((1, 1, 1 << 16, 1 << 16), "act8_pack")
+    assert lib.ms_class_ce_ws_bytes(1 << 15, 8, 5, (1 << 15) + 1, 0, 1) == 0

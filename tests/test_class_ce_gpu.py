@@ -321,3 +321,54 @@ def test_unaligned_views():
     got = ops.class_ce(shift(h), shift(w), shift(b), shift(lab))
     for a, c in zip(want, got):
         assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("shape,V", [((1, 512), 700), ((2, 512, 16, 17), 900), ((130, 640), 9000), ((2, 64, 18, 20), 300), ((40, 16), 9)])
+def test_whatever_the_workspace_held(shape, V):
+    h, w, b, lab = make(shape, V, seed=21)
+    N, C = shape[:2]
+    nbytes = ops.lib.ms_class_ce_ws_bytes(N, C, V, lab.numel() // N, 0, 1)
+    got = []
+    for fill in (0, 255):                # 255: every float and half of it a NaN
+        block = torch.full((nbytes,), fill, dtype=torch.uint8, device="cuda")
+        del block                        # the caching allocator hands the block to the call
+        got.append(ops.class_ce(h, w, b, lab, mean_over="valid"))
+    for a, c in zip(*got):
+        assert torch.equal(a, c) and torch.isfinite(a).all()
+
+
+@pytest.mark.parametrize("images", [17, 33])
+def test_features_of_more_than_two_and_four_gigabytes(images):
+    g = torch.Generator(device="cuda").manual_seed(images)
+    shape, V = (images, 64, 1024, 1024), 7
+    h = torch.randn(shape, generator=g, device="cuda", dtype=B)
+    w = (torch.randn(V, 64, generator=g, device="cuda") / 8)
+    lab = torch.randint(0, V, (images, 1024, 1024), generator=g, device="cuda")
+    gr = torch.randn(lab.shape, generator=g, device="cuda")
+    nll, lse = ops.class_ce_fwd(h, w, None, lab)
+    dh = ops.class_ce_bwd(h, w, None, lab, lse, gr, need_dw=False)[0]
+    for i in (0, 15, 16, images - 1):
+        cut = (slice(i, i + 1), slice(None), slice(1016, 1024))
+        hc, lc, gc = h[cut].contiguous(), lab[i:i + 1, 1016:].contiguous(), gr[i:i + 1, 1016:].contiguous()
+        r = reference(hc, w, None, lc, gc.double().reshape(-1))
+        close(nll[i, 1016:].reshape(-1), r["nll"], 2 * r["dz"] + 16 * U32 * (r["lse"].abs() + r["nll"] + 1), "nll")
+        close(rows_of(dh[cut], 64), r["dh"], tolerances(r, B, F)[0], "dh")
+
+
+def test_more_rows_than_one_axis_of_a_launch_holds():
+    P, C, V = (1 << 26) + 300, 130, 5
+    g = torch.Generator(device="cuda").manual_seed(2)
+    h = torch.randn(P, C, generator=g, device="cuda", dtype=B)
+    w = (torch.randn(V, C, generator=g, device="cuda") / C ** 0.5).to(B)
+    b = torch.randn(V, generator=g, device="cuda") * 0.3
+    lab = torch.randint(0, V, (P,), generator=g, device="cuda")
+    gr = torch.randn(P, generator=g, device="cuda")
+    nll, lse = ops.class_ce_fwd(h, w, b, lab)
+    dh = ops.class_ce_bwd(h, w, b, lab, lse, gr, need_dw=False)[0]
+    for a in (0, (1 << 25) - 50, (1 << 26) - 50, P - 100):
+        s = slice(a, a + 100)
+        r = reference(h[s], w, b, lab[s], gr[s].double())
+        close(nll[s], r["nll"], 2 * r["dz"] + 16 * U32 * (r["lse"].abs() + r["nll"] + 1), "nll")
+        # the lowest step of G is that of the largest upstream gradient of all rows (at most 7 of a normal draw, times the largest feature, below 8)
+        low = 7 * 8 * 2.0 ** -36 / r["x"].abs().amax(1, keepdim=True).clamp_min(1e-30) * V * r["w"].abs().amax(0)
+        close(dh[s], r["dh"], tolerances(r, B, B)[0] + low, "dh")
