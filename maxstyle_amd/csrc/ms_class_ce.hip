@@ -308,14 +308,12 @@ __device__ __forceinline__ ms_h8 ce_frag(const _Float16* tile, int mn, int ks, i
 
 // One BM x BN tile, (BM / WM) x (BN / WN) per wave, LDS double-buffered: slab t + 1 is on its way while slab t is multiplied; one barrier a slab.
 template <int BM, int BN, int WM, int WN, int ST, bool ACOL, bool BCOL, int EPI>
-__global__ __launch_bounds__(WM * WN * 64) void ce_gemm_kernel(CeGemm g) {
+__device__ __forceinline__ void ce_gemm_tile(CeGemm g, int id, _Float16 (*sm)[(BM + BN) * kCeBK]) {
   constexpr int NW = WM * WN, TM = BM / WM, TN = BN / WN, MI = TM / 16, NJ = TN / 16;
   static_assert((ST & (ST - 1)) == 0, "slab t lies in buffer t mod ST");
-  __shared__ __attribute__((aligned(1024))) _Float16 sm[ST][(BM + BN) * kCeBK];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q = lane >> 4, li = lane & 15;
   const int wm = wave / WN, wn = wave % WN;
   // Tiles of one XCD (workgroups are dealt to the 8 of them in turn) are neighbours: they share operand panels in that XCD's L2.
-  int id = blockIdx.x;
   const int tiles = g.mt * g.nt * g.split, per = tiles >> 3;
   if (id < per * 8) id = (id & 7) * per + (id >> 3);
   const int sp = id / (g.mt * g.nt);
@@ -503,6 +501,19 @@ __global__ __launch_bounds__(WM * WN * 64) void ce_gemm_kernel(CeGemm g) {
       }
     }
   }
+}
+
+template <int BM, int BN, int WM, int WN, int ST, bool ACOL, bool BCOL, int EPI>
+__global__ __launch_bounds__(WM * WN * 64) void ce_gemm_kernel(CeGemm g) {
+  __shared__ __attribute__((aligned(1024))) _Float16 sm[ST][(BM + BN) * kCeBK];
+  ce_gemm_tile<BM, BN, WM, WN, ST, ACOL, BCOL, EPI>(g, blockIdx.x, sm);
+}
+// dh and dw of a piece in one launch, where both take tiles of T: the first nh workgroups dh (its operands as HROWS says), the others dw.
+template <int T, int ST, bool HROWS>
+__global__ __launch_bounds__(256) void ce_grads_kernel(CeGemm h, CeGemm w, int nh) {
+  __shared__ __attribute__((aligned(1024))) _Float16 sm[ST][2 * T * kCeBK];
+  if ((int)blockIdx.x < nh) ce_gemm_tile<T, T, 2, 2, ST, !HROWS, HROWS, CE_OUT>(h, blockIdx.x, sm);
+  else ce_gemm_tile<T, T, 2, 2, ST, true, true, CE_OUT>(w, (int)blockIdx.x - nh, sm);
 }
 
 // The sums behind a piece's products, one launch: db from G's epilogue, dh and dw from their K-splits (each a range of workgroups; any may be empty).
@@ -747,8 +758,10 @@ static int ce_run(const CeArgs& a, const char* who) {
         sums.dbpart = f32(k.o_db); sums.dbn = tile.nt * 2; sums.dbstride = (size_t)k.vb; sums.db = a.db; sums.dbfirst = p0 == 0; sums.dbV = vr; sums.dbv0 = v0;
         sums.dbblocks = cdiv(vr, 64);
       }
+      CeGemm gh{}, gw{};
+      CeTile th{}, tw{};
       if (a.dh != nullptr) {        // dh^T [channels][pixels] = w^T G^T, or dh [rows][channels] = G w where the channels are neighbours
-        CeGemm o{};
+        CeGemm& o = gh;
         const CeOperand ow{w + (size_t)v0 * k.Cp, wpl, k.Cp, k.Cp}, og{G, gpl, k.vb, 0};
         const int pw = hb ? 1 : k.wp, pg = hb ? 1 : 2;
         if (rows_form) ce_pairs(o, pg, pw); else ce_pairs(o, pw, pg);
@@ -756,25 +769,42 @@ static int ce_run(const CeArgs& a, const char* who) {
         o.out = f32(k.o_px); o.out_split = (size_t)cp * k.pb;
         if (rows_form) {
           o.a = og; o.b = ow; o.out_ld = (int)cp;
-          if (int e = ce_gemm<CE_OUT, false, true>(o, ce_tile<CE_OUT>(rows, a.C, o.split, pn, cp), st, "class_ce_dh")) return e;
+          th = ce_tile<CE_OUT>(rows, a.C, o.split, pn, cp);
         } else {
           o.a = ow; o.b = og; o.out_ld = k.pb;
-          if (int e = ce_gemm<CE_OUT, true, false>(o, ce_tile<CE_OUT>(a.C, rows, o.split, cp, pn), st, "class_ce_dh")) return e;
+          th = ce_tile<CE_OUT>(a.C, rows, o.split, cp, pn);
         }
         CeSum& q = sums.h;
         q = CeSum{o.out, o.out_split, o.out_ld, o.split, fx, hb ? f32(k.o_ax) : (float*)a.dh, a.dh, v0 == 0, v0 + vn >= k.Vp, rows_form ? rows : a.C, rows_form ? a.C : rows, p0, a.HW, a.C, 0, 0};
         q.rblocks = cdiv(q.rows, 4); q.blocks = q.rblocks * std::min(cdiv(q.cols, 64), rows_form ? 4 : 64);
       }
       if (a.dw != nullptr) {        // dw [classes][channels] = G^T h
-        CeGemm o{};
+        CeGemm& o = gw;
         o.a = CeOperand{G, gpl, k.vb, k.vb}; o.b = CeOperand{x + (size_t)p0 * k.Cp, xpl, k.Cp, k.Cp};
         ce_pairs(o, wb ? 1 : 2, wb ? 1 : k.xp);
         o.ksteps = cdiv(rows, kCeBK); o.split = std::min(k.split_w, std::max(1, o.ksteps * o.nseg / kCeDeep));
         o.out = f32(k.o_pw); o.out_ld = (int)cp; o.out_split = (size_t)k.vb * cp;
-        if (int e = ce_gemm<CE_OUT, true, true>(o, ce_tile<CE_OUT>(vr, a.C, o.split, vn, cp), st, "class_ce_dw")) return e;
+        tw = ce_tile<CE_OUT>(vr, a.C, o.split, vn, cp);
         CeSum& q = sums.w;
         q = CeSum{o.out, o.out_split, o.out_ld, o.split, fw, wb ? f32(k.o_aw) : (float*)a.dw, a.dw, p0 == 0, p0 + pn >= k.Pp, vr, a.C, (long)v0, 1, a.C, 0, 0};
         q.rblocks = cdiv(q.rows, 4); q.blocks = q.rblocks * std::min(cdiv(q.cols, 64), 4);
+      }
+      if (th.t == tw.t && th.t < 256) {
+        gh.mt = th.mt; gh.nt = th.nt; gw.mt = tw.mt; gw.nt = tw.nt;
+        const int nh = th.mt * th.nt * gh.split, n = nh + tw.mt * tw.nt * gw.split;
+        if (n > 0) {
+          if (th.t == 128 && rows_form) MS_LAUNCH((ce_grads_kernel<128, 2, true>), dim3(n), dim3(256), 0, st, gh, gw, nh);
+          else if (th.t == 128) MS_LAUNCH((ce_grads_kernel<128, 2, false>), dim3(n), dim3(256), 0, st, gh, gw, nh);
+          else if (rows_form) MS_LAUNCH((ce_grads_kernel<64, 4, true>), dim3(n), dim3(256), 0, st, gh, gw, nh);
+          else MS_LAUNCH((ce_grads_kernel<64, 4, false>), dim3(n), dim3(256), 0, st, gh, gw, nh);
+          if (int e = check_launch("class_ce_grads")) return e;
+        }
+      } else {
+        if (a.dh != nullptr) {
+          if (rows_form) { if (int e = ce_gemm<CE_OUT, false, true>(gh, th, st, "class_ce_dh")) return e; }
+          else { if (int e = ce_gemm<CE_OUT, true, false>(gh, th, st, "class_ce_dh")) return e; }
+        }
+        if (a.dw != nullptr) { if (int e = ce_gemm<CE_OUT, true, true>(gw, tw, st, "class_ce_dw")) return e; }
       }
       const int blocks = sums.dbblocks + sums.h.blocks + sums.w.blocks;
       if (blocks > 0) {
