@@ -221,7 +221,7 @@ __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict_
   __syncthreads();
   if (grp != 0) return;
   for (int k = 1; k < 16; ++k) ce_merge(m, l, sh[k][el].x, sh[k][el].y);
-  const float lg = __builtin_amdgcn_logf(l), ln2 = 0.693147180559945309f;      // (log2)
+  const float lg = ce_log2(l), ln2 = 0.693147180559945309f;      // (log2)
   float ls = m + lg;
   double acc = 0.0;
   if (rg.gp != nullptr) {

@@ -359,7 +359,7 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
       zl[j] += __shfl_xor(zl[j], 16, 64);             // (one lane of the four holds it, the others 0)
       zl[j] += __shfl_xor(zl[j], 32, 64);
       fac = 1.f / l[j];
-      const float lg = __builtin_amdgcn_logf(l[j]) - kCnTop;      // log2
+      const float lg = ce_log2(l[j], (int)kCnTop);
       lse2 = m[j] + lg;
       const float ln2 = 0.693147180559945309f, nll = lab[j] >= 0 ? ((m[j] - zl[j]) + lg) * ln2 : 0.f;
       if (q == 0 && p < P) {

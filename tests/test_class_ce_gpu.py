@@ -372,3 +372,13 @@ def test_more_rows_than_one_axis_of_a_launch_holds():
         # the lowest step of G is that of the largest upstream gradient of all rows (at most 7 of a normal draw, times the largest feature, below 8)
         low = 7 * 8 * 2.0 ** -36 / r["x"].abs().amax(1, keepdim=True).clamp_min(1e-30) * V * r["w"].abs().amax(0)
         close(dh[s], r["dh"], tolerances(r, B, B)[0] + low, "dh")
+
+
+@pytest.mark.parametrize("shape,V", [((1, 16, 60, 60), 5), ((4, 64, 30, 30), 700), ((4000, 136), 400)])
+def test_errors_of_rows_do_not_add_up(shape, V):
+    """The log-sums are off by single roundings that lie on both sides: their mean stays below what the exponential's and the logarithm's cut results leave (half a step of
+    [0, 1) each, 2 u32) and four standard deviations of the roundings (uniform, at most one step, 16 u32, of values in [8, 16), P of them)."""
+    h, w, b, lab = make(shape, V, seed=31, void=0.0)
+    lse = ops.class_ce_fwd(h, w, b, lab)[1].double().reshape(-1)
+    want = torch.logsumexp(rows_of(h.double(), shape[1]) @ w.double().T + b.double(), 1)
+    assert abs(float((lse - want).mean())) <= 2 * U32 + 4 * 16 * U32 / 12 ** 0.5 / lab.numel() ** 0.5
