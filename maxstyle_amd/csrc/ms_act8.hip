@@ -178,16 +178,16 @@ __global__ __launch_bounds__(kA8Threads) void act8_bwd_reduce_kernel(const void*
                                                                      const float* __restrict__ s, const float4* __restrict__ coef, void* __restrict__ gout, void* __restrict__ uout,
                                                                      float2* __restrict__ part, int C, int HW, int nb, int seg, int S, int N, float slope) {
   using V = A8Vec<AT, VEC>;
-  __shared__ float red[16];
+  __shared__ double redd[16];
   const int si = blockIdx.x % S, pl = blockIdx.x / S;
   const int n = pl / C, c = pl - n * C;
   const size_t plane = (size_t)pl, base = plane * HW;
   const A8Chan a = a8_chan(coef, c, ref != nullptr);
   const int beg = si * seg, end = min(HW, beg + seg);
-  float s1 = 0.f, s2 = 0.f;
+  double d1 = 0.0, d2 = 0.0;            // (in fp32 a thread's 64 terms left dgamma and dbeta 1.6e-7 off; the additions are hidden behind the loads)
 #pragma unroll 4
   for (int i = beg + (int)threadIdx.x * V::n; i < end; i += kA8Threads * V::n) {
-    float g[4];
+    float g[4], s1 = 0.f, s2 = 0.f;
     V::ldg(gin, base + i, g);
     const int w = V::ldq(q, base + i), rw = ref != nullptr ? V::ldq(ref, base + i) : 0;
     const float sc = s[plane * nb + (i >> 8)];
@@ -200,12 +200,13 @@ __global__ __launch_bounds__(kA8Threads) void act8_bwd_reduce_kernel(const void*
       s2 += o[j] * (a.off + (float)k * sc);
       if (OUT && uout != nullptr) u[j] = (float)(a.ctr + (double)k * (double)sc);
     }
+    d1 += (double)s1; d2 += (double)s2;
     if (OUT && gout != nullptr) V::stg(gout, base + i, o);
     if (OUT && uout != nullptr) V::stg(uout, base + i, u);
   }
-  s1 = block_sum(s1, red);
-  s2 = block_sum(s2, red);
-  if (threadIdx.x == 0) part[(size_t)c * ((size_t)N * S) + (size_t)n * S + si] = make_float2(s1, s2);
+  d1 = block_sum_d(d1, redd);
+  d2 = block_sum_d(d2, redd);
+  if (threadIdx.x == 0) part[(size_t)c * ((size_t)N * S) + (size_t)n * S + si] = make_float2((float)d1, (float)d2);
 }
 
 // du = scale (g' - S1/M - (x' - mean) invstd^2 S2/M)
