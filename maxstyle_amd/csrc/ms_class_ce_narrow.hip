@@ -1,4 +1,4 @@
-// Head + softmax cross entropy over many classes, narrow form (C <= 128): no operand and no product ever leaves the chip; see ms_class_ce.h.
+// Head + softmax cross entropy over many classes, narrow form (C <= 128, unless there are many classes for few rows): no operand and no product ever leaves the chip; see ms_class_ce.h.
 //
 //   prep    w -> fp16 planes in the order the LDS wants them, 64 classes a chunk with one power-of-two scale (an "image": the next kernel's DMA copies it as it
 //           lies); rows that take part counted
@@ -733,9 +733,11 @@ static CnPlan cn_plan(int N, int C, int V, int HW, int types, bool grad) {
 }
 
 bool ce_narrow_ok(int N, int C, int V, int HW) {
-  // The class loop of a wave is serial: with many classes and few rows the wide form's tiles over classes fill the chip better.
+  // A wave's loop over classes is serial, 0.015 + 0.00027 C us a class until the rows fill the chip; the wide form spreads classes over workgroups, starts 15 us later and
+  // takes 4e-6 us a row and class.  Training calls, fp32, narrow / wide in us: 64 channels, 600 classes: 48 / 39 at 64 rows, 54 / 61 at 4096, 117 / 245 at 65536;
+  // 16 channels, 1536 classes: 49 / 40, 53 / 70, 119 / 470; 128 channels, 1536 classes: 111 / 44, 139 / 75, 367 / 606.
   const long P = (long)N * HW;
-  return C <= 128 && (V <= 1536 || P >= 32768) && P < (1L << 30);
+  return C <= 128 && P < (1L << 30) && (double)V * (0.015 + 0.00027 * C - 4e-6 * (double)P) <= 15.0;
 }
 size_t ce_narrow_ws_bytes(int N, int C, int V, int HW, int types, bool grad) { return cn_plan(N, C, V, HW, types, grad).total; }
 

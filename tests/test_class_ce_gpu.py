@@ -382,3 +382,17 @@ def test_errors_of_rows_do_not_add_up(shape, V):
     lse = ops.class_ce_fwd(h, w, b, lab)[1].double().reshape(-1)
     want = torch.logsumexp(rows_of(h.double(), shape[1]) @ w.double().T + b.double(), 1)
     assert abs(float((lse - want).mean())) <= 2 * U32 + 4 * 16 * U32 / 12 ** 0.5 / lab.numel() ** 0.5
+
+
+def test_both_forms_over_many_rows_and_classes():
+    """Several pieces of rows and classes in the wide form (more than 128 channels), as rows and as planes, and the narrow form's long class loop."""
+    for shape, V, hdt, wdt in (((9001, 136), 8300, B, B), ((14000, 136), 17000, B, B), ((7100, 136), 17000, F, F), ((28, 136, 16, 16), 17000, B, F), ((12000, 64), 9001, F, F),
+                               ((8, 16, 32, 33), 7000, B, F)):
+        h, w, b, lab = make(shape, V, hdt, wdt, seed=1, wscale=2.0)
+        P = lab.numel()
+        r = reference(h, w, b, lab, torch.full((P,), 1.0 / P, dtype=torch.float64, device="cuda"))
+        loss, dh, dw, db = ops.class_ce(h, w, b, lab)
+        tdh, tdw, tdb = tolerances(r, hdt, wdt)
+        close(rows_of(dh, shape[1]), r["dh"], tdh, "dh")
+        close(dw, r["dw"], tdw, "dw")
+        close(db, r["db"], tdb, "db")
