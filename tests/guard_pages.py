@@ -1,7 +1,6 @@
 """Guard pages for the GPU tests: every tensor the package allocates ends (or starts) at the edge of its own hipMalloc'd block.
 
-On this pool a hipMalloc of a multiple of 2 MiB is followed by an unmapped page (tools/probes/oob_probe.hip: one byte past the end is a "Memory access fault by GPU",
-the process aborts); smaller blocks are carved from mapped 2 MiB fragments and a read past their end returns silently.  With PYTORCH_NO_CUDA_MEMORY_CACHING=1 every
+A hipMalloc of a multiple of 2 MiB is followed by an unmapped page (one byte past its end is a memory fault, the process aborts); smaller blocks are carved from mapped 2 MiB fragments and a read past their end returns silently.  With PYTORCH_NO_CUDA_MEMORY_CACHING=1 every
 torch allocation is its own hipMalloc, so a tensor placed at the END of a block rounded up to 2 MiB turns any access past its last element into a crash - a past-the-end
 sanitizer for the kernels' operand addressing (GPU AddressSanitizer is not available here).  Round 6 found such a read by accident (the Winograd appendix, DESIGN.md
 section 3); this makes the search deliberate.
