@@ -39,6 +39,13 @@ __device__ __forceinline__ float ce_log2(float x, int less = 0) {
   return (float)(e - less) + __builtin_amdgcn_logf(__builtin_amdgcn_ldexpf(x, -e));
 }
 
+// A product as fp32 holds it, for what is split: left to itself the compiler rounds the product to fp16 straight (v_fma_mixlo) where it forms hi and by way of fp32 (v_cvt) where it
+// forms lo, and for one element in some thousands the two planes then belong to different hi (2^-11 off).
+__device__ __forceinline__ float ce_rounded(float x) {
+  asm("" : "+v"(x));
+  return x;
+}
+
 // {hi, lo} planes of a scaled value
 __device__ __forceinline__ void ce_split(float x, _Float16& hi, _Float16& lo) {
   hi = (_Float16)x;

@@ -461,7 +461,7 @@ __device__ __forceinline__ void ce_gemm_tile(CeGemm g, int id, _Float16 (*sm)[(B
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           db[r] = __builtin_fmaf(acc[i][j][r], gp[j], db[r]);
-          acc[i][j][r] *= rj[j] * ff[r];
+          acc[i][j][r] = ce_rounded(acc[i][j][r] * (rj[j] * ff[r]));
         }
       }
       if (g.dbpart != nullptr) {
