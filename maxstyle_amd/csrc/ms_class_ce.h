@@ -6,7 +6,8 @@
 //
 // Numbers on the matrix cores.  Products run on v_mfma_f32_16x16x32_f16 with fp32 accumulation.  Every row of h and of w is scaled by a power of two of its own
 // (ex[p], ew[v]: exact, put back in the epilogue) so that its largest element lies in [2^13, 2^14), then split into fp16 planes: an fp32 value into two
-// (11 + 11 bits, x = hi + lo to 2^-22 relative or 2^-39 of the row's largest), a bf16 value (8 bits) into one, exactly down to 2^-37 of the row's largest.
+// (11 + 11 bits, x = hi + lo to 2^-22 relative or 2^-39 of the row's largest; where lo is kept 2^12 times as large, 2^-51), a bf16 value (8 bits) into one, exactly down to
+// 2^-37 of the row's largest.
 // A product of two-plane operands is hi hi + hi lo + lo hi (lo lo is below 2^-22): three matrix instructions for fp32 x fp32, two for bf16 x fp32, one for
 // bf16 x bf16.  fp32's own matrix instruction does 1/16 of the fp16 rate, so three of these are 5 times its speed at its accuracy.
 #pragma once
@@ -23,7 +24,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kCeTopExp = 13;         // scaled rows: largest magnitude in [2^13, 2^14)
 constexpr int kCePad = 256;           // rows of the packed operands are padded to whole tiles
 
-// the power of two that brings `amax` to [2^13, 2^14); 1 for a row of zeros or one with an infinity / NaN (it stays one), no smaller than 2^-100
+// the exponent of the power of two that `amax` is divided by to lie in [2^13, 2^14); 0 for a row of zeros or one with an infinity / NaN (it stays one), no smaller than 2^-100
 __device__ __forceinline__ int ce_exponent(float amax) {
   const unsigned b = __float_as_uint(amax);
   if (b >= 0x7F800000u || b == 0u) return 0;
@@ -52,7 +53,15 @@ __device__ __forceinline__ void ce_split(float x, _Float16& hi, _Float16& lo) {
   lo = (_Float16)(x - (float)hi);
 }
 
-// ... of eight at once: conversions in pairs, and x - hi as one multiply-add that reads the half-precision operand as it is (the factor -1 is hidden from the compiler, which
+// {hi, 2^12 lo}: the low plane keeps its 11 bits far below the high plane's lowest step (values to 2^-37 instead of 2^-25).  A product's low pairs are summed first and that sum
+// brought back by 2^-12 before the high pair is added.
+constexpr int kCeLoExp = 12;
+__device__ __forceinline__ void ce_split_far(float x, _Float16& hi, _Float16& lo) {
+  hi = (_Float16)x;
+  lo = (_Float16)((x - (float)hi) * (float)(1 << kCeLoExp));
+}
+
+// ... {hi, lo} of eight at once: conversions in pairs, and x - hi as one multiply-add that reads the half-precision operand as it is (the factor -1 is hidden from the compiler, which
 // would make a conversion and a subtraction of it; 104 classes x 16 channels x 1 M pixels 168 -> 163 us)
 typedef _Float16 ms_h2 __attribute__((ext_vector_type(2)));
 typedef float ms_f2 __attribute__((ext_vector_type(2)));

@@ -4,6 +4,7 @@
 //   pack w, pack h      fp16 planes [rows][channels], power-of-two scales, padded to whole tiles
 //   logits -> stats     tile of z stays in registers: (max, sum exp) of each row and class tile, and the label's own z
 //   join                lse and nll of every row, loss in 64 bits
+//   level               the scales that G is formed with; rows and classes far smaller than the largest are moved towards its scale
 //   per piece           G (logits again, written as fp16 planes), dh += G w, dw += G^T h; db from G's epilogue
 // The logits are never written; G exists for one piece at a time (kCePieceBytes: it
 // stays in the 256 MB last-level cache between its writer and its two readers).
@@ -54,7 +55,7 @@ __device__ __forceinline__ void ce_pack_row(const CePack& a, int r) {
   const int e = ce_exponent(__uint_as_float(am));
   const float inv = ce_pow2(-e);
   if (lane == 0) {
-    a.f[r] = ce_pow2(e);
+    a.f[r] = am == 0u ? 0.f : ce_pow2(e);                // 0: a row of zeros (ce_level_kernel)
     if (a.bpad != nullptr) a.bpad[r] = r < a.rows ? (a.b != nullptr ? a.b[r] * kLog2e : 0.f) : -__builtin_inff();
   }
   for (int c = lane * 8; c < a.Cp; c += 512) {
@@ -69,7 +70,7 @@ __device__ __forceinline__ void ce_pack_row(const CePack& a, int r) {
     }
     ms_h8 hi, lo;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) { _Float16 x, y; ce_split(v[k] * inv, x, y); hi[k] = x; lo[k] = y; }
+    for (int k = 0; k < 8; ++k) { _Float16 x, y; ce_split_far(v[k] * inv, x, y); hi[k] = x; lo[k] = y; }
     *reinterpret_cast<ms_h8*>(a.out + (size_t)r * a.Cp + c) = hi;
     if (PL == 2) *reinterpret_cast<ms_h8*>(a.out + a.plane + (size_t)r * a.Cp + c) = lo;
   }
@@ -109,13 +110,13 @@ __global__ __launch_bounds__(1024) void ce_pack_planes_kernel(const void* __rest
   for (int k = 0; k < 16; ++k) am = max(am, smax[k][lane]);
   const int e = ce_exponent(__uint_as_float(am));
   const float inv = ce_pow2(-e);
-  if (wave == 0) fx[p] = ce_pow2(e);
+  if (wave == 0) fx[p] = am == 0u ? 0.f : ce_pow2(e);
   for (int c0 = wave * 8; c0 < Cp; c0 += 128) {
     ms_h8 hi, lo;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       _Float16 x, z;
-      ce_split((live && c0 + k < C) ? IO::ld1(h, base + (size_t)(c0 + k) * HW) * inv : 0.f, x, z);
+      ce_split_far((live && c0 + k < C) ? IO::ld1(h, base + (size_t)(c0 + k) * HW) * inv : 0.f, x, z);
       hi[k] = x; lo[k] = z;
     }
     *reinterpret_cast<ms_h8*>(out + (size_t)p * Cp + c0) = hi;
@@ -144,16 +145,23 @@ __device__ __forceinline__ int ce_count(const int* __restrict__ slots, int n, in
   return red[0] + red[1] + red[2] + red[3];
 }
 
-__device__ __forceinline__ int ce_row_exponent(float g, float fx) {
+constexpr int kCeNone = -100000;
+// exponent of g_p 2^ex[p]; none for a row without a gradient or of zeros
+__device__ __forceinline__ int ce_grad_exponent(float g) {
   const unsigned b = __float_as_uint(g) & 0x7FFFFFFFu;
-  return (b != 0u && b < 0x7F800000u) ? (int)(b >> 23) - 126 + (int)(__float_as_uint(fx) >> 23) - 127 : -100000;
+  return (b != 0u && b < 0x7F800000u) ? (int)(b >> 23) - 126 : kCeNone;
+}
+__device__ __forceinline__ int ce_scale_exponent(float f) { return f > 0.f ? (int)(__float_as_uint(f) >> 23) - 127 : kCeNone; }
+__device__ __forceinline__ int ce_row_exponent(float g, float fx) {
+  const int a = ce_grad_exponent(g), b = ce_scale_exponent(fx);
+  return (a == kCeNone || b == kCeNone) ? kCeNone : a + b;
 }
 // The upstream gradient of every row: grad[p], 0 where the label is not a class.  A row without one gets a log-sum of infinity: exp(z - inf) = 0 whatever its logits are.
 // rowmax[workgroup]: the largest exponent of g_p 2^ex[p].
 __global__ __launch_bounds__(256) void ce_rowgrad_kernel(const float* __restrict__ grad, const int* __restrict__ lab32, const float* __restrict__ fx, float* __restrict__ gp,
                                                          const float* __restrict__ lse_in, float* __restrict__ lse2, int* __restrict__ rowmax, long P, long Pp) {
   __shared__ int red[4];
-  int e = -100000;
+  int e = kCeNone;
   for (long p = (long)blockIdx.x * 256 + threadIdx.x; p < Pp; p += (long)gridDim.x * 256) {
     const float g = (p < P && lab32[p] >= 0) ? grad[p] : 0.f;
     e = max(e, ce_row_exponent(g, fx[p]));
@@ -167,36 +175,86 @@ __global__ __launch_bounds__(256) void ce_rowgrad_kernel(const float* __restrict
   if (threadIdx.x == 0) rowmax[blockIdx.x] = max(max(red[0], red[1]), max(red[2], red[3]));
 }
 
-// One workgroup: the loss, and the power of two (scal[0]) that brings the largest |G| 2^(ex + ew) below 2^14.
-__global__ __launch_bounds__(1024) void ce_scalars_kernel(const double* __restrict__ lsum, int n, float sign, int mean_valid, const int* __restrict__ slots, int nslots, long P,
-                                                          float* __restrict__ loss, const int* __restrict__ rowmax, int nrow, const float* __restrict__ fw, int V, int* __restrict__ scal) {
+// The loss (first workgroup), and the scales that G is formed with.
+//
+// One G serves both products: G'[p,v] = G[p,v] 2^(r[p] + c[v] + scal), dh[p] = 2^-(r[p] + scal) sum_v G' w/2^c[v], dw[v] = 2^-(c[v] + scal) sum_p G' h/2^r[p].  With the rows' own
+// exponents, r = ex, a row (class) far smaller than the largest would have its G' far below the largest although neither dh of the row nor dw of the class depends on its size, and a row
+// of zeros has no exponent at all.  So every row's exponent of g_p 2^r[p], and every c[v], is brought to at least the largest less kCeWindow - rows of zeros for nothing, others by
+// dividing their planes by that much, as long as these keep 24 bits of the row's largest (kCeMove1 / 2: one / two planes).  Within 2^30 of the largest, G' is held to 2^-22 of itself
+// (one plane: 2^-12) or 2^-41 (2^-30) g_p, whatever the row's and the class's size are.  Rows within the window, the ordinary case, are not touched.
+constexpr int kCeWindow = 4, kCeMove1 = 16, kCeMove2 = 26;
+struct CeLevel {
+  const double* lsum; int n; float sign; int mean_valid; const int* slots; int nslots; long P; float* loss;
+  const int* rowmax; int nrow; const float *fx, *gp, *fw; float *fx2, *fw2; _Float16 *x, *w; size_t xpl, wpl; int xp, wp, V, Vp, Cp; long Pp; int* scal;
+};
+__device__ __forceinline__ void ce_move(_Float16* row, size_t plane, int planes, int Cp, int lane, int by) {
+  const float f = ce_pow2(-by);
+  for (int c = lane * 8; c < Cp; c += 512) {
+    ms_h8 hi = *reinterpret_cast<const ms_h8*>(row + c), lo;
+    if (planes == 2) lo = *reinterpret_cast<const ms_h8*>(row + plane + c);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float v = planes == 2 ? (float)hi[k] + (float)lo[k] * (1.f / (float)(1 << kCeLoExp)) : (float)hi[k];
+      _Float16 a, b;
+      ce_split_far(v * f, a, b);
+      hi[k] = a; lo[k] = b;
+    }
+    *reinterpret_cast<ms_h8*>(row + c) = hi;
+    if (planes == 2) *reinterpret_cast<ms_h8*>(row + plane + c) = lo;
+  }
+}
+__global__ __launch_bounds__(1024) void ce_level_kernel(CeLevel a) {
   __shared__ double redd[16];
   __shared__ int redi[32];
-  if (loss != nullptr) {
-    const int cnt = mean_valid ? ce_count(slots, nslots, redi) : 0;
-    double a = 0.0;
-    for (int i = threadIdx.x; i < n; i += 1024) a += lsum[i];
-    a = block_sum_d(a, redd);
-    if (threadIdx.x == 0) loss[0] = (float)((double)sign * a / (double)(mean_valid ? max(cnt, 1) : P));
+  if (a.loss != nullptr && blockIdx.x == 0) {
+    const int cnt = a.mean_valid ? ce_count(a.slots, a.nslots, redi) : 0;
+    double s = 0.0;
+    for (int i = threadIdx.x; i < a.n; i += 1024) s += a.lsum[i];
+    s = block_sum_d(s, redd);
+    if (threadIdx.x == 0) a.loss[0] = (float)((double)a.sign * s / (double)(a.mean_valid ? max(cnt, 1) : a.P));
   }
-  if (rowmax == nullptr) return;
-  int er = -100000, ew = -100000;
-  for (int i = threadIdx.x; i < nrow; i += 1024) er = max(er, rowmax[i]);
+  if (a.rowmax == nullptr) return;
+  int er = kCeNone, ew = kCeNone;
 #pragma unroll 4
-  for (int v = threadIdx.x * 4; v < V; v += 4096) {        // (padded to whole tiles)
-    const float4 f = *reinterpret_cast<const float4*>(fw + v);
+  for (int i = threadIdx.x; i < a.nrow; i += 1024) er = max(er, a.rowmax[i]);
+#pragma unroll 4
+  for (int v = threadIdx.x * 4; v < a.V; v += 4096) {        // (padded to whole tiles)
+    const float4 f = *reinterpret_cast<const float4*>(a.fw + v);
     const float ff[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
-    for (int k = 0; k < 4; ++k) if (v + k < V) ew = max(ew, (int)(__float_as_uint(ff[k]) >> 23) - 127);
+    for (int k = 0; k < 4; ++k) if (v + k < a.V) ew = max(ew, ce_scale_exponent(ff[k]));
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) { er = max(er, __shfl_xor(er, off, 64)); ew = max(ew, __shfl_xor(ew, off, 64)); }
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) { redi[threadIdx.x >> 6] = er; redi[16 + (threadIdx.x >> 6)] = ew; }
+  if (lane == 0) { redi[wave] = er; redi[16 + wave] = ew; }
   __syncthreads();
-  if (threadIdx.x != 0) return;
   for (int k = 0; k < 16; ++k) { er = max(er, redi[k]); ew = max(ew, redi[16 + k]); }
-  scal[0] = er < -50000 ? 0 : min(max(kCeTopExp - (er + ew), -120), 120);
+  if (er == kCeNone) er = 0;
+  if (ew == kCeNone) ew = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.scal[0] = min(max(kCeTopExp - (er + ew), -120), 120);
+  // a wave takes 16 classes or rows: one lane each finds the new exponent, the whole wave moves those that need it
+  for (long i0 = ((long)blockIdx.x * 16 + wave) * 16; i0 < a.Vp + a.Pp; i0 += (long)gridDim.x * 256) {
+    const bool cls = i0 < a.Vp;
+    const long r0 = cls ? i0 : i0 - a.Vp;
+    const int planes = cls ? a.wp : a.xp;
+    int by = 0;
+    if (lane < 16) {
+      const int e = ce_scale_exponent((cls ? a.fw : a.fx)[r0 + lane]), g = cls ? 0 : ce_grad_exponent(a.gp[r0 + lane]), top = (cls ? ew : er) - kCeWindow - g;
+      int to = e == kCeNone ? 0 : e;
+      if (g != kCeNone) {
+        if (e == kCeNone) to = min(max(top, -100), 120);
+        else to = min(max(e, min(top, e + (planes == 2 ? kCeMove2 : kCeMove1))), max(e, 120));
+      }
+      (cls ? a.fw2 : a.fx2)[r0 + lane] = ce_pow2(to);
+      by = e == kCeNone ? 0 : to - e;
+    }
+    for (unsigned long long m = __ballot(by != 0); m != 0; m &= m - 1) {
+      const int k = __builtin_ctzll(m);
+      ce_move((cls ? a.w : a.x) + (size_t)(r0 + k) * a.Cp, cls ? a.wpl : a.xpl, planes, a.Cp, lane, __shfl(by, k, 64));
+    }
+  }
 }
 
 struct CeRowGrad { float* gp; const float* fx; float sign; int mean_valid; const float* scale_dev; const int* slots; int nslots; int* rowmax; };
@@ -248,7 +306,7 @@ __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict_
 struct CeOperand { const _Float16* p; size_t plane; int ld; int cols; };      // ROW: [mn][k], ld = row stride; COL: [k][mn], cols = valid columns
 struct CeGemm {
   CeOperand a, b;
-  int nseg, pa[3], pb[3];         // plane pairs summed into one accumulator
+  int nseg, pa[3], pb[3];         // plane pairs summed into one accumulator: the low ones, then the high one
   int ksteps;                     // K / 64 of one pair
   int mt, nt, split;
   // logits epilogues
@@ -324,7 +382,7 @@ __device__ __forceinline__ void ce_gemm_tile(CeGemm g, int id, _Float16 (*sm)[(B
   const int mt = gi * GRP + gr % gm, nt = gr / gm;
   const int m0 = mt * BM, n0 = nt * BN;
   const int steps = g.ksteps * g.nseg;
-  const int k0 = (int)((long)steps * sp / g.split), k1 = (int)((long)steps * (sp + 1) / g.split);
+  const int k0 = (int)((long)steps * sp / g.split), k1 = (int)((long)steps * (sp + 1) / g.split), klow = g.ksteps * (g.nseg - 1);      // steps below klow: low pairs
 
   ms_f4 acc[MI][NJ];
 #pragma unroll
@@ -343,32 +401,43 @@ __device__ __forceinline__ void ce_gemm_tile(CeGemm g, int id, _Float16 (*sm)[(B
   };
   constexpr int kLoads = (BM + BN) * kCeBK * 2 / 1024 / NW;         // DMA instructions of a slab and wave
 #pragma unroll
-  for (int t = 0; t < ST - 1; ++t) if (k0 + t < k1) stage(k0 + t);
-  for (int t = k0; t < k1; ++t) {
-    if (ST > 2 && t + ST - 2 < k1) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kLoads * (ST - 2)) : "memory");      // the ST - 2 slabs behind t may be on their way
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();                    // slab t has landed for every wave, and nobody reads the buffer that slab t + ST - 1 goes to
-    if (t + ST - 1 < k1) stage(t + ST - 1);
-    const _Float16* sa = &sm[t & (ST - 1)][0];
-    const _Float16* sb = sa + BM * kCeBK;
-    // All fragments of the slab first, then its products in one run at raised priority: the other workgroup's (wave's) reads and DMA fill the gaps (1163 -> 1115 us for
-    // 6400 rows x 512 channels x 32768 classes).  A ring of four slabs of 32 with counted waits was slower (1298: a barrier per 32).
-    ms_h8 fa[2][MI], fb[2][NJ];
+  for (int s = 0; s < ST - 1; ++s) if (k0 + s < k1) stage(k0 + s);
+  int t = k0;
+#pragma unroll 1
+  for (int high = 0; high < 2; ++high) {      // low pairs, then the high one (a test of t inside one loop cost the 128 x 128 products 10 - 12 %)
+    const int te = high ? k1 : min(klow, k1);
+    for (; t < te; ++t) {
+      if (ST > 2 && t + ST - 2 < k1) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kLoads * (ST - 2)) : "memory");      // the ST - 2 slabs behind t may be on their way
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();                    // slab t has landed for every wave, and nobody reads the buffer that slab t + ST - 1 goes to
+      if (t + ST - 1 < k1) stage(t + ST - 1);
+      const _Float16* sa = &sm[t & (ST - 1)][0];
+      const _Float16* sb = sa + BM * kCeBK;
+      // All fragments of the slab first, then its products in one run at raised priority: the other workgroup's (wave's) reads and DMA fill the gaps (1163 -> 1115 us for
+      // 6400 rows x 512 channels x 32768 classes).  A ring of four slabs of 32 with counted waits was slower (1298: a barrier per 32).
+      ms_h8 fa[2][MI], fb[2][NJ];
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
+      for (int ks = 0; ks < 2; ++ks) {
 #pragma unroll
-      for (int i = 0; i < MI; ++i) fa[ks][i] = ce_frag<BM, ACOL>(sa, wm * TM + i * 16, ks, lane);
+        for (int i = 0; i < MI; ++i) fa[ks][i] = ce_frag<BM, ACOL>(sa, wm * TM + i * 16, ks, lane);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) fb[ks][j] = ce_frag<BN, BCOL>(sb, wn * TN + j * 16, ks, lane);
+        for (int j = 0; j < NJ; ++j) fb[ks][j] = ce_frag<BN, BCOL>(sb, wn * TN + j * 16, ks, lane);
+      }
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[ks][i], fb[ks][j], acc[i][j], 0, 0, 0);
+      __builtin_amdgcn_s_setprio(0);
     }
-    __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
+    if (!high && te > k0) {
 #pragma unroll
       for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[ks][i], fb[ks][j], acc[i][j], 0, 0, 0);
-    __builtin_amdgcn_s_setprio(0);
+        for (int j = 0; j < NJ; ++j) acc[i][j] *= 1.f / (float)(1 << kCeLoExp);
+    }
   }
 
   // Fragment layout of the result: column n = lane & 15, rows m = 4 (lane >> 4) + 0..3.
@@ -487,7 +556,7 @@ __device__ __forceinline__ void ce_gemm_tile(CeGemm g, int id, _Float16 (*sm)[(B
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const _Float16 hi = (_Float16)acc[i][j][r];
-            v[r] = pl == 0 ? hi : (_Float16)(acc[i][j][r] - (float)hi);
+            v[r] = pl == 0 ? hi : (_Float16)((acc[i][j][r] - (float)hi) * (float)(1 << kCeLoExp));
           }
           const int row = wn * TN + j * 16 + li, col = wm * TM + i * 16 + q * 4;
           *reinterpret_cast<ms_h4*>(tile + row * BM + (((col >> 3) ^ (row & kSwz)) * 8) + (col & 7)) = v;
@@ -574,7 +643,7 @@ struct CePlan {
   int pb, vb;                    // rows / classes of a piece
   int nparts, sb;                // partial statistics of a row, rows whose statistics are formed at a time
   int split_x, split_w;
-  size_t o_x, o_w, o_fx, o_fw, o_b, o_lab, o_lse, o_zl, o_gp, o_part, o_scal, o_slots, o_rowmax, o_lsum, o_g, o_db, o_px, o_pw, o_ax, o_aw, total;
+  size_t o_x, o_w, o_fx, o_fw, o_fx2, o_fw2, o_b, o_lab, o_lse, o_zl, o_gp, o_part, o_scal, o_slots, o_rowmax, o_lsum, o_g, o_db, o_px, o_pw, o_ax, o_aw, total;
 };
 static size_t ce_al(size_t n) { return (n + 255) & ~(size_t)255; }
 static long ce_up(long a, long b) { return (a + b - 1) / b * b; }
@@ -603,6 +672,7 @@ static CePlan ce_plan(int N, int C, int V, int HW, int types, bool grad) {
   // (two of a tile; 64-wide tiles, twice as many, are taken for less than 128 tiles of 128 x 128: 512 x 254 pairs at most)
   const size_t stats = std::max((size_t)k.nparts * k.sb * 8, (size_t)2 << 20);
   if (!grad) { k.o_part = take(stats); k.total = o; return k; }
+  k.o_fx2 = take(k.Pp * 4); k.o_fw2 = take((size_t)k.Vp * 4);
   // The statistics are read before the first piece of G is written: they share its memory.
   k.o_part = o;
   k.o_g = take(std::max((size_t)k.gpl * k.pb * k.vb * 2, stats));
@@ -656,9 +726,10 @@ static int ce_gemm(CeGemm g, const CeTile& c, hipStream_t st, const char* what) 
   return check_launch(what);
 }
 static void ce_pairs(CeGemm& g, int a, int b) {       // planes of the two operands -> products
-  g.nseg = 1; g.pa[0] = g.pb[0] = 0;
+  g.nseg = 0;
   if (b == 2) { g.pa[g.nseg] = 0; g.pb[g.nseg++] = 1; }
   if (a == 2) { g.pa[g.nseg] = 1; g.pb[g.nseg++] = 0; }
+  g.pa[g.nseg] = g.pb[g.nseg] = 0; ++g.nseg;
 }
 
 static int ce_run(const CeArgs& a, const char* who) {
@@ -730,10 +801,17 @@ static int ce_run(const CeArgs& a, const char* who) {
     if (int e = check_launch("class_ce_rowgrad")) return e;
   }
   if (need_grad || a.loss != nullptr) {
-    MS_LAUNCH(ce_scalars_kernel, dim3(1), dim3(1024), 0, st, (const double*)(ws + k.o_lsum), (int)(k.Pp / 64), a.sign, a.mean_valid, slots, nslots, k.P, a.loss,
-              need_grad ? rowmax : (const int*)nullptr, nrow, fw, a.V, scal);
-    if (int e = check_launch("class_ce_scalars")) return e;
+    CeLevel l{};
+    l.lsum = (const double*)(ws + k.o_lsum); l.n = (int)(k.Pp / 64); l.sign = a.sign; l.mean_valid = a.mean_valid; l.slots = slots; l.nslots = nslots; l.P = k.P; l.loss = a.loss;
+    if (need_grad) {
+      l.rowmax = rowmax; l.nrow = nrow; l.fx = fx; l.gp = gp; l.fw = fw; l.fx2 = f32(k.o_fx2); l.fw2 = f32(k.o_fw2); l.x = x; l.w = w; l.xpl = xpl; l.wpl = wpl;
+      l.xp = k.xp; l.wp = k.wp; l.V = a.V; l.Vp = k.Vp; l.Cp = k.Cp; l.Pp = k.Pp; l.scal = scal;
+    }
+    const int blocks = need_grad ? (int)std::min<long>(kNumCU, (k.Vp + k.Pp) / 256) : 1;        // (every workgroup finds the largest exponents for itself)
+    MS_LAUNCH(ce_level_kernel, dim3(blocks), dim3(1024), 0, st, l);
+    if (int e = check_launch("class_ce_level")) return e;
   }
+  if (need_grad) { fx = f32(k.o_fx2); fw = f32(k.o_fw2); g.fx = fx; g.fw = fw; }
   if (!need_grad) return MS_OK;
   const long cp = ce_up(k.Cp, 128);
   for (long p0 = 0; p0 < k.Pp; p0 += k.pb) {

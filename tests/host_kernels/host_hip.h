@@ -122,15 +122,14 @@ inline void __syncthreads() {
   else while (host::bar_gen == g) host::yield();
 }
 template <typename T> inline T __shfl_xor(T v, int off, int) { const int k = host::exchange(v); return host::of<T>(k, host::fibers[host::cur].lane ^ off); }
-inline bool __any(bool p) {
-  const int k = host::exchange((int)p);
-  const host::Wave& w = host::waves[host::fibers[host::cur].wave];
-  const int base = host::fibers[host::cur].wave * host::kLanes;
-  bool r = false;
-  for (int l = 0; l < host::kLanes; ++l) if (base + l < host::nthreads && !host::fibers[base + l].done) r |= host::of<int>(k, l) != 0;
-  (void)w;
+template <typename T> inline T __shfl(T v, int lane, int) { const int k = host::exchange(v); return host::of<T>(k, lane); }
+inline unsigned long long __ballot(bool p) {
+  const int k = host::exchange((int)p), base = host::fibers[host::cur].wave * host::kLanes;
+  unsigned long long r = 0;
+  for (int l = 0; l < host::kLanes; ++l) if (base + l < host::nthreads && !host::fibers[base + l].done && host::of<int>(k, l) != 0) r |= 1ull << l;
   return r;
 }
+inline bool __any(bool p) { return __ballot(p) != 0; }
 inline int atomicMax(int* p, int v) { const int o = *p; if (v > o) *p = v; return o; }
 template <typename... P, typename... A>
 inline void hipLaunchKernelGGL(void (*f)(P...), dim3 grid, dim3 block, unsigned, hipStream_t, A... a) { host::launch(grid, block, [=]() { f(a...); }); }

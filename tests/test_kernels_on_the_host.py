@@ -19,7 +19,7 @@ def child(args):
     return subprocess.run([sys.executable] + args, cwd=HERE, env=ENV, capture_output=True, text=True, timeout=900)
 
 
-@pytest.mark.parametrize("which,seed,count", [("class_ce", 3, 120), ("class_ce_pieces", 2, 120), ("act8", 1, 100)])
+@pytest.mark.parametrize("which,seed,count", [("class_ce", 1, 240), ("class_ce_pieces", 2, 120), ("act8", 1, 100)])
 def test_every_access_is_inside_its_buffer(which, seed, count):
     r = child(["sweep.py", which, str(seed), str(count)])
     assert r.returncode == 0 and r.stdout.endswith("done\n"), (r.returncode, r.stdout[-400:], r.stderr[-800:])
@@ -31,3 +31,9 @@ def test_an_access_outside_ends_the_child():
             "print(lib.ms_act8_pack(g.p(x), None, g.p(q), g.p(s), 1, 1, %d, None), flush=True)")
     assert child(["-c", code % ("end", 1024, 1024)]).stdout == "0\n"
     assert child(["-c", code % ("end", 1024, 1025)]).returncode == -11
+
+
+@pytest.mark.parametrize("form", ["wide"])
+def test_gradients_of_rows_and_classes_of_any_size(form):
+    r = child(["scales.py", form])
+    assert r.returncode == 0 and r.stdout.endswith("done\n"), "\n".join(l for l in r.stdout.splitlines() if "FAIL" in l) + r.stderr[-800:]
