@@ -79,4 +79,19 @@ __device__ __forceinline__ void ce_split8(ms_f4 a, ms_f4 b, ms_h8& hi, ms_h8& lo
   hi = H.h; lo = L.h;
 }
 
+// ... {hi, 2^12 lo} of eight at once: 2^12 (x - hi) as a multiply-add of the half-precision operand and 2^12 x
+__device__ __forceinline__ void ce_split8_far(ms_f4 a, ms_f4 b, ms_h8& hi, ms_h8& lo) {
+  union { ms_h2 p[4]; ms_h8 h; } H, L;
+  float neg = -(float)(1 << kCeLoExp);
+  asm("" : "+s"(neg));
+  const ms_f2 v[4] = {{a[0], a[1]}, {a[2], a[3]}, {b[0], b[1]}, {b[2], b[3]}};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    H.p[i] = __builtin_convertvector(v[i], ms_h2);
+    const ms_f2 r = {__builtin_fmaf((float)H.p[i][0], neg, v[i][0] * (float)(1 << kCeLoExp)), __builtin_fmaf((float)H.p[i][1], neg, v[i][1] * (float)(1 << kCeLoExp))};
+    L.p[i] = __builtin_convertvector(r, ms_h2);
+  }
+  hi = H.h; lo = L.h;
+}
+
 }  // namespace ms

@@ -196,7 +196,7 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
     am = max(am, (unsigned)__shfl_xor((int)am, 32, 64));
     const int e = ce_exponent(__uint_as_float(am));
     const float inv = ce_pow2(-e);
-    fx[j] = ce_pow2(e);
+    fx[j] = am == 0u ? 0.f : ce_pow2(e);          // 0: a pixel of zeros, which sets no scale in the class pass
 #pragma unroll
     for (int ks = 0; ks < KN; ++ks)
 #pragma unroll
@@ -474,7 +474,9 @@ __global__ __launch_bounds__(256, 2) void cn_classes_kernel(CnwArgs a) {
   }
   const int t0 = (int)((long)a.tiles * blockIdx.x / a.splits), t1 = (int)((long)a.tiles * (blockIdx.x + 1) / a.splits);
 
-  // G 2^ex is scaled so that the largest |g_p| 2^ex met so far lies below 2^kCeTopExp: the partial sums are moved along when a tile brings a larger one.
+  // G 2^ex is scaled so that the largest |g_p| 2^ex met so far lies below 2^kCeTopExp: the partial sums are moved along when a tile brings a larger one.  A pixel of zeros takes no part
+  // in that: its G is not needed for dw.  The low plane of G is kept 2^12 times as large, against the pixels' high plane divided by 2^12: G holds its bits to 2^-37, so that one pixel of
+  // large features (2^10 and more of the others) does not push the others' G into fp16's lowest steps.
   int kmax = -100000;
   float gn = 0.f;
   if (threadIdx.x < 2) tmax[threadIdx.x] = -100000;
@@ -515,7 +517,7 @@ __global__ __launch_bounds__(256, 2) void cn_classes_kernel(CnwArgs a) {
       rows[0][threadIdx.x] = prow[0]; rows[1][threadIdx.x] = prow[1]; rows[2][threadIdx.x] = prow[2] * prow[0]; rows[3][threadIdx.x] = prow[2];
       labs[threadIdx.x] = plab;
       const unsigned gb = __float_as_uint(prow[2]) & 0x7FFFFFFFu;
-      int e = (gb != 0u && gb < 0x7F800000u) ? (int)(gb >> 23) - 126 + (int)(__float_as_uint(prow[0]) >> 23) - 127 : -100000;
+      int e = (gb != 0u && gb < 0x7F800000u && prow[0] > 0.f) ? (int)(gb >> 23) - 126 + (int)(__float_as_uint(prow[0]) >> 23) - 127 : -100000;
 #pragma unroll
       for (int off = 32; off > 0; off >>= 1) e = max(e, __shfl_xor(e, off, 64));
       if (lane == 0) atomicMax(&tmax[t & 1], e);
@@ -619,7 +621,7 @@ __global__ __launch_bounds__(256, 2) void cn_classes_kernel(CnwArgs a) {
             }
         }
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) ce_split8(s[0][j], s[1][j], gh[j], gl[j]);
+        for (int j = 0; j < NJ; ++j) ce_split8_far(s[0][j], s[1][j], gh[j], gl[j]);
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
           const int row = c * 16 + li;
@@ -633,8 +635,9 @@ __global__ __launch_bounds__(256, 2) void cn_classes_kernel(CnwArgs a) {
 #pragma unroll
           for (int j = 0; j < NJ; ++j) o[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh.h, gh[j], o[c][j], 0, 0, 0);
           if (kG2) {
+            const ms_h8 xd = xh.h * (_Float16)(1.f / (float)(1 << kCeLoExp));
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) o[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh.h, gl[j], o[c][j], 0, 0, 0);
+            for (int j = 0; j < NJ; ++j) o[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xd, gl[j], o[c][j], 0, 0, 0);
             if (HP == 2) {
 #pragma unroll
               for (int j = 0; j < NJ; ++j) o[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl.h, gh[j], o[c][j], 0, 0, 0);

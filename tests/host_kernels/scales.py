@@ -60,7 +60,7 @@ def cases(narrow):
             if name == "spread gradients":
                 grad = grad * 2.0 ** rng.uniform(-30, 0, P)
             if name == "large row":
-                hr[7] *= 1e4
+                hr[7] *= 1e6 if narrow else 1e4
             h = np.moveaxis(hr.reshape((shape[0],) + shape[2:] + (C,)), -1, 1).astype(np.float32)
             yield name, hb, wb, np.ascontiguousarray(h), w.astype(np.float32), b.astype(np.float32), lab, grad.astype(np.float32)
         shape, V = ((1, 64, 16, 16), 151) if narrow else ((256, 136), 700)

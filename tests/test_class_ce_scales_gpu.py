@@ -41,7 +41,7 @@ def make(name, shape, V, hdt, wdt, narrow):
     if name == "spread gradients":
         gr = gr * spread(P, 30)
     if name == "large row":
-        hr[7] *= 1e4
+        hr[7] *= 1e6 if narrow else 1e4
     if name == "all classes zero":
         w = w * 0
     if name == "all rows zero":
@@ -88,3 +88,10 @@ def check(name, shape, V, hdt, wdt, narrow):
 @pytest.mark.parametrize("shape,V", [((256, 512), 8192), ((2, 136, 12, 13), 1000), ((40, 130), 33)])
 def test_wide_form(name, hdt, wdt, shape, V):
     check(name, shape, V, hdt, wdt, False)
+
+
+@pytest.mark.parametrize("name", CASES)
+@pytest.mark.parametrize("hdt,wdt", [(F, F), (B, B)])
+@pytest.mark.parametrize("shape,V", [((2, 64, 40, 40), 151), ((1, 16, 50, 37), 104), ((3000, 100), 40)])
+def test_narrow_form(name, hdt, wdt, shape, V):
+    check(name, shape, V, hdt, wdt, True)

@@ -33,7 +33,7 @@ def test_an_access_outside_ends_the_child():
     assert child(["-c", code % ("end", 1024, 1025)]).returncode == -11
 
 
-@pytest.mark.parametrize("form", ["wide"])
+@pytest.mark.parametrize("form", ["wide", "narrow"])
 def test_gradients_of_rows_and_classes_of_any_size(form):
     r = child(["scales.py", form])
     assert r.returncode == 0 and r.stdout.endswith("done\n"), "\n".join(l for l in r.stdout.splitlines() if "FAIL" in l) + r.stderr[-800:]
