@@ -182,10 +182,12 @@ __global__ __launch_bounds__(256) void ce_rowgrad_kernel(const float* __restrict
 // of zeros has no exponent at all.  So every row's exponent of g_p 2^r[p], and every c[v], is brought to at least the largest less kCeWindow - rows of zeros for nothing, others by
 // dividing their planes by that much, as long as these keep 24 bits of the row's largest (kCeMove1 / 2: one / two planes).  Within 2^30 of the largest, G' is held to 2^-22 of itself
 // (one plane: 2^-12) or 2^-41 (2^-30) g_p, whatever the row's and the class's size are.  Rows within the window, the ordinary case, are not touched.
-constexpr int kCeWindow = 4, kCeMove1 = 16, kCeMove2 = 26;
+// A class that is switched off (b = -inf) may hold anything finite and sets no scale; where it holds more than 4 times the largest of the others its planes are cleared (its G is 0, but
+// for a row with this very label, whose loss is infinite).
+constexpr int kCeWindow = 4, kCeMove1 = 16, kCeMove2 = 26, kCeClear = 1000;
 struct CeLevel {
   const double* lsum; int n; float sign; int mean_valid; const int* slots; int nslots; long P; float* loss;
-  const int* rowmax; int nrow; const float *fx, *gp, *fw; float *fx2, *fw2; _Float16 *x, *w; size_t xpl, wpl; int xp, wp, V, Vp, Cp; long Pp; int* scal;
+  const int* rowmax; int nrow; const float *fx, *gp, *fw, *bpad; float *fx2, *fw2; _Float16 *x, *w; size_t xpl, wpl; int xp, wp, V, Vp, Cp; long Pp; int* scal;
 };
 __device__ __forceinline__ void ce_move(_Float16* row, size_t plane, int planes, int Cp, int lane, int by) {
   const float f = ce_pow2(-by);
@@ -196,7 +198,7 @@ __device__ __forceinline__ void ce_move(_Float16* row, size_t plane, int planes,
     for (int k = 0; k < 8; ++k) {
       const float v = planes == 2 ? (float)hi[k] + (float)lo[k] * (1.f / (float)(1 << kCeLoExp)) : (float)hi[k];
       _Float16 a, b;
-      ce_split_far(v * f, a, b);
+      ce_split_far(by == kCeClear ? 0.f : v * f, a, b);
       hi[k] = a; lo[k] = b;
     }
     *reinterpret_cast<ms_h8*>(row + c) = hi;
@@ -219,10 +221,10 @@ __global__ __launch_bounds__(1024) void ce_level_kernel(CeLevel a) {
   for (int i = threadIdx.x; i < a.nrow; i += 1024) er = max(er, a.rowmax[i]);
 #pragma unroll 4
   for (int v = threadIdx.x * 4; v < a.V; v += 4096) {        // (padded to whole tiles)
-    const float4 f = *reinterpret_cast<const float4*>(a.fw + v);
-    const float ff[4] = {f.x, f.y, f.z, f.w};
+    const float4 f = *reinterpret_cast<const float4*>(a.fw + v), b = *reinterpret_cast<const float4*>(a.bpad + v);
+    const float ff[4] = {f.x, f.y, f.z, f.w}, bb[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-    for (int k = 0; k < 4; ++k) if (v + k < a.V) ew = max(ew, ce_scale_exponent(ff[k]));
+    for (int k = 0; k < 4; ++k) if (bb[k] != -__builtin_inff()) ew = max(ew, ce_scale_exponent(ff[k]));
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) { er = max(er, __shfl_xor(er, off, 64)); ew = max(ew, __shfl_xor(ew, off, 64)); }
@@ -247,8 +249,13 @@ __global__ __launch_bounds__(1024) void ce_level_kernel(CeLevel a) {
         if (e == kCeNone) to = min(max(top, -100), 120);
         else to = min(max(e, min(top, e + (planes == 2 ? kCeMove2 : kCeMove1))), max(e, 120));
       }
+      if (cls && e > ew + 2 && e != kCeNone) {          // (switched off)
+        to = ew;
+        by = kCeClear;
+      } else {
+        by = e == kCeNone ? 0 : to - e;
+      }
       (cls ? a.fw2 : a.fx2)[r0 + lane] = ce_pow2(to);
-      by = e == kCeNone ? 0 : to - e;
     }
     for (unsigned long long m = __ballot(by != 0); m != 0; m &= m - 1) {
       const int k = __builtin_ctzll(m);
@@ -804,7 +811,7 @@ static int ce_run(const CeArgs& a, const char* who) {
     CeLevel l{};
     l.lsum = (const double*)(ws + k.o_lsum); l.n = (int)(k.Pp / 64); l.sign = a.sign; l.mean_valid = a.mean_valid; l.slots = slots; l.nslots = nslots; l.P = k.P; l.loss = a.loss;
     if (need_grad) {
-      l.rowmax = rowmax; l.nrow = nrow; l.fx = fx; l.gp = gp; l.fw = fw; l.fx2 = f32(k.o_fx2); l.fw2 = f32(k.o_fw2); l.x = x; l.w = w; l.xpl = xpl; l.wpl = wpl;
+      l.rowmax = rowmax; l.nrow = nrow; l.fx = fx; l.gp = gp; l.fw = fw; l.bpad = bp; l.fx2 = f32(k.o_fx2); l.fw2 = f32(k.o_fw2); l.x = x; l.w = w; l.xpl = xpl; l.wpl = wpl;
       l.xp = k.xp; l.wp = k.wp; l.V = a.V; l.Vp = k.Vp; l.Cp = k.Cp; l.Pp = k.Pp; l.scal = scal;
     }
     const int blocks = need_grad ? (int)std::min<long>(kNumCU, (k.Vp + k.Pp) / 256) : 1;        // (every workgroup finds the largest exponents for itself)

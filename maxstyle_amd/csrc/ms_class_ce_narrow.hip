@@ -70,7 +70,8 @@ __global__ __launch_bounds__(256) void cn_prep_kernel(const void* __restrict__ w
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
       const int i = k * 256 + threadIdx.x, r = i / kW, c = i % kW;
-      x[k] = (v0 + r < V && c < C) ? IO::ld1(w, (size_t)(v0 + r) * C + c) : 0.f;
+      // a class that is switched off (b = -inf) may hold anything finite: its logit is -inf, and it sets no scale
+      x[k] = (v0 + r < V && c < C && (b == nullptr || b[v0 + r] != -__builtin_inff())) ? IO::ld1(w, (size_t)(v0 + r) * C + c) : 0.f;
       const unsigned bits = __float_as_uint(x[k]) & 0x7FFFFFFFu;
       am = max(am, bits < 0x7F800000u ? bits : 0u);          // (an infinity or NaN spoils its own class only)
     }

@@ -29,7 +29,7 @@ def cases(narrow):
     F, B = 0, 1
     shape, V = ((1, 64, 16, 16), 151) if narrow else ((256, 136), 700)
     for hb, wb in ((F, F), (B, F), (F, B), (B, B)):
-        for name in ("plain", "zero row", "zero class", "both", "both, small", "padded", "spread rows", "spread classes", "spread gradients", "large row", "confident", "one channel"):
+        for name in ("plain", "zero row", "zero class", "both", "both, small", "padded", "spread rows", "spread classes", "spread gradients", "large row", "switched off", "confident", "one channel"):
             rng = np.random.default_rng(5)
             if name == "one channel":
                 if narrow:
@@ -59,6 +59,9 @@ def cases(narrow):
                 w *= 2.0 ** rng.uniform(-15 if narrow else -30, 0, (V, 1))
             if name == "spread gradients":
                 grad = grad * 2.0 ** rng.uniform(-30, 0, P)
+            if name == "switched off":          # ... classes whose weights are anything finite
+                w[3::7], b[3::7] = 1e30, -np.inf
+                lab[np.isin(lab, np.arange(3, V, 7))] += 1
             if name == "large row":
                 hr[7] *= 1e6 if narrow else 1e4
             h = np.moveaxis(hr.reshape((shape[0],) + shape[2:] + (C,)), -1, 1).astype(np.float32)

@@ -11,7 +11,7 @@ from maxstyle_amd import ops
 
 pytestmark = pytest.mark.gpu
 F, B = torch.float32, torch.bfloat16
-CASES = ["plain", "zero row", "zero class", "both", "both, small", "padded", "spread rows", "spread classes", "spread gradients", "large row", "all classes zero", "all rows zero"]
+CASES = ["plain", "zero row", "zero class", "both", "both, small", "padded", "spread rows", "spread classes", "spread gradients", "large row", "switched off", "all classes zero", "all rows zero"]
 
 
 def rows_of(t):
@@ -40,6 +40,10 @@ def make(name, shape, V, hdt, wdt, narrow):
         w = w * spread(V, 15 if narrow else 30).unsqueeze(1)
     if name == "spread gradients":
         gr = gr * spread(P, 30)
+    if name == "switched off":          # ... classes whose weights are anything finite
+        off = torch.arange(V) % 7 == 3
+        w[off], b[off] = 1e30, float("-inf")
+        lab[off[lab]] += 1
     if name == "large row":
         hr[7] *= 1e6 if narrow else 1e4
     if name == "all classes zero":
