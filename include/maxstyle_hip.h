@@ -579,6 +579,9 @@ MS_STABLE int ms_head_ce_ds(const float* h, const float* w, const float* b, cons
  * h [N][C][HW] (rows of features [T][C]: N = T, HW = 1), w [V][C], b [V] or NULL, labels [N][HW]; dh like h, dw like w.  types: bit 0 h / dh are bf16, bit 1 w / dw
  * are bf16, otherwise fp32; b, db, loss, nll, lse are fp32.  Up to 8192 channels, 2^20 classes, 2^30 rows.  A row whose label is not a class gives nothing to the
  * loss and exactly 0 to every gradient, whatever its features hold; b may be -infinity for classes that are switched off.
+ * Numbers: an fp32 element of h or w enters the products to 2^-22 of itself or 2^-39 of the largest of its row (up to 128 channels: of 64 neighbouring classes), a bf16
+ * one as it is; G = g (softmax - hot) to 2^-22 of itself or 2^-41 g, or 2^-11 and 2^-29 g where h AND w are bf16 - for rows, classes and upstream gradients g within
+ * 2^30 of the largest; sums are fp32 or wider.  softmax = exp(z - lse) carries 2^-23 |lse|.
  * ms_class_ce_fwd: nll and lse of every row, ms_class_ce_bwd: the gradients for an upstream gradient of every row (grad [N][HW]) and the lse of that forward.
  * Deterministic.  ws: ms_class_ce_ws_bytes(.., need_grad = 1 when any gradient is asked for), 16-byte aligned, free again when the stream has passed the call. */
 MS_STABLE size_t ms_class_ce_ws_bytes(int N, int C, int V, int HW, int types, int need_grad);

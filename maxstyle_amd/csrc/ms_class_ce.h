@@ -9,7 +9,7 @@
 // (11 + 11 bits, x = hi + lo to 2^-22 relative or 2^-39 of the row's largest; where lo is kept 2^12 times as large, 2^-51), a bf16 value (8 bits) into one, exactly down to
 // 2^-37 of the row's largest.
 // A product of two-plane operands is hi hi + hi lo + lo hi (lo lo is below 2^-22): three matrix instructions for fp32 x fp32, two for bf16 x fp32, one for
-// bf16 x bf16.  fp32's own matrix instruction does 1/16 of the fp16 rate, so three of these are 5 times its speed at its accuracy.
+// bf16 x bf16; G has two planes unless h and w are both bf16.  fp32's own matrix instruction does 1/16 of the fp16 rate, so three of these are 5 times its speed at its accuracy.
 #pragma once
 #include "ms_common.h"
 

@@ -181,7 +181,7 @@ __global__ __launch_bounds__(256) void ce_rowgrad_kernel(const float* __restrict
 // exponents, r = ex, a row (class) far smaller than the largest would have its G' far below the largest although neither dh of the row nor dw of the class depends on its size, and a row
 // of zeros has no exponent at all.  So every row's exponent of g_p 2^r[p], and every c[v], is brought to at least the largest less kCeWindow - rows of zeros for nothing, others by
 // dividing their planes by that much, as long as these keep 24 bits of the row's largest (kCeMove1 / 2: one / two planes).  Within 2^30 of the largest, G' is held to 2^-22 of itself
-// (one plane: 2^-12) or 2^-41 (2^-30) g_p, whatever the row's and the class's size are.  Rows within the window, the ordinary case, are not touched.
+// (one plane: 2^-11) or 2^-41 (2^-29) g_p, whatever the row's and the class's size are.  Rows within the window, the ordinary case, are not touched.
 // A class that is switched off (b = -inf) may hold anything finite and sets no scale; where it holds more than 4 times the largest of the others its planes are cleared (its G is 0, but
 // for a row with this very label, whose loss is infinite).
 constexpr int kCeWindow = 4, kCeMove1 = 16, kCeMove2 = 26, kCeClear = 1000;
@@ -848,8 +848,7 @@ static int ce_run(const CeArgs& a, const char* who) {
       if (a.dh != nullptr) {        // dh^T [channels][pixels] = w^T G^T, or dh [rows][channels] = G w where the channels are neighbours
         CeGemm& o = gh;
         const CeOperand ow{w + (size_t)v0 * k.Cp, wpl, k.Cp, k.Cp}, og{G, gpl, k.vb, 0};
-        const int pw = hb ? 1 : k.wp, pg = hb ? 1 : 2;
-        if (rows_form) ce_pairs(o, pg, pw); else ce_pairs(o, pw, pg);
+        if (rows_form) ce_pairs(o, k.gpl, k.wp); else ce_pairs(o, k.wp, k.gpl);
         o.ksteps = cdiv(vr, kCeBK); o.split = std::min(k.split_x, std::max(1, o.ksteps * o.nseg / kCeDeep));
         o.out = f32(k.o_px); o.out_split = (size_t)cp * k.pb;
         if (rows_form) {
@@ -866,7 +865,7 @@ static int ce_run(const CeArgs& a, const char* who) {
       if (a.dw != nullptr) {        // dw [classes][channels] = G^T h
         CeGemm& o = gw;
         o.a = CeOperand{G, gpl, k.vb, k.vb}; o.b = CeOperand{x + (size_t)p0 * k.Cp, xpl, k.Cp, k.Cp};
-        ce_pairs(o, wb ? 1 : 2, wb ? 1 : k.xp);
+        ce_pairs(o, k.gpl, k.xp);
         o.ksteps = cdiv(rows, kCeBK); o.split = std::min(k.split_w, std::max(1, o.ksteps * o.nseg / kCeDeep));
         o.out = f32(k.o_pw); o.out_ld = (int)cp; o.out_split = (size_t)k.vb * cp;
         tw = ce_tile<CE_OUT>(vr, a.C, o.split, vn, cp);

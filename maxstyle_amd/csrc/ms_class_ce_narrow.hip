@@ -338,7 +338,7 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
           for (int j = 0; j < NJ; ++j) o[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh, gh[j], o[c][j], 0, 0, 0);
 #pragma unroll
           for (int j = 0; j < NJ; ++j) o[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh, gl[j], o[c][j], 0, 0, 0);
-          if (WP == 2 && HP == 2) {         // (a bf16 dh is the gradient of w held to 11 bits)
+          if (WP == 2) {                    // (also for a bf16 dh: where the classes' weights are nearly equal dh is their difference)
             const ms_h8 wl = cn_tr2<KS>(wp + IM::kPlane, h2 * 32, h2 * 32 + 16, c * 16, lane);
 #pragma unroll
             for (int j = 0; j < NJ; ++j) o[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wl, gh[j], o[c][j], 0, 0, 0);
@@ -379,7 +379,7 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
     if (DH) {
       const size_t wrow = (size_t)max(lab[j], 0) * a.C;
       const float f = scale * fac;
-      float wl[CT][4];                    // the label's weights, rounded as the products' were (16 bytes a lane: 4-byte loads from 64 rows at once cost 100 us a million pixels)
+      float wl[CT][4];                    // the label's weights (16 bytes a lane: 4-byte loads from 64 rows at once cost 100 us a million pixels)
       if (a.w_vec) {
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
@@ -391,15 +391,6 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
         for (int c = 0; c < CT; ++c)
 #pragma unroll
           for (int r = 0; r < 4; ++r) wl[c][r] = ActIO<WT>::ld1(a.w, wrow + min(c * 16 + q * 4 + r, a.C - 1));
-      }
-      if (HP == 1 && WP == 2) {
-#pragma unroll
-        for (int c = 0; c < CT; ++c)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const unsigned u = __float_as_uint(wl[c][r]);
-            wl[c][r] = __uint_as_float((u + 0xFFFu + ((u >> 13) & 1u)) & ~0x1FFFu);
-          }
       }
 #pragma unroll
       for (int c = 0; c < CT; ++c)
@@ -583,7 +574,7 @@ __global__ __launch_bounds__(256, 2) void cn_classes_kernel(CnwArgs a) {
             }
         }
         ms_h8 gh[NJ], gl[NJ];
-        constexpr bool kG2 = WP == 2;          // planes of G: two for an fp32 dw
+        constexpr bool kG2 = HP == 2 || WP == 2;          // planes of G: one where nothing is fp32
         bool here = false;
         int y4[2][4];
 #pragma unroll

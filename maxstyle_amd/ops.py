@@ -474,7 +474,10 @@ def class_ce(h, w, b, labels, loss_sign=1.0, mean_over="all", need_dh=True, need
     h [N,C,*spatial] or rows [T,C], fp32 or bf16; w [V,C] (or [V,C,1,1]), fp32 or bf16; b [V] fp32 or None; labels [N,*spatial] int64.  A label outside [0,V) takes its
     row out: nothing in the loss, exactly 0 in the gradients, whatever its features hold.  mean_over: "all" rows (cross_entropy_2D's mean) or the "valid" ones.
     grad_scale: an upstream gradient, a 1-element fp32 CUDA tensor (read on the device).  Runs on the current stream, can be captured into a graph, gives the same bits
-    every time."""
+    every time.
+
+    Products are fp32-accurate wherever h or w is fp32 (2^-22 an element, fp32 sums).  Where both are bf16, softmax - hot is rounded to fp16's 11 bits before the products
+    that make dh and dw."""
     if mean_over not in ("all", "valid"):
         raise ValueError("class_ce: mean_over is 'all' or 'valid'")
     N, C, V, HW, types = _class_ce_args(h, w, b, labels)

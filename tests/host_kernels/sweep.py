@@ -4,7 +4,7 @@ A read or write outside a buffer ends the process; margins that a page cannot gu
 printed before it runs.  class_ce_pieces: the limits of a piece and of the larger tiles lowered, so that small inputs take several pieces and every tile size.
 
 Tolerances of class_ce (u = 2^-24): logits |dz| <= A (3 2^-22 + (3 C + 8) u), A = sum_c |w h| + |b|; G relative 2 |dz| + 2^-21 and 2 u; its planes and the other operand's 3 2^-22, or
-2^-11 each where the call is all bf16 or the gradient's other operand is held in one plane; sums of 3 terms a step; half a step of the result's type."""
+G's 2^-11 where h and w are both bf16; sums of 3 terms a step; half a step of the result's type."""
 import random
 import sys
 
@@ -32,7 +32,7 @@ def class_ce_bounds(e, h, w, b, hb, wb):
     dz = A * (3 * 2.0 ** -22 + (3 * C + 8) * U)
     mag = e["rounded"]
     err = mag * ((2 * dz + 2.0 ** -21)[:, None] + 2 * U)
-    gx, gw = 2 * 2.0 ** -11 if hb else 3 * 2.0 ** -22, 2 * 2.0 ** -11 if wb else 3 * 2.0 ** -22
+    gx = gw = 2.0 ** -11 if hb and wb else 3 * 2.0 ** -22
     half = {0: U, 1: 2.0 ** -8}
     planes = lambda a: np.moveaxis(a.reshape((h.shape[0],) + h.shape[2:] + (C,)), -1, 1)
     tdh = planes(err @ np.abs(wd) + mag @ np.abs(wd) * (gx + (3 * V + 8) * U)) + half[hb] * np.abs(e["dh"])
