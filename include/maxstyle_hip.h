@@ -571,6 +571,11 @@ MS_STABLE int ms_head_ce(const float* h, const float* w, const float* b, const i
 MS_STABLE int ms_head_ce_ds(const float* h, const float* w, const float* b, const int64_t* labels, float* dh, float* logits, float* loss_out,
                   const int* loss_slot_dev, int N, int C, int K, int HW, float loss_sign, const float* grad_scale_dev, void* ws, size_t ws_bytes, void* stream);
 
+/* Mean softmax cross entropy of logits as they are, any number of classes (custom_loss.py:1043-1078): loss_out[0] = loss_sign * sum_p (log sum_k exp z[n,k,hw] - z[n,labels,hw]) / (N*HW);
+ * a label outside [0,K) adds nothing.  logits [N][K][HW] fp32, read once; masked classes may be anything down to -infinity.  Deterministic.  ws: ms_logit_ce_ws_bytes(), 8-byte aligned. */
+MS_STABLE size_t ms_logit_ce_ws_bytes(void);
+MS_STABLE int ms_logit_ce(const float* logits, const int64_t* labels, float* loss_out, int N, int K, int HW, float loss_sign, void* ws, size_t ws_bytes, void* stream);
+
 /* ---- head + softmax cross entropy over MANY classes, the logits never kept ------------------------------------------------------------------------
  * ms_head_ce's operator without its limits (K <= 4, C <= 64), with all gradients in the one call:
  *   z[p,v] = sum_c w[v,c] h[p,c] + b[v];  lse[p] = log sum_v exp z[p,v];  nll[p] = lse[p] - z[p,labels[p]], 0 where the label is outside [0,V)

@@ -162,6 +162,8 @@ SIGNATURES = {
     "ms_class_ce": (c_int, [c_void, c_void, c_f32p, c_i64p, c_f32p, c_void, c_void, c_f32p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_f32p, c_void, c_size, c_void]),
     "ms_class_ce_fwd": (c_int, [c_void, c_void, c_f32p, c_i64p, c_f32p, c_f32p, c_int, c_int, c_int, c_int, c_int, c_void, c_size, c_void]),
     "ms_class_ce_bwd": (c_int, [c_void, c_void, c_f32p, c_i64p, c_f32p, c_f32p, c_void, c_void, c_f32p, c_int, c_int, c_int, c_int, c_int, c_void, c_size, c_void]),
+    "ms_logit_ce_ws_bytes": (c_size, []),
+    "ms_logit_ce": (c_int, [c_f32p, c_i64p, c_f32p, c_int, c_int, c_int, c_float, c_void, c_size, c_void]),
     "ms_act8_block": (c_int, []),
     "ms_act8_pack": (c_int, [c_f32p, c_f32p, c_void, c_f32p, c_int, c_int, c_int, c_void]),
     "ms_act8_unpack": (c_int, [c_void, c_f32p, c_f32p, c_f32p, c_int, c_int, c_int, c_void]),

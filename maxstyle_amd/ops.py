@@ -528,6 +528,26 @@ def class_ce_bwd(h, w, b, labels, lse, grad, need_dh=True, need_dw=True):
     return dh, dw, db
 
 
+def logit_ce(logits, labels, loss_sign=1.0):
+    """loss_sign * mean softmax cross entropy of `logits` [N,K,*spatial] fp32 against `labels` [N,*spatial] int64 (ms_logit_ce), a 0-dim tensor; any K.  One read of the logits as they are: a
+    class may be masked with anything down to -inf.  A label outside [0,K) adds nothing to the sum; the mean is over all pixels."""
+    _need_cuda_f32(logits)
+    if logits.dim() < 2 or logits.numel() == 0:
+        raise ValueError("logit_ce: logits are [N,K,*spatial], not empty")
+    N, K = logits.shape[:2]
+    if labels.dtype != torch.int64 or not labels.is_cuda or not labels.is_contiguous() or labels.device != logits.device:
+        raise TypeError("labels must be a contiguous int64 tensor [N,*spatial] on the device of the logits")
+    if tuple(labels.shape) != (N,) + tuple(logits.shape[2:]):
+        raise ValueError(f"logit_ce: labels must be {(N,) + tuple(logits.shape[2:])}; got {tuple(labels.shape)}")
+    if labels.numel() > 1 << 30:
+        raise ValueError("logit_ce: supported up to 2^30 pixels")
+    with _on(logits.device):
+        out = torch.empty((), device=logits.device, dtype=torch.float32)
+        ws = torch.empty(lib.ms_logit_ce_ws_bytes(), dtype=torch.uint8, device=logits.device)
+        check(lib.ms_logit_ce(logits.data_ptr(), labels.data_ptr(), out.data_ptr(), N, K, labels.numel() // N, float(loss_sign), ws.data_ptr(), ws.numel(), _stream()), "ms_logit_ce")
+    return out
+
+
 # ---------------------------------------------------------------------------------------------------------
 # activation checkpoints in 8 bits
 # ---------------------------------------------------------------------------------------------------------

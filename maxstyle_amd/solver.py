@@ -26,9 +26,9 @@ def cross_entropy_2D(input, target, weight=None, size_average=True):
     if weight is not None or not size_average or target.dim() != 3:
         raise NotImplementedError("only the un-weighted, size-averaged label-map form used by the MaxStyle loop")
     n, c, h, w = input.shape
-    eye = torch.eye(c, device=input.device, dtype=torch.float32)
     if c > ops.HEAD_MAX_CLASSES:             # more classes than the small head's kernels hold
-        return ops.class_ce(input.contiguous().float(), eye, None, target.contiguous(), need_dh=False, need_dw=False)[0]
+        return ops.logit_ce(input.contiguous().float(), target.contiguous())
+    eye = torch.eye(c, device=input.device, dtype=torch.float32)
     loss, _, _ = ops.head_ce(input.contiguous().float(), eye, None, target.contiguous(), loss_sign=1.0, need_dh=False)
     return loss[0]
 

@@ -1,4 +1,4 @@
-"""Random calls of the kernels' host build, every buffer between unmapped pages: python sweep.py class_ce|class_ce_pieces|act8 SEED COUNT.
+"""Random calls of the kernels' host build, every buffer between unmapped pages: python sweep.py class_ce|class_ce_pieces|logit_ce|act8 SEED COUNT.
 
 A read or write outside a buffer ends the process; margins that a page cannot guard are checked; results are compared with the definition in 64 bits.  The case is
 printed before it runs.  class_ce_pieces: the limits of a piece and of the larger tiles lowered, so that small inputs take several pieces and every tile size.
@@ -76,6 +76,39 @@ def class_ce(r, lib, show):
             assert (np.abs(o[k] - e[k]) <= t[k]).all(), k
 
 
+def logit_ce(r, lib, show):
+    while True:
+        N, K, HW = log(r, 1, 6), log(r, 1, 3000), log(r, 1, 3000)
+        if N * K * HW <= 400000:
+            break
+    HW = HW // 4 * 4 if r.random() < 0.5 and HW >= 4 else HW
+    mode, align, mask = r.choice(["end", "start"]), r.choice([16, 4]), r.choice([None, -1e4, -1e12, -3.4028234663852886e38, -np.inf])
+    rng = np.random.default_rng(r.randrange(1 << 30))
+    z = (3 * rng.standard_normal((N, K, HW))).astype(np.float32)
+    lab = rng.integers(0, K, (N, HW))
+    if mask is not None:
+        keep = rng.random((N, K, HW)) < 0.5
+        np.put_along_axis(keep, lab[:, None], True, 1)
+        z = np.where(keep, z, np.float32(mask))
+    lab[rng.random(lab.shape) < 0.1] = r.choice([-1, K, -100])
+    show(N, K, HW, mode, align, mask)
+    c = g.Call(mode)
+    Z, L, out = c.put(z, align), c.put(lab.astype(np.int64), 8), c.block(4, 4)
+    lib.ms_logit_ce_ws_bytes.restype = g.ctypes.c_size_t
+    ws = c.block(lib.ms_logit_ce_ws_bytes(), 8)
+    assert lib.ms_logit_ce(g.p(Z), g.p(L), g.p(out), N, K, HW, g.ctypes.c_float(1.0), g.p(ws), g.ctypes.c_size_t(ws.nbytes), None) == 0
+    got = float(out.array(np.float32, (1,))[0])
+    assert c.done()
+    zd = z.astype(np.float64)
+    m = zd.max(1)
+    with np.errstate(all="ignore"):
+        lse = m + np.log(np.exp(zd - m[:, None]).sum(1))
+    ok = (lab >= 0) & (lab < K)
+    nll = np.where(ok, lse - np.take_along_axis(zd, np.where(ok, lab, 0)[:, None], 1)[:, 0], 0)
+    # exponents to 2 u |z - max| log2(e), of at most 30 where a term counts; K fp32 additions; the difference and the logarithm 4 u of their size
+    assert abs(got - nll.sum() / nll.size) <= (K + 100) * U + 8 * U * (np.abs(nll).sum() / nll.size + 1), (got, nll.sum() / nll.size)
+
+
 def act8(r, lib, show):
     while True:
         shape = (log(r, 1, 40), log(r, 1, 300), log(r, 1, 400), log(r, 1, 400)) if r.random() < 0.7 else (1, log(r, 1, 3), log(r, 100, 700), log(r, 100, 700))
@@ -119,7 +152,7 @@ def act8(r, lib, show):
 
 
 def main(which, seed, count):
-    run, lib = {"class_ce": class_ce, "class_ce_pieces": class_ce, "act8": act8}[which], build.load(PIECES if which == "class_ce_pieces" else None)
+    run, lib = {"class_ce": class_ce, "class_ce_pieces": class_ce, "act8": act8, "logit_ce": logit_ce}[which], build.load(PIECES if which == "class_ce_pieces" else None)
     r = random.Random(seed)
     for i in range(count):
         run(r, lib, lambda *case: print(which, seed, i, *case, flush=True))

@@ -57,3 +57,14 @@ def test_sizes_that_no_launch_holds_are_refused():
     with pytest.raises(ValueError, match="2\\^31"):
         ops._act8_dims((1, 1, 1 << 16, 1 << 16), "act8_pack")
     assert lib.ms_class_ce_ws_bytes(1 << 15, 8, 5, (1 << 15) + 1, 0, 1) == 0
+
+
+def test_logit_ce_refuses_before_any_launch():
+    buf = ctypes.create_string_buffer(1 << 15)
+    p = (ctypes.addressof(buf) + 15) & ~15
+    n = lib.ms_logit_ce_ws_bytes()
+    assert lib.ms_logit_ce(p, p, p, 0, 5, 4, 1.0, p, n, 0) == -1 and lib.ms_logit_ce(p, p, p, 1 << 15, 5, (1 << 15) + 1, 1.0, p, n, 0) == -1
+    assert lib.ms_logit_ce(0, p, p, 1, 5, 4, 1.0, p, n, 0) == -1 and lib.ms_logit_ce(p, p, 0, 1, 5, 4, 1.0, p, n, 0) == -1
+    assert lib.ms_logit_ce(p, p, p, 1, 5, 4, 1.0, p, n - 1, 0) == -3 and lib.ms_logit_ce(p, p, p, 1, 5, 4, 1.0, p + 4, n, 0) == -2
+    with pytest.raises(RuntimeError, match="MI355X only"):
+        ops.logit_ce(torch.randn(1, 5, 4, 4), torch.zeros(1, 4, 4, dtype=torch.int64))
