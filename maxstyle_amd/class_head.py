@@ -32,8 +32,12 @@ def class_cross_entropy(h, weight, bias, labels, reduction="mean"):
     eager graph still holds ends the process, so a call that would record one raises."""
     if reduction not in ("mean", "valid", "sum", "none"):
         raise ValueError("class_cross_entropy: reduction is 'mean', 'valid', 'sum' or 'none'")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (h, weight, bias)) and h.is_cuda and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("class_cross_entropy: not under graph capture with gradients; capture ops.class_ce (loss and gradients in one call)")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (h, weight, bias)):
+        if h.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("class_cross_entropy: not under graph capture with gradients; capture ops.class_ce (loss and gradients in one call)")
+    elif reduction != "none":            # value only: summed by the operator's own kernels (a library sum over many blocks would put a memset into a captured graph)
+        return ops.class_ce(h, weight, bias, labels, loss_sign=float(labels.numel()) if reduction == "sum" else 1.0, mean_over="valid" if reduction == "valid" else "all",
+                            need_dh=False, need_dw=False)[0]
     nll = _ClassCrossEntropy.apply(h, weight, bias, labels)
     if reduction == "none":
         return nll
