@@ -18,9 +18,8 @@ class _ClassCrossEntropy(torch.autograd.Function):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("class_cross_entropy: its backward cannot be captured into a graph; capture ops.class_ce or ops.class_ce_bwd")
         h, weight, bias, labels, lse = ctx.saved_tensors
-        need_b = bias is not None and ctx.needs_input_grad[2]
-        dh, dw, db = ops.class_ce_bwd(h, weight, bias, labels, lse, grad.float().contiguous(), need_dh=ctx.needs_input_grad[0], need_dw=ctx.needs_input_grad[1] or need_b)
-        return dh, (dw if ctx.needs_input_grad[1] else None), (db if need_b else None), None
+        dh, dw, db = ops.class_ce_bwd(h, weight, bias, labels, lse, grad.float().contiguous(), *ctx.needs_input_grad[:3])
+        return dh, dw, db, None
 
 
 def class_cross_entropy(h, weight, bias, labels, reduction="mean"):

@@ -509,19 +509,20 @@ def class_ce_fwd(h, w, b, labels):
     return nll, lse
 
 
-def class_ce_bwd(h, w, b, labels, lse, grad, need_dh=True, need_dw=True):
-    """Gradients (dh, dw, db) of sum(grad * nll) for class_ce_fwd's nll, from its inputs and its lse (ms_class_ce_bwd).  grad [N,*spatial] fp32."""
+def class_ce_bwd(h, w, b, labels, lse, grad, need_dh=True, need_dw=True, need_db=None):
+    """Gradients (dh, dw, db) of sum(grad * nll) for class_ce_fwd's nll, from its inputs and its lse (ms_class_ce_bwd).  grad [N,*spatial] fp32.  need_db: as need_dw unless said."""
     N, C, V, HW, types = _class_ce_args(h, w, b, labels)
     _need_cuda_f32(lse, grad)
     for t in (lse, grad):
         if t.shape != labels.shape or t.device != h.device:
             raise ValueError("class_ce_bwd: lse and grad have the shape and the device of labels")
-    if not (need_dh or need_dw):
+    need_db = (need_dw if need_db is None else need_db) and b is not None
+    if not (need_dh or need_dw or need_db):
         return None, None, None
     with _on(h.device):
         dh = torch.empty_like(h) if need_dh else None
         dw = torch.empty_like(w) if need_dw else None
-        db = torch.empty_like(b) if (need_dw and b is not None) else None
+        db = torch.empty_like(b) if need_db else None
         ws = _class_ce_ws(N, C, V, HW, types, True, h.device)
         check(lib.ms_class_ce_bwd(h.data_ptr(), w.data_ptr(), _ptr(b), labels.data_ptr(), lse.data_ptr(), grad.data_ptr(), _ptr(dh), _ptr(dw), _ptr(db), N, C, V, HW, types,
                                   ws.data_ptr(), ws.numel(), _stream()), "ms_class_ce_bwd")

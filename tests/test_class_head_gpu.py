@@ -54,3 +54,25 @@ def test_no_sum_of_the_library_is_captured(monkeypatch):
         with torch.no_grad():
             maxstyle_amd.class_cross_entropy(h, w, b, lab, reduction=reduction)
     assert not used
+
+
+@pytest.mark.parametrize("shape,V", [((2, 64, 20, 20), 50), ((300, 136), 700)])
+def test_only_what_is_asked_for(shape, V, monkeypatch):
+    """Every subset of the gradients has the bits of the whole call, and nothing else is computed or returned."""
+    h, w, b, lab = make(shape, V, 3)
+    gr = torch.randn(lab.shape, generator=torch.Generator().manual_seed(1)).cuda()
+    lse = ops.class_ce_fwd(h, w, b, lab)[1]
+    whole = ops.class_ce_bwd(h, w, b, lab, lse, gr)
+    for k in range(1, 8):
+        need = [bool(k & 1), bool(k & 2), bool(k & 4)]
+        got = ops.class_ce_bwd(h, w, b, lab, lse, gr, *need)
+        for a, c, n in zip(got, whole, need):
+            assert (a is None) if not n else torch.equal(a, c)
+        seen = []
+        inner = ops.class_ce_bwd
+        monkeypatch.setattr(ops, "class_ce_bwd", lambda *a, **kw: seen.append(inner(*a, **kw)) or seen[-1])
+        leaves = [t.clone().requires_grad_(n) for t, n in zip((h, w, b), need)]
+        (maxstyle_amd.class_cross_entropy(*leaves, lab, reduction="none") * gr).sum().backward()
+        monkeypatch.setattr(ops, "class_ce_bwd", inner)
+        for t, c, n, made in zip(leaves, whole, need, seen[0]):
+            assert (t.grad is None and made is None) if not n else torch.equal(t.grad, c)
