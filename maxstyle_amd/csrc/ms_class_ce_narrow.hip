@@ -217,7 +217,10 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
   for (int j = 0; j < NJ; ++j) {
     key[j] = lab[j] >= 0 && ((lab[j] >> 2) & 3) == q ? lab[j] >> 5 : -1;
     m[j] = -__builtin_inff(); l[j] = 0.f; zl[j] = 0.f;
-    if (!online) m[j] = pw + j * 16 < P ? a.lse_in[pw + j * 16] * kLog2e : 0.f;
+    if (!online) {
+      m[j] = pw + j * 16 < P ? a.lse_in[pw + j * 16] * kLog2e : 0.f;
+      if (m[j] == -__builtin_inff()) m[j] = __builtin_nanf("");          // every class is switched off: there is no softmax
+    }
 #pragma unroll
     for (int c = 0; c < CT; ++c) o[c][j] = ms_f4{0.f, 0.f, 0.f, 0.f};
   }

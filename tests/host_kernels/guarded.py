@@ -164,7 +164,7 @@ def exact_ce(h, w, b, lab, hb, wb, mean_valid, grad=None, sign=1.0, dtype=np.flo
     G = np.where(ok[:, None], G * g[:, None], 0).astype(dtype)
     planes = lambda a: np.moveaxis(a.reshape((h.shape[0],) + h.shape[2:] + (h.shape[1],)), -1, 1)
     return dict(loss=sign * float(nll.astype(np.float64).sum()) / n, nll=nll, lse=(m + np.log(t))[:, 0], dh=planes(G @ wd), dw=G.T @ x, db=G.sum(0), G=G, ok=ok,
-                rounded=mag, zmax=float(np.abs(z[e > 0]).max()), mdh=planes(mag @ np.abs(wd)), mdw=mag.T @ np.abs(x),
+                rounded=mag, zmax=float(np.abs(z[e > 0]).max(initial=0)), mdh=planes(mag @ np.abs(wd)), mdw=mag.T @ np.abs(x),
                 tdh=planes(np.repeat(np.abs(g)[:, None], V, 1) @ np.abs(wd)), tdw=np.repeat(np.abs(g)[None], V, 0) @ np.abs(x))
 
 

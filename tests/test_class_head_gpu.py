@@ -76,3 +76,16 @@ def test_only_what_is_asked_for(shape, V, monkeypatch):
         monkeypatch.setattr(ops, "class_ce_bwd", inner)
         for t, c, n, made in zip(leaves, whole, need, seen[0]):
             assert (t.grad is None and made is None) if not n else torch.equal(t.grad, c)
+
+
+@pytest.mark.parametrize("shape,V", [((1, 16, 8, 8), 70), ((40, 136), 300)])
+def test_every_class_switched_off(shape, V):
+    """There is no softmax then: loss and gradients are NaN, as the definition's, whichever entry makes them; rows without a class still get exactly 0."""
+    h, w, b, lab = make(shape, V, 4)
+    b = torch.full_like(b, float("-inf"))
+    ok = (lab >= 0).reshape(-1)
+    rows = lambda t: t.movedim(1, -1).reshape(-1, t.shape[1])
+    nll, lse = ops.class_ce_fwd(h, w, b, lab)
+    assert torch.isnan(nll.reshape(-1)[ok]).all() and (nll.reshape(-1)[~ok] == 0).all()
+    for loss, dh, dw, db in (ops.class_ce(h, w, b, lab), (nll.sum(),) + ops.class_ce_bwd(h, w, b, lab, lse, torch.ones_like(nll))):
+        assert torch.isnan(loss) and torch.isnan(rows(dh)[ok]).all() and (rows(dh)[~ok] == 0).all() and torch.isnan(dw).all() and torch.isnan(db).all()
