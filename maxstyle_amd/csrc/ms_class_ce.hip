@@ -246,7 +246,7 @@ __global__ __launch_bounds__(1024) void ce_level_kernel(CeLevel a) {
       const int e = ce_scale_exponent((cls ? a.fw : a.fx)[r0 + lane]), g = cls ? 0 : ce_grad_exponent(a.gp[r0 + lane]), top = (cls ? ew : er) - kCeWindow - g;
       int to = e == kCeNone ? 0 : e;
       if (g != kCeNone) {
-        if (e == kCeNone) to = min(max(top, -100), 120);
+        if (e == kCeNone) to = min(max(top, -126), 126);
         else to = min(max(e, min(top, e + (planes == 2 ? kCeMove2 : kCeMove1))), max(e, 120));
       }
       if (cls && e > ew + 2 && e != kCeNone) {          // (switched off)
