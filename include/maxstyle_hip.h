@@ -586,7 +586,7 @@ MS_STABLE int ms_logit_ce(const float* logits, const int64_t* labels, float* los
  * loss and exactly 0 to every gradient, whatever its features hold; b may be -infinity for classes that are switched off.
  * Numbers: an fp32 element of h or w enters the products to 2^-22 of itself or 2^-39 of the largest of its row (up to 128 channels: of 64 neighbouring classes), a bf16
  * one as it is; G = g (softmax - hot) to 2^-22 of itself or 2^-41 g, or 2^-11 and 2^-29 g where h AND w are bf16 - for rows, classes and upstream gradients g within
- * 2^30 of the largest; sums are fp32 or wider.  softmax = exp(z - lse) carries 2^-23 |lse|.
+ * 2^30 of the largest; sums are fp32 or wider.  ms_class_ce_bwd's softmax = exp(z - lse) carries the 2^-24 |lse| of the fp32 lse; ms_class_ce's does not.
  * ms_class_ce_fwd: nll and lse of every row, ms_class_ce_bwd: the gradients for an upstream gradient of every row (grad [N][HW]) and the lse of that forward.
  * Deterministic.  ws: ms_class_ce_ws_bytes(.., need_grad = 1 when any gradient is asked for), 16-byte aligned, free again when the stream has passed the call. */
 MS_STABLE size_t ms_class_ce_ws_bytes(int N, int C, int V, int HW, int types, int need_grad);

@@ -33,12 +33,21 @@ __device__ __forceinline__ int ce_exponent(float amax) {
 }
 __device__ __forceinline__ float ce_pow2(int e) { return __uint_as_float((unsigned)(min(max(e, -126), 127) + 127) << 23); }
 
-// log2(x 2^-less), x >= 0: the exponent apart from the logarithm of the mantissa in [1, 2).  The log instruction cuts its result off: of x = 2^9 .. 2^13 it would lie half a step of 8 .. 16
+// log2(x) - less, x >= 0 (less: a whole number): the exponent apart from the logarithm of the mantissa in [1, 2).  The log instruction cuts its result off: of x = 2^9 .. 2^13 it would lie half a step of 8 .. 16
 // (4.8e-7) too low on average, and the gradients of a few thousand rows add such a bias up (db 1.2e-6 instead of 1e-7 off).
-__device__ __forceinline__ float ce_log2(float x, int less = 0) {
+__device__ __forceinline__ float ce_log2(float x, float less = 0.f) {
   const int e = __builtin_amdgcn_frexp_expf(x) - 1;
-  return (float)(e - less) + __builtin_amdgcn_logf(__builtin_amdgcn_ldexpf(x, -e));
+  return ((float)e - less) + __builtin_amdgcn_logf(__builtin_amdgcn_ldexpf(x, -e));
 }
+
+// A log-sum L (in log2) is subtracted from logits as the fp32 value next to it; with what that leaves over, d = L - fp32(L) and c = 2^d, exp2(z - L) = exp2(z - fp32(L)) / c and
+// G = g (exp2(z - L) - hot) = g / c (exp2(z - fp32(L)) - c hot): the rounding of a log-sum of 40 (2^-19) costs nothing, and a row that is sure of its label keeps what is left of 1 - p.
+__device__ __forceinline__ float ce_rest(float m, float lg, float rounded) { return (m - rounded) + lg; }      // L = m + lg
+__device__ __forceinline__ float ce_rest_nat(float lse, float rounded) {                                       // L = lse log2(e)
+  const float d = __builtin_fmaf(lse, kLog2e, -rounded) + lse * 1.92596299112661746e-8f;
+  return fminf(fmaxf(d, -1.f), 1.f);                  // (beyond 2^24 the fp32 log-sum itself is whole units off)
+}
+__device__ __forceinline__ float ce_lse_nat(float m, float lg) { return (float)(((double)m + (double)lg) * 0.69314718055994530942); }
 
 // A product as fp32 holds it, for what is split: left to itself the compiler rounds the product to fp16 straight (v_fma_mixlo) where it forms hi and by way of fp32 (v_cvt) where it
 // forms lo, and for one element in some thousands the two planes then belong to different hi (2^-11 off).

@@ -159,14 +159,19 @@ __device__ __forceinline__ int ce_row_exponent(float g, float fx) {
 // The upstream gradient of every row: grad[p], 0 where the label is not a class.  A row without one gets a log-sum of infinity: exp(z - inf) = 0 whatever its logits are.
 // rowmax[workgroup]: the largest exponent of g_p 2^ex[p].
 __global__ __launch_bounds__(256) void ce_rowgrad_kernel(const float* __restrict__ grad, const int* __restrict__ lab32, const float* __restrict__ fx, float* __restrict__ gp,
-                                                         const float* __restrict__ lse_in, float* __restrict__ lse2, int* __restrict__ rowmax, long P, long Pp) {
+                                                         const float* __restrict__ lse_in, float* __restrict__ lse2, float* __restrict__ hot, int* __restrict__ rowmax, long P, long Pp) {
   __shared__ int red[4];
   int e = kCeNone;
   for (long p = (long)blockIdx.x * 256 + threadIdx.x; p < Pp; p += (long)gridDim.x * 256) {
     const float g = (p < P && lab32[p] >= 0) ? grad[p] : 0.f;
     e = max(e, ce_row_exponent(g, fx[p]));
-    gp[p] = g;
-    lse2[p] = g == 0.f ? __builtin_inff() : lse_in[p] * kLog2e;
+    float ls = __builtin_inff(), d = 0.f;
+    if (g != 0.f) {
+      ls = lse_in[p] * kLog2e;
+      d = ce_rest_nat(lse_in[p], ls);
+    }
+    gp[p] = g * __builtin_amdgcn_exp2f(-d);
+    lse2[p] = ls; hot[p] = __builtin_amdgcn_exp2f(d);
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) e = max(e, __shfl_xor(e, off, 64));
@@ -264,7 +269,7 @@ __global__ __launch_bounds__(1024) void ce_level_kernel(CeLevel a) {
   }
 }
 
-struct CeRowGrad { float* gp; const float* fx; float sign; int mean_valid; const float* scale_dev; const int* slots; int nslots; int* rowmax; };
+struct CeRowGrad { float *gp, *hot; const float* fx; float sign; int mean_valid; const float* scale_dev; const int* slots; int nslots; int* rowmax; };
 
 // part[t][p] = {max, sum exp} over one class range -> lse, nll; loss partials in 64 bits; with r.gp the rows' upstream gradients (ce_rowgrad_kernel's work).  64 rows a workgroup, 16 threads each over the class ranges.  All in units of log2.
 __device__ __forceinline__ void ce_merge(float& m, float& l, float mo, float lo) {
@@ -291,7 +296,8 @@ __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict_
   double acc = 0.0;
   if (rg.gp != nullptr) {
     const float g = (p < P && lab32[p] >= 0) ? rg.sign / (float)(rg.mean_valid ? max(cnt, 1) : P) * (rg.scale_dev != nullptr ? *rg.scale_dev : 1.f) : 0.f;
-    rg.gp[p] = g;
+    const float d = g == 0.f ? 0.f : ce_rest(m, lg, ls);
+    rg.gp[p] = g * __builtin_amdgcn_exp2f(-d); rg.hot[p] = __builtin_amdgcn_exp2f(d);
     if (g == 0.f) ls = __builtin_inff();
     int e = ce_row_exponent(g, rg.fx[p]);
 #pragma unroll
@@ -300,7 +306,7 @@ __global__ __launch_bounds__(1024) void ce_join_kernel(const float2* __restrict_
   }
   lse2[p] = ls;
   if (p < P) {
-    if (lse_out != nullptr) lse_out[p] = (m + lg) * ln2;
+    if (lse_out != nullptr) lse_out[p] = ce_lse_nat(m, lg);
     const float v = lab32[p] >= 0 ? ((m - zlab[p]) + lg) * ln2 : 0.f;        // (max - z) + log sum: nothing cancels where the label has the maximum
     if (nll_out != nullptr) nll_out[p] = v;
     acc = (double)v;
@@ -317,7 +323,7 @@ struct CeGemm {
   int ksteps;                     // K / 64 of one pair
   int mt, nt, split;
   // logits epilogues
-  const float *fw, *bpad, *fx; const int* lab; const float* lse; const float* gp; const int* scal;
+  const float *fw, *bpad, *fx; const int* lab; const float *lse, *gp, *hot; const int* scal;
   float2* part; size_t part_stride; float* zlab;
   _Float16* g; size_t g_plane; int g_ld; float* dbpart; size_t db_stride;
   int v0; long p0;                // first class / row of this piece
@@ -511,12 +517,12 @@ __device__ __forceinline__ void ce_gemm_tile(CeGemm g, int id, _Float16 (*sm)[(B
   }
   if (EPI == CE_GRAD || EPI == CE_GRAD2) {
     const float gn = ce_pow2(g.scal[0]);
-    float gp[NJ], ls[NJ], rj[NJ];
+    float gp[NJ], ls[NJ], rj[NJ], hot[NJ];
     bool here = false;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const size_t p = (size_t)g.p0 + n0 + wn * TN + j * 16 + li;
-      gp[j] = g.gp[p]; ls[j] = g.lse[p];
+      gp[j] = g.gp[p]; ls[j] = g.lse[p]; hot[j] = g.hot[p];
       rj[j] = gp[j] * g.fx[p] * gn;
       here |= (unsigned)lab[j] < (unsigned)(MI * 16);
     }
@@ -532,7 +538,7 @@ __device__ __forceinline__ void ce_gemm_tile(CeGemm g, int id, _Float16 (*sm)[(B
         for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r] * ff[r], fs[j], bb[r]) - ls[j]);
         if (here) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[i][j][r] -= lab[j] == i * 16 + r ? 1.f : 0.f;
+          for (int r = 0; r < 4; ++r) acc[i][j][r] -= lab[j] == i * 16 + r ? hot[j] : 0.f;
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -650,7 +656,7 @@ struct CePlan {
   int pb, vb;                    // rows / classes of a piece
   int nparts, sb;                // partial statistics of a row, rows whose statistics are formed at a time
   int split_x, split_w;
-  size_t o_x, o_w, o_fx, o_fw, o_fx2, o_fw2, o_b, o_lab, o_lse, o_zl, o_gp, o_part, o_scal, o_slots, o_rowmax, o_lsum, o_g, o_db, o_px, o_pw, o_ax, o_aw, total;
+  size_t o_x, o_w, o_fx, o_fw, o_fx2, o_fw2, o_hot, o_b, o_lab, o_lse, o_zl, o_gp, o_part, o_scal, o_slots, o_rowmax, o_lsum, o_g, o_db, o_px, o_pw, o_ax, o_aw, total;
 };
 static size_t ce_al(size_t n) { return (n + 255) & ~(size_t)255; }
 static long ce_up(long a, long b) { return (a + b - 1) / b * b; }
@@ -679,7 +685,7 @@ static CePlan ce_plan(int N, int C, int V, int HW, int types, bool grad) {
   // (two of a tile; 64-wide tiles, twice as many, are taken for less than 128 tiles of 128 x 128: 512 x 254 pairs at most)
   const size_t stats = std::max((size_t)k.nparts * k.sb * 8, (size_t)2 << 20);
   if (!grad) { k.o_part = take(stats); k.total = o; return k; }
-  k.o_fx2 = take(k.Pp * 4); k.o_fw2 = take((size_t)k.Vp * 4);
+  k.o_fx2 = take(k.Pp * 4); k.o_fw2 = take((size_t)k.Vp * 4); k.o_hot = take(k.Pp * 4);
   // The statistics are read before the first piece of G is written: they share its memory.
   k.o_part = o;
   k.o_g = take(std::max((size_t)k.gpl * k.pb * k.vb * 2, stats));
@@ -783,9 +789,10 @@ static int ce_run(const CeArgs& a, const char* who) {
     MS_LAUNCH(ce_count_kernel, dim3(nslots), dim3(256), 0, st, a.labels, k.P, a.V, slots);
     if (int e = check_launch("class_ce_count")) return e;
   }
-  const CeRowGrad rg{gp, fx, a.sign, a.mean_valid, a.scale_dev, slots, nslots, rowmax};
+  float* hot = need_grad ? f32(k.o_hot) : nullptr;
+  const CeRowGrad rg{gp, hot, fx, a.sign, a.mean_valid, a.scale_dev, slots, nslots, rowmax};
   CeGemm g{};
-  g.fw = fw; g.bpad = bp; g.fx = fx; g.lab = lab; g.lse = lse; g.gp = gp; g.scal = scal; g.zlab = zl;
+  g.fw = fw; g.bpad = bp; g.fx = fx; g.lab = lab; g.lse = lse; g.gp = gp; g.hot = hot; g.scal = scal; g.zlab = zl;
   if (a.lse_in == nullptr) {
     // logits -> statistics: M = classes, N = rows
     for (long p0 = 0; p0 < k.Pp; p0 += k.sb) {
@@ -804,7 +811,7 @@ static int ce_run(const CeArgs& a, const char* who) {
   }
   const int nrow = a.lse_in != nullptr ? (int)std::min<long>(k.Pp / 256, kCeRowBlocks) : (int)(k.Pp / 64);
   if (a.lse_in != nullptr) {
-    MS_LAUNCH(ce_rowgrad_kernel, dim3(nrow), dim3(256), 0, st, a.grad, lab, fx, gp, a.lse_in, lse, rowmax, k.P, k.Pp);
+    MS_LAUNCH(ce_rowgrad_kernel, dim3(nrow), dim3(256), 0, st, a.grad, lab, fx, gp, a.lse_in, lse, hot, rowmax, k.P, k.Pp);
     if (int e = check_launch("class_ce_rowgrad")) return e;
   }
   if (need_grad || a.loss != nullptr) {

@@ -143,7 +143,7 @@ struct CnArgs {
   const void *h, *w; const int64_t* labels; const char* img; const int* slots; int nslots;
   float *nll, *lse_out; const float *lse_in, *grad, *scale_dev; float sign; int mean_valid, drop;
   void* dh; double* lsum;
-  float *fx, *lse2, *gp; int* lab;          // what the class pass needs of every row (NULL: it does not run)
+  float *fx, *lse2, *gp, *hot; int* lab;    // what the class pass needs of every row (NULL: it does not run)
   long P; int C, HW, V, nch, w_vec;
   int full;                                 // C is the kernel's full width and h spans less than 4 GB: addresses are a scalar base and a 32-bit offset
 };
@@ -370,18 +370,23 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
     const int p = pw + j * 16;
-    float lse2 = m[j], fac = 1.f / 512.f;
-    if (online) {
+    float lse2 = m[j], fac = 1.f, rest = 0.f;
+    const float top = m[j] == -__builtin_inff() ? kCnTop : m[j] - (m[j] - kCnTop);          // what the exponentials were raised by (kCnTop where m holds it)
+    if (!online) {
+      rest = ce_rest_nat(a.lse_in[min(p, P - 1)], lse2);
+      fac = __builtin_amdgcn_exp2f(-top) * __builtin_amdgcn_exp2f(-rest);
+    } else {
       l[j] += __shfl_xor(l[j], 16, 64);
       l[j] += __shfl_xor(l[j], 32, 64);
       zl[j] += __shfl_xor(zl[j], 16, 64);             // (one lane of the four holds it, the others 0)
       zl[j] += __shfl_xor(zl[j], 32, 64);
       fac = 1.f / l[j];
-      const float lg = ce_log2(l[j], (int)kCnTop);
+      const float lg = ce_log2(l[j], top);
       lse2 = m[j] + lg;
+      rest = ce_rest(m[j], lg, lse2);
       const float ln2 = 0.693147180559945309f, nll = lab[j] >= 0 ? ((m[j] - zl[j]) + lg) * ln2 : 0.f;
       if (q == 0 && p < P) {
-        if (a.nll != nullptr) { a.nll[p] = nll; a.lse_out[p] = lse2 * ln2; }
+        if (a.nll != nullptr) { a.nll[p] = nll; a.lse_out[p] = ce_lse_nat(m[j], lg); }
         acc_l += (double)nll;
       }
     }
@@ -389,7 +394,8 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
     if (lab[j] >= 0) gp = a.grad != nullptr ? a.grad[p] : a.sign / cnt * (a.scale_dev != nullptr ? *a.scale_dev : 1.f);
     if (a.fx != nullptr) {
       if (q == 0) {                                   // (arrays padded to whole workgroups)
-        a.fx[p] = fx[j]; a.gp[p] = gp; a.lab[p] = lab[j];
+        const float d = gp == 0.f ? 0.f : rest;
+        a.fx[p] = fx[j]; a.gp[p] = gp * __builtin_amdgcn_exp2f(-d); a.hot[p] = __builtin_amdgcn_exp2f(d); a.lab[p] = lab[j];
         a.lse2[p] = gp == 0.f ? __builtin_inff() : lse2;        // a row that takes no part: exp2(z - inf) = 0 whatever z is
       }
     }
@@ -442,7 +448,7 @@ __global__ __launch_bounds__(256, 2) void cn_pixels_kernel(CnArgs a) {
 
 // ------------------------------------------------------------------------------------------------------------------------------ dw, db
 struct CnwArgs {
-  const void* h; const char* img; const float *fx, *lse2, *gp; const int* lab;
+  const void* h; const char* img; const float *fx, *lse2, *gp, *hot; const int* lab;
   float *dwp, *dbp; size_t dw_split; int db_split;
   long P; int C, HW, V, units, wpx, splits, tiles;
 };
@@ -456,7 +462,7 @@ __global__ __launch_bounds__(256, 2) void cn_classes_kernel(CnwArgs a) {
   using IM = CnImage<KS, WP>;
   constexpr int CT = CnW<KS>::kCT, KN = CnW<KS>::kN, KF = CnW<KS>::kF, kC = CnW<KS>::kW, kTasks = kC * (TP / 8) / 256;
   __shared__ __attribute__((aligned(1024))) _Float16 xs[HP * kC * TP];
-  __shared__ __attribute__((aligned(16))) float rows[4][TP];       // 2^ex, lse, g_p 2^ex, g_p
+  __shared__ __attribute__((aligned(16))) float rows[5][TP];       // 2^ex, lse, g_p 2^ex, g_p, the label's 1 in units of exp2(z - lse)
   __shared__ __attribute__((aligned(16))) int labs[TP];
   __shared__ int tmax[2];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q = lane >> 4, li = lane & 15;
@@ -491,7 +497,7 @@ __global__ __launch_bounds__(256, 2) void cn_classes_kernel(CnwArgs a) {
   if (threadIdx.x < 2) tmax[threadIdx.x] = -100000;
 
   float pre[kTasks][8];
-  float prow[3];
+  float prow[4];
   int plab;
   auto load = [&](int t) {
     const long p0 = (long)t * TP;
@@ -516,14 +522,14 @@ __global__ __launch_bounds__(256, 2) void cn_classes_kernel(CnwArgs a) {
     }
     if (threadIdx.x < TP) {
       const long p = p0 + threadIdx.x;        // (the row arrays are padded)
-      prow[0] = a.fx[p]; prow[1] = a.lse2[p]; prow[2] = a.gp[p]; plab = a.lab[p];
+      prow[0] = a.fx[p]; prow[1] = a.lse2[p]; prow[2] = a.gp[p]; prow[3] = a.hot[p]; plab = a.lab[p];
     }
   };
   if (t0 < t1) load(t0);
   for (int t = t0; t < t1; ++t) {
     __syncthreads();                           // nobody reads the tile before this one
     if (threadIdx.x < TP) {
-      rows[0][threadIdx.x] = prow[0]; rows[1][threadIdx.x] = prow[1]; rows[2][threadIdx.x] = prow[2] * prow[0]; rows[3][threadIdx.x] = prow[2];
+      rows[0][threadIdx.x] = prow[0]; rows[1][threadIdx.x] = prow[1]; rows[2][threadIdx.x] = prow[2] * prow[0]; rows[3][threadIdx.x] = prow[2]; rows[4][threadIdx.x] = prow[3];
       labs[threadIdx.x] = plab;
       const unsigned gb = __float_as_uint(prow[2]) & 0x7FFFFFFFu;
       int e = (gb != 0u && gb < 0x7F800000u && prow[0] > 0.f) ? (int)(gb >> 23) - 126 + (int)(__float_as_uint(prow[0]) >> 23) - 127 : -100000;
@@ -594,11 +600,14 @@ __global__ __launch_bounds__(256, 2) void cn_classes_kernel(CnwArgs a) {
         constexpr bool kG2 = HP == 2 || WP == 2;          // planes of G: one where nothing is fp32
         bool here = false;
         int y4[2][4];
+        float h4[2][4];
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
           const int pr = p0 + tt * 16 + q * 4;
           const float4 f = *reinterpret_cast<const float4*>(&rows[0][pr]), ls = *reinterpret_cast<const float4*>(&rows[1][pr]);
           const int4 yy = *reinterpret_cast<const int4*>(&labs[pr]);
+          const float4 hh = *reinterpret_cast<const float4*>(&rows[4][pr]);
+          h4[tt][0] = hh.x; h4[tt][1] = hh.y; h4[tt][2] = hh.z; h4[tt][3] = hh.w;
           const float ff[4] = {f.x * wl2, f.y * wl2, f.z * wl2, f.w * wl2}, l4[4] = {ls.x, ls.y, ls.z, ls.w};
           y4[tt][0] = yy.x - v0; y4[tt][1] = yy.y - v0; y4[tt][2] = yy.z - v0; y4[tt][3] = yy.w - v0;
 #pragma unroll
@@ -610,11 +619,12 @@ __global__ __launch_bounds__(256, 2) void cn_classes_kernel(CnwArgs a) {
         }
         if (__any(here)) {             // some pixel's label is among this wave's classes
 #pragma unroll
-          for (int tt = 0; tt < 2; ++tt)
+          for (int tt = 0; tt < 2; ++tt) {
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) s[tt][j][r] -= y4[tt][r] - li == j * 16 ? 1.f : 0.f;
+              for (int r = 0; r < 4; ++r) s[tt][j][r] -= y4[tt][r] - li == j * 16 ? h4[tt][r] : 0.f;
+          }
         }
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
@@ -714,7 +724,7 @@ __global__ __launch_bounds__(1024) void cn_join_kernel(const float* __restrict__
 // ------------------------------------------------------------------------------------------------------------------------------ host
 struct CnPlan {
   int KS, nch, Vp, nslots; long P, Pp, wgs; int njw, units, wpx, vblocks, tp, tiles, splits;
-  size_t o_img, o_slots, o_lsum, o_fx, o_lse, o_gp, o_lab, o_dw, o_db, total;
+  size_t o_img, o_slots, o_lsum, o_fx, o_lse, o_gp, o_hot, o_lab, o_dw, o_db, total;
 };
 static CnPlan cn_plan(int N, int C, int V, int HW, int types, bool grad) {
   CnPlan k{};
@@ -736,7 +746,7 @@ static CnPlan cn_plan(int N, int C, int V, int HW, int types, bool grad) {
   k.o_img = take((size_t)k.nch * ((size_t)((types & 2) ? 1 : 2) * 64 * kW * 2 + 1024));
   k.o_slots = take(kCnPrep * 4); k.o_lsum = take((size_t)k.wgs * 8);
   if (grad) {
-    k.o_fx = take(k.Pp * 4); k.o_lse = take(k.Pp * 4); k.o_gp = take(k.Pp * 4); k.o_lab = take(k.Pp * 4);
+    k.o_fx = take(k.Pp * 4); k.o_lse = take(k.Pp * 4); k.o_gp = take(k.Pp * 4); k.o_hot = take(k.Pp * 4); k.o_lab = take(k.Pp * 4);
     k.o_dw = take((size_t)k.splits * k.wpx * k.Vp * kW * 4);
     k.o_db = take((size_t)k.splits * k.wpx * k.Vp * 4);
   }
@@ -766,7 +776,7 @@ static int cn_run(const CeArgs& a, const CnPlan& k) {
   p.h = a.h; p.w = a.w; p.labels = a.labels; p.img = ws + k.o_img; p.slots = slots; p.nslots = k.nslots;
   p.nll = a.nll; p.lse_out = a.lse; p.lse_in = a.lse_in; p.grad = a.grad; p.scale_dev = a.scale_dev; p.sign = a.sign; p.mean_valid = a.mean_valid; p.drop = need_grad ? 1 : 0;
   p.dh = a.dh; p.lsum = a.loss != nullptr ? (double*)(ws + k.o_lsum) : nullptr;
-  if (need_dw) { p.fx = (float*)(ws + k.o_fx); p.lse2 = (float*)(ws + k.o_lse); p.gp = (float*)(ws + k.o_gp); p.lab = (int*)(ws + k.o_lab); }
+  if (need_dw) { p.fx = (float*)(ws + k.o_fx); p.lse2 = (float*)(ws + k.o_lse); p.gp = (float*)(ws + k.o_gp); p.hot = (float*)(ws + k.o_hot); p.lab = (int*)(ws + k.o_lab); }
   p.full = a.C == CnW<KS>::kW && (size_t)a.N * a.HW * a.C * sizeof(HT) <= 0xFFFFFFFFu;
   p.w_vec = a.C % 4 == 0 && (reinterpret_cast<uintptr_t>(a.w) & (4 * sizeof(WT) - 1)) == 0;
   p.P = k.P; p.C = a.C; p.HW = a.HW; p.V = a.V; p.nch = k.nch;
@@ -776,7 +786,7 @@ static int cn_run(const CeArgs& a, const CnPlan& k) {
   if (int e = check_launch("class_ce_pixels")) return e;
   if (need_dw) {
     CnwArgs c{};
-    c.h = a.h; c.img = p.img; c.fx = p.fx; c.lse2 = p.lse2; c.gp = p.gp; c.lab = p.lab;
+    c.h = a.h; c.img = p.img; c.fx = p.fx; c.lse2 = p.lse2; c.gp = p.gp; c.hot = p.hot; c.lab = p.lab;
     c.dwp = (float*)(ws + k.o_dw); c.dbp = (float*)(ws + k.o_db); c.dw_split = (size_t)k.Vp * kW; c.db_split = k.Vp;
     c.P = k.P; c.C = a.C; c.HW = a.HW; c.V = a.V; c.units = k.units; c.wpx = k.wpx; c.splits = k.splits; c.tiles = k.tiles;
     const dim3 gw((unsigned)k.splits, (unsigned)k.vblocks);

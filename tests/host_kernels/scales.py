@@ -2,7 +2,8 @@
 
 Every row of dh and every class of dw is judged by itself, against its own terms m = |G|-magnitudes times the other operand: the error's norm over |m|'s, its median, 99 % quantile
 and maximum over rows (classes).  An element of G is held to 2^-41 g_p at least, so m takes every p as 2^-20 more than it is.  The bar is what the plain form leaves in fp32 on the same input: 4 times its quantile, plus 3 2^-22 (both operands of a product are held to 2^-22, and
-the product of the two low planes is left out), plus 2 2^-24 max|z| log2(e) (z - lse, both rounded at that size, is an exponent).  A bf16 result adds half a step, 2^-8 of the value;
+the product of the two low planes is left out), plus 2 2^-24 max|z| log2(e) where the gradients come from
+a stored lse (z - lse, both rounded at that size, is an exponent; one call for loss and gradients has 2^-22 in its place).  A bf16 result adds half a step, 2^-8 of the value;
 where h and w are both bf16, G has 11 bits: 2^-11."""
 import sys
 
@@ -86,8 +87,12 @@ def main(form):
             fail = [] if own["inside"] else ["inside"]
             for k in a:
                 fail += [k] if not (a[k] <= 4 * c[k] + bar).all() else []
+            if name in ("plain", "confident", "near classes"):          # loss and gradients in one call: no log-sum is rounded in between
+                e1, p1 = (g.exact_ce(h, w, b, lab, hb, wb, False, dtype=t) for t in (np.float64, np.float32))
+                a1, c1 = errors(g.class_ce(lib, h, w, b, lab, hb, wb), e1, bf), errors(p1, e1, {"dh": 0, "dw": 0})
+                fail += ["one call: %s %s" % (k, a1[k]) for k in a1 if not (a1[k] <= 4 * c1[k] + 4 * 2.0 ** -22 + (2.0 ** -11 if hb and wb else 0)).all()]
             bad += len(fail)
-            print(form, name, "bf16" if hb else "fp32", "bf16" if wb else "fp32", *("%s %.1e %.1e %.1e (plain %.1e %.1e %.1e)" % ((k,) + tuple(a[k]) + tuple(c[k])) for k in a), "FAIL" if fail else "",
+            print(form, name, "bf16" if hb else "fp32", "bf16" if wb else "fp32", *("%s %.1e %.1e %.1e (plain %.1e %.1e %.1e)" % ((k,) + tuple(a[k]) + tuple(c[k])) for k in a), "FAIL %s" % fail if fail else "",
                   flush=True)
     print("done" if not bad else "%d outside" % bad, flush=True)
     return bad

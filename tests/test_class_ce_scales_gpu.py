@@ -103,3 +103,19 @@ def test_wide_form(name, hdt, wdt, shape, V):
 @pytest.mark.parametrize("shape,V", [((2, 64, 40, 40), 151), ((1, 16, 50, 37), 104), ((3000, 100), 40)])
 def test_narrow_form(name, hdt, wdt, shape, V):
     check(name, shape, V, hdt, wdt, True)
+
+
+@pytest.mark.parametrize("name", ["plain", "confident", "near classes"])
+@pytest.mark.parametrize("hdt,wdt", [(F, F), (B, F), (B, B)])
+@pytest.mark.parametrize("shape,V", [((256, 136), 700), ((2, 512, 16, 17), 900), ((2, 64, 40, 40), 151), ((1, 16, 50, 37), 104)])
+def test_loss_and_gradients_in_one_call(name, hdt, wdt, shape, V):
+    """No log-sum is stored in between, so the size of the logits does not enter: 4 times plain fp32's own error, plus 4 2^-22 of the terms (both operands, the product of the low planes, G)."""
+    h, w, b, lab, gr = make(name, shape, V, hdt, wdt, True)
+    if name == "confident":
+        hr = rows_of(h).float() + 6 * w.float()[lab.reshape(-1)]
+        h = hr.reshape((shape[0],) + tuple(shape[2:]) + (shape[1],)).movedim(-1, 1).contiguous().to(hdt)
+    _, dh, dw, _ = ops.class_ce(h, w, b, lab)
+    e, plain = definition(h, w, b, lab, gr, torch.float64), definition(h, w, b, lab, gr, F)
+    for k, own, dt in (("dh", rows_of(dh), hdt), ("dw", dw, wdt)):
+        a, c = quantiles(own, e, k, dt == B), quantiles(plain[k], e, k, False)
+        assert (a <= 4 * c + 4 * 2.0 ** -22 + (2.0 ** -11 if hdt == B and wdt == B else 0)).all(), (k, a.tolist(), c.tolist())
