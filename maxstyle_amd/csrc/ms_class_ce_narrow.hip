@@ -10,8 +10,8 @@
 // 8 P V C products, and nothing of size P V is stored.  What a training call waits for is the vector unit: counted over whole kernels, a logit (the padding's included) costs 18 vector
 // instructions in the pixel pass and 15 - 16 in the class pass, 9 where the value alone is asked for, an exp2 among them.  Of the pixel pass's, 5.6 are the loop's exponent, sum and split into
 // planes; the others scale the logit, keep the maximum and pick the label's logit (more of it where labels do not come in regions), or belong to the pixels' load and dh.
-// 1M pixels, 104 classes, 16 channels: pixel pass 76 us, every cycle of the vector unit taken; class pass 85, 75 % of them.  256 classes, 64 channels (bf16): 231 and 216 us, 71 % and 63 %,
-// the matrix cores 33 % and 26 %.  The value alone, 295k x 1000 classes x 64: 130 us, 83 % and 43 %.
+// 1M pixels, 104 classes, 16 channels: pixel pass 81 us, every cycle of the vector unit taken; class pass 85, 75 % of them.  256 classes, 64 channels (bf16): 231 and 225 us, 71 % and 60 %,
+// the matrix cores 33 % and 25 %.  The value alone, 295k x 1000 classes x 64: 133 us, 83 % and 43 %.
 #include <algorithm>
 #include <type_traits>
 #include "ms_class_ce.h"
