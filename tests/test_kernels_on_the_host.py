@@ -19,7 +19,7 @@ def child(args):
     return subprocess.run([sys.executable] + args, cwd=HERE, env=ENV, capture_output=True, text=True, timeout=900)
 
 
-@pytest.mark.parametrize("which,seed,count", [("class_ce", 1, 240), ("class_ce_pieces", 2, 120), ("logit_ce", 1, 150), ("act8", 1, 100)])
+@pytest.mark.parametrize("which,seed,count", [("class_ce", 3, 120), ("class_ce", 1, 60), ("class_ce_pieces", 2, 80), ("logit_ce", 1, 100), ("act8", 1, 60)])
 def test_every_access_is_inside_its_buffer(which, seed, count):
     r = child(["sweep.py", which, str(seed), str(count)])
     assert r.returncode == 0 and r.stdout.endswith("done\n"), (r.returncode, r.stdout[-400:], r.stderr[-800:])
